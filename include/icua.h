@@ -219,6 +219,103 @@ int icua_quantize_noalloc(int fmt, const float* d_m, int rows, int cols, void* d
 int icua_quantize_bench(int fmt, const float* d_m, int rows, int cols, void* d_codes, void* d_sb, int iters,
                         double* avg_us);
 
+/* ---- paged K/V caches: several sequences in one pool of pages, on device buffers ----
+ * The reference has one contiguous cache of one session (kc/vc, Engine.swift:110-112); these operators
+ * serve batches of sequences of any lengths, which may share pages (a common prompt prefix).
+ *
+ * A pool holds K and V of one layer as row-major .icua matrices of 128 columns (the head dimension),
+ * rows [page][KV head][slot in the page]: fp16 values (ICUA_FMT_F16), or q8 codes and their fp16
+ * scales, four a row (ICUA_FMT_Q8); icua_dequant reads them as such.  A pool of one page of max_ctx
+ * slots has the layout of the engine's cache.  Pool slot numbers are page * page_slots + slot.
+ *
+ * The calls enqueue on `stream` (a hipStream_t; NULL: the null stream) and return without waiting, so
+ * that a layer's calls follow each other; they allocate nothing, keep nothing and can be captured
+ * into a graph.  Buffers and stream belong to the current device.  Arguments are checked before
+ * anything is enqueued.  What lies in device memory (page tables, lengths, positions, slots) cannot
+ * be checked by the host: numbers that point outside the pool or the tables are never followed (what
+ * happens to their rows is said at each call).  Row strides are in values and multiples of 8; value
+ * buffers are aligned to 16 bytes. */
+enum { ICUA_TYPE_F32 = 0, ICUA_TYPE_F16 = 1 };
+
+typedef struct {
+    int32_t fmt;             /* ICUA_FMT_F16 or ICUA_FMT_Q8 */
+    int32_t n_kv;            /* KV heads, 1..1024 */
+    int32_t page_slots;      /* a positive multiple of 16 */
+    int32_t n_pages;         /* n_pages * n_kv * page_slots < 2^31 */
+    void *k, *v;             /* fp16 values or int8 codes */
+    void *k_scales, *v_scales; /* q8: fp16 [rows][4]; else NULL */
+} icua_pages_t;
+
+/* Writes n_tokens tokens to their slots, after the norm and the rotation of a layer's attention input
+ * (k_qk_norm_rope, Shaders.swift:871-923): y = x / sqrt(mean(x^2) + eps) * norm for each query and key
+ * head (norm NULL: y = x), then the rotation of the first rot_dim values by the table row of the
+ * token's position, pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`.  Queries go to q,
+ * keys and values to the pool: rounded to fp16, or quantised with the bytes that icua_quantize gives.
+ * Arithmetic is fp32.  Values are as fp16 can hold them (q8: up to 127 * 65504).
+ * A token whose slot is outside the pool (-1, say) has its queries made and is not stored; one whose
+ * position is outside the table gets NaN queries and is not stored.  The slots of one call differ. */
+typedef struct {
+    int32_t type, q_type;    /* ICUA_TYPE_* of qkv and of q */
+    int32_t n_tokens;        /* 0: nothing to do */
+    int32_t n_heads;         /* query heads; 0: keys and values alone */
+    const void* qkv;         /* [n_tokens] rows: n_heads query, n_kv key and n_kv value heads of 128 */
+    int64_t qkv_stride;      /* 0: dense */
+    void* q;                 /* [n_tokens] rows of n_heads heads */
+    int64_t q_stride;        /* 0: dense */
+    const float *q_norm, *k_norm; /* [128] or NULL */
+    float eps;
+    const float* rope;       /* [rope_rows][rot_dim / 2] (cos, sin) */
+    int32_t rope_rows;
+    int32_t rot_dim;         /* a multiple of 8 up to 128; 0: no rotation */
+    int32_t interleaved;
+    const int32_t* pos;      /* [n_tokens] table rows (unused without rotation) */
+    const int32_t* slots;    /* [n_tokens] pool slots */
+} icua_paged_store_t;
+int icua_paged_store(const icua_pages_t* pages, const icua_paged_store_t* args, void* stream);
+
+/* Attention of every sequence's new tokens over its slots, causal (k_attention and k_prefill_attn,
+ * Shaders.swift:1101-1289, over a batch): sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of q
+ * and kv_len[s] slots in the pages of row s of the table, the new tokens' K/V included; token i of m
+ * sees slots 0 .. kv_len - m + i, and a token that sees none gets zeros.  Query head h reads KV head
+ * h * n_kv / n_heads.  Rows of q behind the last sequence's keep their outputs as they are.
+ * fp32 queries are computed to fp32 accuracy (fp16 hi + lo operands), fp16 ones with fp16 operands;
+ * scores, softmax and sums are fp32.  max_q and max_kv bound the sequences' new tokens and slots (0:
+ * n_tokens, table_width * page_slots) and decide the launch with n_seqs and n_tokens; slots past
+ * max_kv are not read, and tokens past max_q have no defined output.  Slots of a page number outside
+ * the pool take no part.  `work` holds icua_paged_attention_work() bytes, written and read within the
+ * call: calls that may run at the same time (other streams, captured graphs) each have their own. */
+typedef struct {
+    int32_t type;            /* ICUA_TYPE_* of q and out */
+    int32_t n_heads;         /* a multiple of n_kv, at most 16 a KV head */
+    int32_t n_seqs, n_tokens, max_q, max_kv;
+    float scale;             /* 0: 1 / sqrt(128) */
+    const void* q;           /* [n_tokens] rows of n_heads heads of 128 */
+    int64_t q_stride;        /* 0: dense */
+    void* out;               /* the same shape */
+    int64_t out_stride;      /* 0: dense */
+    const int32_t* q_start;  /* [n_seqs + 1], rising */
+    const int32_t* kv_len;   /* [n_seqs] */
+    const int32_t* tables;   /* [n_seqs][table_width] page numbers */
+    int32_t table_width;
+    void* work;
+    size_t work_bytes;
+} icua_paged_attention_t;
+int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t* args, void* stream);
+/* Bytes of `work` for a call with exactly these sizes (the pointers in args are not looked at). */
+int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, size_t* bytes);
+
+/* Reads rows of the pool back: for row r, KV head g the 128 values at pool slot slots[r], as fp32 (the
+ * exact scale * code of q8) or fp16 (rounded), to k and v (either NULL) + r * token_stride + g *
+ * head_stride (both 0: [n_rows][n_kv][128]).  Rows whose slot is outside the pool keep their outputs. */
+typedef struct {
+    int32_t type;            /* ICUA_TYPE_* of k and v */
+    int32_t n_rows;
+    const int32_t* slots;    /* [n_rows] */
+    void *k, *v;
+    int64_t token_stride, head_stride;
+} icua_paged_load_t;
+int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

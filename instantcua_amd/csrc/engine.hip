@@ -1696,4 +1696,190 @@ int icua_dequant(int fmt, const void* d_codes, const void* d_sb, int K, int row0
     return 0;
 }
 
+// ---- paged K/V caches
+
+// Whether a value buffer is set and aligned for 16-byte accesses.
+static bool buffer_ok(const void* p) { return p && (uintptr_t)p % 16 == 0; }
+
+static int pages_check(const icua_pages_t* p, PageMap& m, bool buffers) {
+    if (!p) return fail("paged: null argument");
+    if (p->fmt != FMT_F16 && p->fmt != FMT_Q8) return fail("paged: the pool's format must be f16 (0) or q8 (1)");
+    if (p->n_kv < 1 || p->n_kv > 1024) return fail("paged: n_kv must be in 1..1024");
+    if (p->page_slots < 1 || p->page_slots % PAGED_TILE)
+        return fail("paged: page_slots must be a positive multiple of " + std::to_string(PAGED_TILE));
+    if (p->n_pages < 1) return fail("paged: the pool has no pages");
+    if ((int64_t)p->n_kv * p->page_slots > INT32_MAX / p->n_pages) return fail("paged: the pool has 2^31 rows or more");
+    m = PageMap{p->n_pages, p->n_kv, p->page_slots};
+    if (!buffers) return 0;
+    if (!buffer_ok(p->k) || !buffer_ok(p->v)) return fail("paged: the pool's buffers must be set and aligned to 16 bytes");
+    if (p->fmt == FMT_Q8 && (!buffer_ok(p->k_scales) || !buffer_ok(p->v_scales)))
+        return fail("paged: the pool's scales must be set and aligned to 16 bytes");
+    return 0;
+}
+
+// A row stride of `width` values (0: dense).
+static int stride_check(const char* what, int64_t& stride, int64_t width) {
+    if (stride == 0) stride = width;
+    if (stride < width || stride % 8) return fail(std::string("paged: ") + what + " must be at least a row and a multiple of 8 values");
+    return 0;
+}
+
+static bool type_ok(int t) { return t == TYPE_F32 || t == TYPE_F16; }
+
+// Work goes to the current device: a stream of another one is refused.
+static int stream_check(void* stream) {
+    int dev = 0, sdev = 0;
+    if (!stream) return 0;
+    HIPCK(hipGetDevice(&dev));
+    HIPCK(hipStreamGetDevice((hipStream_t)stream, &sdev));
+    if (dev != sdev) return fail("paged: the stream belongs to another device than the current one");
+    return 0;
+}
+
+int icua_paged_store(const icua_pages_t* pages, const icua_paged_store_t* args, void* stream) {
+    PagedStoreArgs a{};
+    if (!args) return fail("paged_store: null argument");
+    if (pages_check(pages, a.map, true)) return -1;
+    if (!type_ok(args->type) || !type_ok(args->q_type)) return fail("paged_store: bad type");
+    if (args->n_tokens < 0) return fail("paged_store: negative n_tokens");
+    if (args->n_heads < 0 || args->n_heads > 16384) return fail("paged_store: n_heads must be in 0..16384");
+    a.n_tokens = args->n_tokens;
+    a.n_heads = args->n_heads;
+    a.qkv_stride = args->qkv_stride;
+    a.q_stride = args->q_stride;
+    if (stride_check("qkv_stride", a.qkv_stride, (int64_t)(a.n_heads + 2 * a.map.n_kv) * HD)) return -1;
+    if (stride_check("q_stride", a.q_stride, (int64_t)a.n_heads * HD)) return -1;
+    if (!(args->eps >= 0.f)) return fail("paged_store: eps must not be negative");
+    if (args->rot_dim < 0 || args->rot_dim > HD || args->rot_dim % 8) return fail("paged_store: rot_dim must be a multiple of 8 up to 128");
+    if (args->n_tokens == 0) return 0;
+    if (!buffer_ok(args->qkv)) return fail("paged_store: qkv must be set and aligned to 16 bytes");
+    if (args->n_heads && !buffer_ok(args->q)) return fail("paged_store: q must be set and aligned to 16 bytes");
+    if (args->q_norm && !buffer_ok(args->q_norm)) return fail("paged_store: q_norm must be aligned to 16 bytes");
+    if (args->k_norm && !buffer_ok(args->k_norm)) return fail("paged_store: k_norm must be aligned to 16 bytes");
+    if (!args->slots) return fail("paged_store: slots must be set");
+    if (args->rot_dim) {
+        if (!buffer_ok(args->rope) || !args->pos) return fail("paged_store: a rotation needs its table, aligned to 16 bytes, and positions");
+        if (args->rope_rows < 1) return fail("paged_store: the rotation's table is empty");
+    }
+    if (stream_check(stream)) return -1;
+    a.k = pages->k;
+    a.v = pages->v;
+    a.k_sb = pages->k_scales;
+    a.v_sb = pages->v_scales;
+    a.rot = args->rot_dim;
+    a.interleaved = args->interleaved != 0;
+    a.rope_rows = args->rope_rows;
+    a.eps = args->eps;
+    a.qkv = args->qkv;
+    a.q = args->q;
+    a.q_norm = args->q_norm;
+    a.k_norm = args->k_norm;
+    a.rope = args->rope;
+    a.pos = args->rot_dim ? args->pos : nullptr;
+    a.slots = args->slots;
+    HIPCK(launch_paged_store(pages->fmt, args->type, args->q_type, a, (hipStream_t)stream));
+    return 0;
+}
+
+// Sizes of an attention call: checked, with the defaults filled in.
+static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention_t* args, bool buffers, PagedAttnArgs& a,
+                           PagedPlan& plan) {
+    if (!args) return fail("paged_attention: null argument");
+    if (pages_check(pages, a.map, buffers)) return -1;
+    if (!type_ok(args->type)) return fail("paged_attention: bad type");
+    if (args->n_heads < 1 || args->n_heads % a.map.n_kv || args->n_heads / a.map.n_kv > 16)
+        return fail("paged_attention: n_heads must be a multiple of n_kv, at most 16 for each");
+    if (args->n_seqs < 0 || args->n_tokens < 0 || args->max_q < 0 || args->max_kv < 0)
+        return fail("paged_attention: negative size");
+    if (args->n_seqs > (1 << 20) || args->n_tokens > (1 << 24)) return fail("paged_attention: more than 2^20 sequences or 2^24 tokens");
+    if (args->table_width < 1 || args->table_width > INT32_MAX / 2 / a.map.page_slots)
+        return fail("paged_attention: table_width must be positive and its pages hold fewer than 2^30 slots");
+    const int slots = args->table_width * a.map.page_slots;
+    a.n_heads = args->n_heads;
+    a.n_seqs = args->n_seqs;
+    a.n_tokens = args->n_tokens;
+    a.table_width = args->table_width;
+    a.max_kv = args->max_kv ? std::min(args->max_kv, slots) : slots;
+    const int max_q = args->max_q ? std::min(args->max_q, args->n_tokens) : args->n_tokens;
+    plan = paged_plan(a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv);
+    return 0;
+}
+static size_t plan_bytes(const PagedPlan& p) { return (p.part_floats + p.ml_floats) * sizeof(float); }
+
+int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, size_t* bytes) {
+    PagedAttnArgs a{};
+    PagedPlan plan{};
+    if (!bytes) return fail("paged_attention_work: null argument");
+    if (attention_sizes(pages, args, false, a, plan)) return -1;
+    *bytes = plan_bytes(plan);
+    return 0;
+}
+
+int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t* args, void* stream) {
+    PagedAttnArgs a{};
+    PagedPlan plan{};
+    if (attention_sizes(pages, args, true, a, plan)) return -1;
+    a.q_stride = args->q_stride;
+    a.out_stride = args->out_stride;
+    if (stride_check("q_stride", a.q_stride, (int64_t)a.n_heads * HD)) return -1;
+    if (stride_check("out_stride", a.out_stride, (int64_t)a.n_heads * HD)) return -1;
+    if (!std::isfinite(args->scale)) return fail("paged_attention: scale must be finite");
+    if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
+    if (!buffer_ok(args->q) || !buffer_ok(args->out)) return fail("paged_attention: q and out must be set and aligned to 16 bytes");
+    if (!args->q_start || !args->kv_len || !args->tables) return fail("paged_attention: q_start, kv_len and tables must be set");
+    const size_t need = plan_bytes(plan);
+    if (need && (!buffer_ok(args->work) || args->work_bytes < need))
+        return fail("paged_attention: work must hold " + std::to_string(need) + " bytes, aligned to 16");
+    if (stream_check(stream)) return -1;
+    a.k = pages->k;
+    a.v = pages->v;
+    a.k_sb = pages->k_scales;
+    a.v_sb = pages->v_scales;
+    a.scale = args->scale == 0.f ? 1.0f / sqrtf((float)HD) : args->scale;
+    a.q = args->q;
+    a.out = args->out;
+    a.q_start = args->q_start;
+    a.kv_len = args->kv_len;
+    a.tables = args->tables;
+    a.one_tile = plan.one_tile;
+    a.tiles = plan.tiles;
+    a.nsplit = plan.nsplit;
+    a.chunk = plan.chunk;
+    a.part = (float*)args->work;
+    a.part_ml = (float2*)(a.part + plan.part_floats);
+    HIPCK(launch_paged_attention(pages->fmt, args->type, a, (hipStream_t)stream));
+    return 0;
+}
+
+int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, void* stream) {
+    PagedLoadArgs a{};
+    if (!args) return fail("paged_load: null argument");
+    if (pages_check(pages, a.map, true)) return -1;
+    if (!type_ok(args->type)) return fail("paged_load: bad type");
+    if (args->n_rows < 0) return fail("paged_load: negative n_rows");
+    a.token_stride = args->token_stride;
+    a.head_stride = args->head_stride;
+    if (a.token_stride == 0 && a.head_stride == 0) {
+        a.token_stride = (int64_t)a.map.n_kv * HD;
+        a.head_stride = HD;
+    }
+    if (a.token_stride < HD || a.head_stride < HD || a.token_stride % 8 || a.head_stride % 8)
+        return fail("paged_load: strides must be at least 128 and multiples of 8 values");
+    if (args->n_rows == 0 || (!args->k && !args->v)) return 0;
+    if ((args->k && !buffer_ok(args->k)) || (args->v && !buffer_ok(args->v)))
+        return fail("paged_load: k and v must be aligned to 16 bytes");
+    if (!args->slots) return fail("paged_load: slots must be set");
+    if (stream_check(stream)) return -1;
+    a.k = pages->k;
+    a.v = pages->v;
+    a.k_sb = pages->k_scales;
+    a.v_sb = pages->v_scales;
+    a.n_rows = args->n_rows;
+    a.slots = args->slots;
+    a.k_out = args->k;
+    a.v_out = args->v;
+    HIPCK(launch_paged_load(pages->fmt, args->type, a, (hipStream_t)stream));
+    return 0;
+}
+
 }  // extern "C"

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "icua_paged.h"
 #include "icua_shared.h"
 
 namespace icua {
@@ -214,6 +215,60 @@ hipError_t launch_quant(int fmt, const float* m, int64_t rows, int64_t cols, voi
 constexpr int64_t QUANT_SCRATCH_GROUPS = (int64_t)8 << 20;
 constexpr int QUANT_MAX_DEVICES = 64;
 hipError_t quant_scratch(uint8_t** out);
+
+// ---- Operators on paged K/V caches (paged.hip); the arguments have been checked by the caller.
+struct PagedStoreArgs {
+    PageMap map;
+    void *k, *v, *k_sb, *v_sb;      // the pool: rows [page][KV head][slot] of 128 values (icua_paged.h)
+    int n_tokens, n_heads, rot, interleaved, rope_rows;
+    float eps;
+    const void* qkv;                // [n_tokens] rows of (n_heads + 2 n_kv) 128 values, qkv_stride apart
+    int64_t qkv_stride;
+    void* q;                        // [n_tokens] rows of n_heads 128 values, q_stride apart
+    int64_t q_stride;
+    const float *q_norm, *k_norm;   // [128] or null
+    const float* rope;              // [rope_rows][rot / 2] (cos, sin)
+    const int32_t *pos, *slots;     // [n_tokens]
+};
+hipError_t launch_paged_store(int fmt, int type, int q_type, const PagedStoreArgs& a, hipStream_t s);
+
+struct PagedLoadArgs {
+    PageMap map;
+    const void *k, *v, *k_sb, *v_sb;
+    int n_rows;
+    const int32_t* slots;           // [n_rows]
+    void *k_out, *v_out;            // either may be null
+    int64_t token_stride, head_stride;
+};
+hipError_t launch_paged_load(int fmt, int type, const PagedLoadArgs& a, hipStream_t s);
+
+// How a call's rows and slots are dealt to workgroups, from its bounds alone (the lengths themselves are
+// in device memory).
+struct PagedPlan {
+    int one_tile;                   // every sequence's rows of a KV head fit one tile of 16
+    int tiles;                      // upper bound of the row tiles
+    int nsplit, chunk;              // slots are split in nsplit ranges of chunk slots
+    size_t part_floats, ml_floats;  // partial rows and their (maximum, denominator) pairs, nsplit > 1
+};
+constexpr int PAGED_MAX_SPLITS = 64;
+PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv);
+struct PagedAttnArgs {
+    PageMap map;
+    const void *k, *v, *k_sb, *v_sb;
+    int n_heads, n_seqs, n_tokens, table_width, max_kv;
+    float scale;
+    const void* q;                  // [n_tokens] rows of n_heads 128 values
+    int64_t q_stride;
+    void* out;
+    int64_t out_stride;
+    const int32_t *q_start;         // [n_seqs + 1] first token of every sequence
+    const int32_t *kv_len;          // [n_seqs] slots, the new tokens' included
+    const int32_t* tables;          // [n_seqs][table_width] pages
+    int one_tile, tiles, nsplit, chunk;
+    float* part;                    // [n_tokens][n_heads][nsplit][128]
+    float2* part_ml;                // [n_tokens][n_heads][nsplit]
+};
+hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s);
 
 // Vision tower (ModelFile.swift:31-45): dimensions, weights, work buffers.
 constexpr int VH = 1024, VFF = 4096, VNH = 16, VHD = 64, VQKV = 3072, VPATCH = 768, MH = 4096;

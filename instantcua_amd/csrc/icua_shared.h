@@ -23,6 +23,8 @@ constexpr int MAXM = 8;
 constexpr int LMH_WAVES = 1024;
 
 enum WeightFormat { FMT_F16 = 0, FMT_Q8 = 1, FMT_Q4 = 2 };
+// Activations of the operators on paged caches.
+enum ActivationType { TYPE_F32 = 0, TYPE_F16 = 1 };
 
 // Decode control block (Shaders.swift:41-54).  The first twelve fields keep the reference
 // layout; the rest are additions of this engine.
