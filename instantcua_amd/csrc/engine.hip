@@ -1841,10 +1841,10 @@ int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t
     a.q_start = args->q_start;
     a.kv_len = args->kv_len;
     a.tables = args->tables;
-    a.one_tile = plan.one_tile;
+    a.rows = plan.rows;
+    a.big = plan.big;
     a.tiles = plan.tiles;
-    a.nsplit = plan.nsplit;
-    a.chunk = plan.chunk;
+    a.part_splits = plan.part_splits;
     a.part = (float*)args->work;
     a.part_ml = (float2*)(a.part + plan.part_floats);
     HIPCK(launch_paged_attention(pages->fmt, args->type, a, (hipStream_t)stream));

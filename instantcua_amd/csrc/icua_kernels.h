@@ -244,11 +244,14 @@ hipError_t launch_paged_load(int fmt, int type, const PagedLoadArgs& a, hipStrea
 
 // How a call's rows and slots are dealt to workgroups, from its bounds alone (the lengths themselves are
 // in device memory).
+struct PagedSplit {
+    int n, chunk;                   // a sequence's slots in n ranges of chunk slots
+};
 struct PagedPlan {
-    int one_tile;                   // every sequence's rows of a KV head fit one tile of 16
-    int tiles;                      // upper bound of the row tiles
-    int nsplit, chunk;              // slots are split in nsplit ranges of chunk slots
-    size_t part_floats, ml_floats;  // partial rows and their (maximum, denominator) pairs, nsplit > 1
+    PagedSplit rows, big;           // for sequences of at most 16 query rows a KV head, and of more
+    int tiles;                      // upper bound of the 128-row tiles of the latter (0: none)
+    int part_splits;                // ranges of a row's partials, > 1 if any sequence's slots are split
+    size_t part_floats, ml_floats;  // partial rows and their (maximum, denominator) pairs
 };
 constexpr int PAGED_MAX_SPLITS = 64;
 PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv);
@@ -264,9 +267,10 @@ struct PagedAttnArgs {
     const int32_t *q_start;         // [n_seqs + 1] first token of every sequence
     const int32_t *kv_len;          // [n_seqs] slots, the new tokens' included
     const int32_t* tables;          // [n_seqs][table_width] pages
-    int one_tile, tiles, nsplit, chunk;
-    float* part;                    // [n_tokens][n_heads][nsplit][128]
-    float2* part_ml;                // [n_tokens][n_heads][nsplit]
+    PagedSplit rows, big;
+    int tiles, part_splits;
+    float* part;                    // [n_tokens][n_heads][part_splits][128]
+    float2* part_ml;                // [n_tokens][n_heads][part_splits]
 };
 hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s);
 

@@ -4,6 +4,7 @@
 // rows [page][KV head][slot]: a (page, head)'s slots are contiguous, so a 16-slot tile is one run of
 // 4 KiB (fp16) or 2 KiB of codes and 128 bytes of scales (q8).
 #include <algorithm>
+#include <type_traits>
 
 #include "icua_device.h"
 #include "icua_kernels.h"
@@ -199,6 +200,16 @@ __global__ __launch_bounds__(256) void paged_load_kernel(PagedLoadArgs a) {
 
 constexpr float P_SHIFT = 15.0f;
 
+// Max over the lanes l and l ^ 32.
+__device__ __forceinline__ float max_x2(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
+    return fmaxf(as_f32(r[0]), as_f32(r[1]));
+}
+// The power of two that scales a query row with this largest magnitude.
+__device__ __forceinline__ int query_shift(float amax) {
+    return amax > 0.f && amax < __builtin_inff() ? 10 - __builtin_amdgcn_frexp_expf(amax) : 0;
+}
+
 // The query rows of a workgroup's tile: which token and head a column stands for.
 struct RowOf {
     int t;     // token of the call, -1: no such row
@@ -235,7 +246,7 @@ __device__ __forceinline__ Query<TYPE> load_query(const PagedAttnArgs& a, const 
             for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
         }
         amax = max_x4(amax);
-        const int k2 = amax > 0.f && amax < __builtin_inff() ? 10 - __builtin_amdgcn_frexp_expf(amax) : 0;
+        const int k2 = query_shift(amax);
         y.c = ldexpf(y.c, -k2);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -306,6 +317,22 @@ __device__ __forceinline__ void load_v(const PagedAttnArgs& a, int row, int lane
     }
 }
 
+// Four int8 codes as exact fp16 values: code + 128 under the exponent of 1024 is 1152 + code.
+__device__ __forceinline__ void codes_h2(uint32_t w, f16x2 y[2]) {
+    const uint32_t u = w ^ 0x80808080u;
+    const f16x2 bias = {(f16)1152.f, (f16)1152.f};
+    y[0] = as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x05010400u)) - bias;
+    y[1] = as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x05030402u)) - bias;
+}
+
+// Replaces values that are no numbers by finite ones; `odd` is not zero if there were any.
+__device__ __forceinline__ void keep_finite(v8h& v, uint32_t& odd) {
+    const v8h top = (v8h)(f16)65504.f, fin = __builtin_elementwise_max(__builtin_elementwise_min(v, top), -top);
+    const u32x4 d = __builtin_bit_cast(u32x4, v) ^ __builtin_bit_cast(u32x4, fin);
+    odd |= d[0] | d[1] | d[2] | d[3];
+    v = fin;
+}
+
 // Eight int8 codes as exact fp16 values.
 __device__ __forceinline__ v8h codes_f16(u32x2 c) {
     v8h y;
@@ -372,6 +399,13 @@ __device__ __forceinline__ void v_operands(const VTile<FMT>* t, VOps<TYPE, FMT>&
     }
 }
 
+// Value d of a row of V, as the products take it.
+template <int FMT>
+__device__ __forceinline__ float row_value(const PagedAttnArgs& a, int64_t row, int d) {
+    if constexpr (FMT == FMT_F16) return (float)((const f16*)a.v)[row * HD + d];
+    return (float)(f16)(h2f(((const uint16_t*)a.v_sb)[row * NG + d / QG]) * (float)((const int8_t*)a.v)[row * HD + d]);
+}
+
 template <int TYPE, int FMT>
 __device__ __forceinline__ f32x4 pv(const VOps<TYPE, FMT>& v, int dt, v8h ph, v8h pl, f32x4 c) {
     c = mfma(v.hi[dt], ph, c);
@@ -380,10 +414,10 @@ __device__ __forceinline__ f32x4 pv(const VOps<TYPE, FMT>& v, int dt, v8h ph, v8
     return c;
 }
 
-// Query rows in tiles of 16: a workgroup has one tile of a (sequence, KV head) and a range of its
-// slots, its four waves take 32-slot steps of it in turn and join through LDS.  K and V go from memory to
-// registers: each is used by one tile alone.  Bound by memory for single tokens and drafts.
-constexpr int ROWS_STEP = 32, ROWS_SUB = WAVE * PAGED_TILE;
+// Sequences with at most 16 query rows a KV head (single tokens, drafts): a workgroup has a (sequence, KV
+// head) and a range of its slots, its four waves take 32-slot steps of it in turn and join through LDS.
+// K and V go from memory to registers: each is used by one tile alone.  Bound by memory.
+constexpr int ROWS_TILE = 16, ROWS_STEP = 32, ROWS_SUB = WAVE * PAGED_TILE;
 
 template <int TYPE, int FMT>
 __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
@@ -391,40 +425,13 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r16 = lane & 15;
     const int g = blockIdx.y, split = blockIdx.z, group = a.n_heads / a.map.n_kv;
-    // The sequence and tile of this workgroup: a sequence has ceil(n_q group / 16) tiles.
-    int s = 0, tile = blockIdx.x;
-    if (a.one_tile) {
-        s = tile;
-        tile = 0;
-    } else {
-        for (;; s += WAVE) {
-            if (s >= a.n_seqs) return;
-            int n = 0;
-            if (s + lane < a.n_seqs)
-                n = (seq_span(a.q_start, a.kv_len, s + lane, a.n_tokens, a.max_kv).n_q * group + 15) / 16;
-            int end = n;
-#pragma unroll
-            for (int o = 1; o < WAVE; o <<= 1) {
-                const int x = __shfl_up(end, o);
-                if (lane >= o) end += x;
-            }
-            const uint64_t past = __ballot(end > tile);
-            if (past) {
-                const int first = __ffsll((unsigned long long)past) - 1;
-                tile -= __shfl(end - n, first);
-                s += first;
-                break;
-            }
-            tile -= __shfl(end, 63);
-        }
-    }
+    const int s = blockIdx.x;
     const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
-    if (tile * 16 >= sp.n_q * group) return;
-    const RowOf row = row_of(sp, tile * 16 + r16, group, g);
-    // Slots that some row of the tile sees: 0 .. lim - 1; all of them see those up to `all`.
-    const int i0 = tile * 16 / group, i1 = min(sp.n_q - 1, (tile * 16 + 15) / group);
-    const int lim = max(0, sp.n_kv - sp.n_q + i1 + 1), all = sp.n_kv - sp.n_q + i0;
-    const int c0 = min(lim, split * a.chunk), c1 = min(lim, c0 + a.chunk);
+    if (sp.n_q == 0 || sp.n_q * group > ROWS_TILE) return;  // the others are paged_chunk_kernel's
+    const RowOf row = row_of(sp, r16, group, g);
+    // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
+    const int lim = sp.n_kv, all = sp.n_kv - sp.n_q;
+    const int c0 = min(lim, split * a.rows.chunk), c1 = min(lim, c0 + a.rows.chunk);
 
     const Query<TYPE> y = load_query<TYPE>(a, row, q);
     f32x4 O[8];
@@ -488,39 +495,30 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
             v_operands<TYPE, FMT>(vt, vo);
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) O[dt] *= corr;
-            // Slots that some rows see and others do not: a value there that is no number must not
-            // reach the rows that do not see it, so each such step is checked, and where one is found the
-            // slots are added one by one to the rows that see them.
-            bool plain = true;
-            if (at + ROWS_STEP - 1 > all) {
-                bool finite = true;
+            // Slots that some rows see and others do not: values there that are no numbers are kept out of the
+            // products and go to the rows that see them.
+            uint32_t odd = 0;
+            if (at + ROWS_STEP - 1 > all)
 #pragma unroll
-                for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) finite &= __builtin_fabsf16(vo.hi[dt][j]) <= (f16)65504.f;
-                plain = __ballot(!finite) == 0;
-            }
-            if (plain) {
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt) O[dt] = pv<TYPE, FMT>(vo, dt, ph, pl, O[dt]);
-            } else {
-                for (int j = 0; j < ROWS_STEP; ++j) {
-                    const bool sees = at + j <= row.last;
-#pragma unroll
-                    for (int dt = 0; dt < 8; ++dt) {
-                        VOps<TYPE, FMT> one;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const bool mine = 16 * (e / 4) + 4 * q + e % 4 == j;
-                            one.hi[dt][e] = mine ? vo.hi[dt][e] : (f16)0.f;
-                            if constexpr (VOps<TYPE, FMT>::LO) one.lo[dt][e] = mine ? vo.lo[dt][e] : (f16)0.f;
-                        }
-                        const f32x4 c = pv<TYPE, FMT>(one, dt, ph, pl, O[dt]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) O[dt][i] = sees ? c[i] : O[dt][i];
-                    }
+                for (int dt = 0; dt < 8; ++dt) {
+                    keep_finite(vo.hi[dt], odd);
+                    if constexpr (VOps<TYPE, FMT>::LO) keep_finite(vo.lo[dt], odd);
                 }
-            }
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) O[dt] = pv<TYPE, FMT>(vo, dt, ph, pl, O[dt]);
+            if (__ballot(odd != 0))
+                for (int j = 0; j < ROWS_STEP; ++j) {
+                    const int r = __builtin_amdgcn_readlane(rows, (at - sub + j) / PAGED_TILE);
+                    if (r < 0 || at + j >= lim) continue;
+                    const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int dt = 0; dt < 8; ++dt) {
+                            const float x = row_value<FMT>(a, vrow, 32 * q + 8 * i + dt);
+                            if (at + j <= row.last && !(fabsf(x) < __builtin_inff())) O[dt][i] += x;
+                        }
+                }
         }
     }
     // Join the waves: lane (r16, q) of each has dims 8 (4 q + i) + dt of row r16.
@@ -542,7 +540,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
     }
     if (row.t < 0) return;
     // Wave w writes dims 8 (4 q + i) + 2 w, + 1.
-    const float inv = a.nsplit > 1 ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+    const float inv = a.rows.n > 1 ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
     const int64_t out_row = (int64_t)row.t * a.n_heads + row.head;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -552,8 +550,8 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) y2[h] += so[w][2 * wave + h][lane][i] * f[w];
         const int d = 8 * (4 * q + i) + 2 * wave;
-        if (a.nsplit > 1) {
-            *(float2*)(a.part + (out_row * a.nsplit + split) * HD + d) = make_float2(y2[0], y2[1]);
+        if (a.rows.n > 1) {
+            *(float2*)(a.part + (out_row * a.part_splits + split) * HD + d) = make_float2(y2[0], y2[1]);
         } else {
             const int64_t o = (int64_t)row.t * a.out_stride + row.head * HD + d;
             if constexpr (TYPE == TYPE_F32)
@@ -562,7 +560,458 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
                 *(f16x2*)((f16*)a.out + o) = f16x2{(f16)(y2[0] * inv), (f16)(y2[1] * inv)};
         }
     }
-    if (a.nsplit > 1 && wave == 0 && q == 0) a.part_ml[out_row * a.nsplit + split] = make_float2(mt, lt);
+    if (a.rows.n > 1 && wave == 0 && q == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
+}
+
+// Sequences with more query rows: flash attention on 128 rows of a (sequence, KV head) a workgroup, eight
+// waves.  Wave w has rows 32 (w & 3) .. + 31 and of each 128 slots the half w >> 2; the two halves keep
+// softmax states of their own, joined through LDS at the end.  K and V are staged in LDS, two stages of
+// 128 slots, by copies that run under the products (fp16: memory to LDS directly; q8 through registers:
+// dequantised to fp16 for fp16 queries, for fp32 ones as exact codes, whose scales go to the sums of a
+// group's products and to the probabilities in fp32).  v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns, lane (column, h)
+// has slots 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major V by
+// transposing LDS reads.
+//
+// A staged row is 16 chunks of 16 bytes, chunk c at place c ^ swizzle(row): both the operand reads of K
+// (8 rows at one chunk) and of V (4 rows at two chunks) then spread over all banks.
+constexpr int CH_ROWS = 128, CH_HALF = 64;
+constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
+constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
+// q8 with fp32 queries: a half's scales [K, V][group][slot] and the largest of V, [group][16-slot tile].
+constexpr int CH_SCALES = 8 * CH_HALF + 16;
+// And for the eight tiles of two stages whether they exist, and whether V has values that are no numbers.
+constexpr int CH_LDS = 2 * CH_STAGE + 4 * CH_SCALES * 4 + 128;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+__device__ __constant__ const u32x4 g_zeros = {0, 0, 0, 0};  // what slots that are not there are copied from
+
+__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+__device__ __forceinline__ f32x16 mfma32(v8h a, v8h b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// All of this wave's copies to LDS and LDS writes are done, then all waves meet.
+__device__ __forceinline__ void staged_barrier() {
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The sequence and tile (of `rows` query rows a KV head) that workgroup tile `index` stands for, over the
+// sequences with more than ROWS_TILE rows; false past the last one.  One wave looks at 64 sequences at a time.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int group, int rows, int index, int& s, int& tile, int& tiles) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
+        int n = 0;
+        if (s0 + lane < a.n_seqs) {
+            n = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv).n_q * group;
+            n = n > ROWS_TILE ? (n + rows - 1) / rows : 0;
+        }
+        int end = n;
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const int x = __shfl_up(end, o);
+            if (lane >= o) end += x;
+        }
+        const uint64_t past = __ballot(end > index);
+        if (past) {
+            const int first = __ffsll((unsigned long long)past) - 1;
+            tile = index - __shfl(end - n, first);
+            tiles = __shfl(n, first);
+            s = s0 + first;
+            return true;
+        }
+        index -= __shfl(end, WAVE - 1);
+    }
+    return false;
+}
+
+template <int TYPE, int FMT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
+    constexpr bool HL = TYPE == TYPE_F32, EXACT = HL && FMT == FMT_Q8;
+    extern __shared__ __align__(1024) uint8_t lds[];
+    int* const tile_ok = (int*)(lds + 2 * CH_STAGE + 4 * CH_SCALES * 4);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
+    const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
+    const int g = blockIdx.x % a.map.n_kv, at = blockIdx.x / a.map.n_kv, split = at % a.big.n;
+    int s, tile, tiles;
+    if (!find_tile(a, group, CH_ROWS, at / a.big.n, s, tile, tiles)) return;
+    s = __builtin_amdgcn_readfirstlane(s);
+    tile = __builtin_amdgcn_readfirstlane(tiles - 1 - tile);  // those that see the most slots first
+    const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
+    const int before = sp.n_kv - sp.n_q;  // token i sees slots up to before + i
+    const int r0 = tile * CH_ROWS + 32 * wi;
+    const bool active = r0 < sp.n_q * group;
+    const int w_first = before + r0 / group, w_last = before + min(sp.n_q - 1, (r0 + 31) / group);
+    const int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
+    const RowOf row = row_of(sp, r0 + c32, group, g);
+    const int c0 = min(lim, split * a.big.chunk), c1 = min(lim, c0 + a.big.chunk);
+    const int it0 = c0 / 128, it1 = (c1 + 127) / 128;
+
+    // Query operands: dims 16 ks + 8 h .. + 7 of the column's row.
+    // Scores are masked before they are scaled, so the scale is positive: a negative one's sign goes to
+    // the query.
+    v8h Qh[8], Ql[HL ? 8 : 1];
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    float qc = fabsf(a.scale) * 1.4426950408889634f;
+    {
+        const int64_t qa = (int64_t)row.t * a.q_stride + row.head * HD + 8 * h;
+        if constexpr (!HL) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) Qh[ks] = row.t < 0 ? v8h{} : *(const v8h*)((const f16*)a.q + qa + 16 * ks) * (f16)sign;
+        } else {
+            f32x4 x[16];
+            float amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                x[k] = row.t < 0 ? f32x4{} : *(const f32x4*)((const float*)a.q + qa + 16 * (k / 2) + 4 * (k % 2));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
+            }
+            amax = max_x2(amax);
+            const int k2 = query_shift(amax);
+            qc = ldexpf(qc, -k2);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = sign * ldexpf(x[k][e], k2);
+                    const f16 hi = (f16)v;
+                    Qh[k / 2][4 * (k % 2) + e] = hi;
+                    Ql[k / 2][4 * (k % 2) + e] = (f16)(v - (float)hi);
+                }
+        }
+    }
+
+    qc = fmaxf(qc, 1e-37f);  // and not zero: products are below 2^40, so this makes scores of 2^-80 at most
+
+    // Staging: wave w copies 16-slot tile w of an iteration's eight.  Lane i of `rows`: the pool row of this
+    // wave's tile in iteration sub + i (-1: no such page).
+    const int32_t* table = a.tables + (int64_t)s * a.table_width;
+    int rows = -1, sub = it0 - WAVE;
+    // Row l / 16 (+ 4 j) of the tile, place l % 16.
+    int src_off[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) src_off[j] = (4 * j + lane / 16) * (HD * 2) + (((lane & 15) ^ swizzle(4 * j + lane / 16)) << 4);
+    auto tile_row = [&](int it) {
+        if (it >= sub + WAVE) {
+            sub = it;
+            const int slot = (sub + lane) * 128 + 16 * wave;
+            rows = slot < c1 ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
+        }
+        return __builtin_amdgcn_readlane(rows, it - sub);
+    };
+    auto issue = [&](int it) {
+        const int r = tile_row(it), slot0 = it * 128 + 16 * wave;
+        uint8_t* st = lds + (it & 1) * CH_STAGE + (wave >> 2) * 2 * CH_MAT + (wave & 3) * 16 * HD * 2;
+        if (lane == 0) tile_ok[(it & 1) * 8 + wave] = r >= 0;
+        const int64_t base = (int64_t)(max(r, 0) + g * a.map.page_slots) * (HD * 2);
+        const int n = r < 0 ? 0 : lim - slot0;  // rows of the tile that are there
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            const uint8_t* src = (const uint8_t*)(kv ? a.v : a.k) + base;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t* p = src + src_off[j & 1] + (j >> 1) * 8 * HD * 2;
+                if (n < 16 && 4 * j + lane / 16 >= n) p = (const uint8_t*)&g_zeros;
+                __builtin_amdgcn_global_load_lds(p, (__attribute__((address_space(3))) void*)(st + kv * CH_MAT + j * 1024), 16, 0, 0);
+            }
+        }
+    };
+
+    // q8: lane l has row l / 4 of the tile and its group l % 4, fetched before the products and put to
+    // LDS after them.
+    u32x4 kc[2], vc[2];
+    uint16_t ksc = 0, vsc = 0;
+    int fetched = -1;
+    auto fetch = [&](int it) {
+        fetched = tile_row(it);
+        const int n = fetched < 0 ? 0 : lim - (it * 128 + 16 * wave);
+        kc[0] = kc[1] = vc[0] = vc[1] = u32x4{0, 0, 0, 0};
+        ksc = vsc = 0;
+        if (lane / 4 < n) {
+            const int64_t r = (int64_t)fetched + g * a.map.page_slots + lane / 4;
+            const uint8_t *k = (const uint8_t*)a.k + r * HD + 32 * (lane & 3), *v = (const uint8_t*)a.v + r * HD + 32 * (lane & 3);
+            kc[0] = *(const u32x4*)k;
+            kc[1] = *(const u32x4*)(k + 16);
+            vc[0] = *(const u32x4*)v;
+            vc[1] = *(const u32x4*)(v + 16);
+            ksc = ((const uint16_t*)a.k_sb)[r * NG + (lane & 3)];
+            vsc = ((const uint16_t*)a.v_sb)[r * NG + (lane & 3)];
+        }
+    };
+    auto put = [&](int it) {
+        uint8_t* st = lds + (it & 1) * CH_STAGE + par * 2 * CH_MAT;
+        const int r = 16 * wi + lane / 4;
+        // V with a scale that is no number, or (fp16 products) takes codes out of fp16's range: what is no
+        // number is kept out of the products, for the rows that may not see it.
+        const bool odd = __ballot(!(h2f(vsc) <= (EXACT ? 65504.f : 65504.f / 127.f))) != 0;
+        if (lane == 0) {
+            tile_ok[(it & 1) * 8 + wave] = fetched >= 0;
+            tile_ok[16 + (it & 1) * 8 + wave] = odd;
+        }
+        if (EXACT && !(h2f(vsc) <= 65504.f)) vsc = 0;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            const f16 sc = __builtin_bit_cast(f16, kv ? vsc : ksc);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const u32x4 w = kv ? vc[k / 2] : kc[k / 2];
+                u32x4 y;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    f16x2 c[2];
+                    codes_h2(w[2 * (k % 2) + x], c);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) y[2 * x + e] = h2_bits(EXACT ? c[e] : c[e] * sc);
+                }
+                if (!EXACT && kv && odd) {
+                    v8h fin = __builtin_bit_cast(v8h, y);
+                    uint32_t some = 0;
+                    keep_finite(fin, some);
+                    y = __builtin_bit_cast(u32x4, fin);
+                }
+                *(u32x4*)(st + kv * CH_MAT + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
+            }
+            if constexpr (EXACT)
+                ((float*)(lds + 2 * CH_STAGE))[((it & 1) * 2 + par) * CH_SCALES + kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = (float)sc;
+        }
+        if constexpr (EXACT) {
+            // The largest scale of each group: over the lanes with the same l % 4.
+            float top = h2f(vsc);
+            top = fmaxf(top, dpp<0x124>(top));  // row_ror:4, 8: within rows of 16 lanes
+            top = fmaxf(top, dpp<0x128>(top));
+            top = max_x4(top);
+            if (lane < 4) ((float*)(lds + 2 * CH_STAGE))[((it & 1) * 2 + par) * CH_SCALES + 8 * CH_HALF + 4 * lane + wi] = top;
+        }
+    };
+
+    f32x16 O[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
+    float m = NEG_INF, l = 0.f;
+    if (it0 < it1) {
+        if constexpr (FMT == FMT_F16) {
+            issue(it0);
+        } else {
+            fetch(it0);
+            put(it0);
+        }
+    }
+    for (int it = it0; it < it1; ++it) {
+        staged_barrier();
+        if (it + 1 < it1) {
+            if constexpr (FMT == FMT_F16)
+                issue(it + 1);
+            else
+                fetch(it + 1);
+        }
+        if constexpr (FMT == FMT_F16) {
+            // Slots that some rows of the workgroup see and others do not may hold values that are no numbers.
+            // In the iterations that have such slots each wave makes its tile of V finite.
+            if (it * 128 + 127 > before + tile * CH_ROWS / group) {
+                uint32_t odd = 0;
+                uint8_t* vt = lds + (it & 1) * CH_STAGE + (2 * par + 1) * CH_MAT + wi * 16 * HD * 2 + lane * 16;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v8h v = *(const v8h*)(vt + 1024 * k);
+                    keep_finite(v, odd);
+                    *(v8h*)(vt + 1024 * k) = v;
+                }
+                const bool any = __ballot(odd != 0) != 0;
+                if (lane == 0) tile_ok[16 + (it & 1) * 8 + wave] = any;
+                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the copies for the next iteration stay in flight
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+        }
+        const int base = it * 128 + CH_HALF * par;
+        if (active && base <= w_last) {
+        const uint8_t* Ks = lds + (it & 1) * CH_STAGE + par * 2 * CH_MAT;
+        const uint8_t* Vs = Ks + CH_MAT;
+        const float* scales = (const float*)(lds + 2 * CH_STAGE) + ((it & 1) * 2 + par) * CH_SCALES;
+        auto k_operand = [&](int kt, int ks) {
+            const int r = kt * 32 + c32;
+            return *(const v8h*)(Ks + r * (HD * 2) + (((2 * ks + h) ^ swizzle(r)) << 4));
+        };
+        f32x16 S[2] = {};
+        if constexpr (!EXACT) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const v8h kf = k_operand(kt, ks);
+                    S[kt] = mfma32(kf, Qh[ks], S[kt]);
+                    if constexpr (HL) S[kt] = mfma32(kf, Ql[ks], S[kt]);
+                }
+        } else {  // a group's sum of codes takes its slot's scale
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                    f32x16 y = {};
+#pragma unroll
+                    for (int ks = 2 * gr; ks < 2 * gr + 2; ++ks) {
+                        const v8h kf = k_operand(kt, ks);
+                        y = mfma32(kf, Qh[ks], y);
+                        y = mfma32(kf, Ql[ks], y);
+                    }
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const f32x4 sc = *(const f32x4*)(scales + gr * CH_HALF + 32 * kt + 8 * b + 4 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) S[kt][4 * b + e] += y[4 * b + e] * sc[e];
+                    }
+                }
+        }
+        // Element i of block kt: slot base + 32 kt + 8 (i / 4) + 4 h + i % 4.
+        const int4 ok = *(const int4*)(tile_ok + (it & 1) * 8 + 4 * par);
+        const bool all_there = (ok.x & ok.y & ok.z & ok.w) != 0;
+        const bool masked = __builtin_amdgcn_readfirstlane(base + CH_HALF - 1 > w_first || !all_there);
+        if (masked) {
+            const int there[4] = {ok.x, ok.y, ok.z, ok.w};
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (base + 32 * kt + 8 * (i / 4) + 4 * h + i % 4 > row.last || !there[2 * kt + i / 8]) S[kt][i] = NEG_INF;
+        }
+        float mb = NEG_INF;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mb = fmaxf(mb, S[kt][i] * qc);
+        mb = max_x2(mb);
+        const float m_new = fmaxf(m, mb);
+        const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+        const float sub_m = m_new == NEG_INF ? 0.f : m_new - P_SHIFT;
+        m = m_new;
+        l *= corr;
+        if (__builtin_amdgcn_ballot_w64(corr != 1.f)) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) O[dt] *= corr;
+        }
+        v8h Ph[EXACT ? 1 : 4], Pl[HL && !EXACT ? 4 : 1];
+        float P[EXACT ? 32 : 1];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = __builtin_amdgcn_exp2f(S[c / 2][8 * (c % 2) + e] * qc - sub_m);
+                l += p;
+                if constexpr (EXACT) {
+                    P[8 * c + e] = p;
+                } else {
+                    Ph[c][e] = (f16)p;
+                    if constexpr (HL) Pl[c][e] = (f16)(p - (float)Ph[c][e]);
+                }
+            }
+        // V^T operand of dims 32 dt + c32 over slots 16 c + 4 h + {0 .. 3, 8 .. 11}.
+        auto v_operand = [&](int c, int dt) {
+            v4s half[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = 16 * c + 8 * k + 4 * h + ((lane & 15) >> 2);
+                const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(
+                    Vs + r * (HD * 2) + ((chunk ^ swizzle(r)) << 4) + 8 * (lane & 1)));
+            }
+            return __builtin_bit_cast(v8h, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        if constexpr (!EXACT) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    const v8h v = v_operand(c, dt);
+                    O[dt] = mfma32(v, Ph[c], O[dt]);
+                    if constexpr (HL) O[dt] = mfma32(v, Pl[c], O[dt]);
+                }
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                // The tile's dims are one group: its scales, by the power of two that brings the half's largest
+                // below 1, go to the probabilities, and the power to the sum.
+                const f32x4 tops = *(const f32x4*)(scales + 8 * CH_HALF + 4 * dt);
+                const int e2 = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+                const float down = ldexpf(1.f, -e2), up = ldexpf(1.f, e2);
+                f32x16 y = {};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    v8h ph, pl;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const f32x4 sc = *(const f32x4*)(scales + 4 * CH_HALF + dt * CH_HALF + 16 * c + 8 * k + 4 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = P[8 * c + 4 * k + e] * (sc[e] * down);
+                            ph[4 * k + e] = (f16)x;
+                            pl[4 * k + e] = (f16)(x - (float)ph[4 * k + e]);
+                        }
+                    }
+                    const v8h v = v_operand(c, dt);
+                    y = mfma32(v, ph, y);
+                    y = mfma32(v, pl, y);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) O[dt][i] += up * y[i];
+            }
+        }
+        // Values that are no numbers were kept out of the products: they go to the rows that see them.
+        if (base + CH_HALF - 1 > w_first || FMT == FMT_Q8) {
+            const int4 odd = *(const int4*)(tile_ok + 16 + (it & 1) * 8 + 4 * par);
+            if (__builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w))
+                for (int j = 0; j < CH_HALF && base + j < lim; ++j) {
+                    const int r = seq_slot_row(a.map, table, a.table_width, base + j);
+                    if (r < 0) continue;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = row_value<FMT>(a, (int64_t)r + g * a.map.page_slots, 32 * (k / 4) + 8 * (k % 4) + 4 * h + e);
+                            if (base + j <= row.last && !(fabsf(x) < __builtin_inff())) O[k / 4][4 * (k % 4) + e] += x;
+                        }
+                }
+        }
+        }
+        if constexpr (FMT == FMT_Q8)
+            if (it + 1 < it1) put(it + 1);
+    }
+
+    // The halves' states join: waves 4 .. 7 hand theirs to waves 0 .. 3.
+    staged_barrier();
+    f32x4* const mo = (f32x4*)lds;                          // [4 waves][16][64 lanes]
+    float2* const mml = (float2*)(lds + 4 * 16 * 64 * 16);  // [4 waves][64 lanes]
+    l = swap32_add(l, l);
+    if (par == 1) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            mo[(wi * 16 + k) * 64 + lane] = f32x4{O[k / 4][4 * (k % 4)], O[k / 4][4 * (k % 4) + 1], O[k / 4][4 * (k % 4) + 2], O[k / 4][4 * (k % 4) + 3]};
+        mml[wi * 64 + lane] = make_float2(m, l);
+    }
+    staged_barrier();
+    if (par == 1 || row.t < 0) return;
+    const float2 ml = mml[wi * 64 + lane];
+    const float mt = fmaxf(m, ml.x);
+    const float f0 = m == mt ? 1.f : __builtin_amdgcn_exp2f(m - mt), f1 = ml.x == mt ? 1.f : __builtin_amdgcn_exp2f(ml.x - mt);
+    const float lt = l * f0 + ml.y * f1;
+    const float inv = a.big.n > 1 ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+    const int64_t out_row = (int64_t)row.t * a.n_heads + row.head;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const f32x4 o1 = mo[(wi * 16 + k) * 64 + lane];
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (O[k / 4][4 * (k % 4) + e] * f0 + o1[e] * f1) * inv;
+        const int d = 32 * (k / 4) + 8 * (k % 4) + 4 * h;
+        if (a.big.n > 1)
+            *(f32x4*)(a.part + (out_row * a.part_splits + split) * HD + d) = y;
+        else
+            store4<TYPE>(a.out, (int64_t)row.t * a.out_stride + row.head * HD + d, y);
+    }
+    if (a.big.n > 1 && h == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
 }
 
 // Joins the splits of a row: one wave a row, two dims a lane.
@@ -572,18 +1021,26 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
     const int lane = threadIdx.x & 63;
     if (row >= (int64_t)a.n_tokens * a.n_heads) return;
     const int t = (int)(row / a.n_heads), head = (int)(row - (int64_t)t * a.n_heads);
-    // Rows of no sequence stay as they are.
-    if (t < max(0, a.q_start[0]) || t >= a.q_start[a.n_seqs]) return;
+    // The row's sequence, 64 at a time; rows of none stay as they are.
+    int n_q = 0;
+    for (int s0 = 0; s0 < a.n_seqs && !n_q; s0 += WAVE) {
+        SeqSpan sp = {0, 0, 0};
+        if (s0 + lane < a.n_seqs) sp = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
+        const uint64_t mine = __ballot(t >= sp.t0 && t < sp.t0 + sp.n_q);
+        if (mine) n_q = __shfl(sp.n_q, __ffsll((unsigned long long)mine) - 1);
+    }
+    const int nsplit = n_q * (a.n_heads / a.map.n_kv) <= ROWS_TILE ? a.rows.n : a.big.n;
+    if (n_q == 0 || nsplit == 1) return;  // unsplit: written already
     float2 ml = make_float2(NEG_INF, 0.f);
-    if (lane < a.nsplit) ml = a.part_ml[row * a.nsplit + lane];
+    if (lane < nsplit) ml = a.part_ml[row * a.part_splits + lane];
     const float m = wave_max(ml.x);
     const float f = ml.x == NEG_INF ? 0.f : ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
     const float l = wave_sum(ml.y * f);
     float2 o = make_float2(0.f, 0.f);
-    for (int i = 0; i < a.nsplit; ++i) {
+    for (int i = 0; i < nsplit; ++i) {
         const float w = as_f32(__builtin_amdgcn_readlane(as_u32(f), i));
         if (w == 0.f) continue;
-        const float2 p = *(const float2*)(a.part + (row * a.nsplit + i) * HD + 2 * lane);
+        const float2 p = *(const float2*)(a.part + (row * a.part_splits + i) * HD + 2 * lane);
         o.x += w * p.x;
         o.y += w * p.y;
     }
@@ -626,40 +1083,54 @@ hipError_t launch_paged_load(int fmt, int type, const PagedLoadArgs& a, hipStrea
     return hipGetLastError();
 }
 
+// Splits of max_kv slots among `per` workgroups of each (sequence, rows, KV head) that make up to `want`
+// in all, each a multiple of 128 slots.
+static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv) {
+    const int64_t most = std::max(1, (max_kv + 127) / 128);
+    const int n = (int)std::min<int64_t>({std::max<int64_t>(1, want / std::max<int64_t>(1, groups)), most, PAGED_MAX_SPLITS});
+    const int chunk = std::max(128, ((max_kv + n - 1) / n + 127) / 128 * 128);
+    return {std::max(1, (max_kv + chunk - 1) / chunk), chunk};
+}
+
 PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv) {
     PagedPlan p{};
     const int group = n_heads / n_kv;
-    p.one_tile = (int64_t)max_q * group <= 16;
-    const int64_t tiles = p.one_tile ? n_seqs : (int64_t)n_tokens * group / 16 + n_seqs;
-    p.tiles = (int)std::min<int64_t>(tiles, 1 << 30);
-    // Slots are split among workgroups until there are four of them for each of the 256 CUs.
-    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, tiles * n_kv));
-    const int most = std::max(1, (max_kv + 127) / 128);  // at least a step for each wave
-    p.nsplit = (int)std::min<int64_t>({want, most, PAGED_MAX_SPLITS});
-    p.chunk = ((max_kv + p.nsplit - 1) / p.nsplit + 127) / 128 * 128;
-    p.nsplit = std::max(1, (max_kv + p.chunk - 1) / std::max(1, p.chunk));
-    if (p.nsplit > 1) {
-        p.part_floats = (size_t)n_tokens * n_heads * p.nsplit * HD;
-        p.ml_floats = (size_t)n_tokens * n_heads * p.nsplit * 2;
+    p.rows = split_slots((int64_t)n_seqs * n_kv, 1024, max_kv);
+    p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
+    if ((int64_t)max_q * group > ROWS_TILE) {
+        p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
+        p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv);
+    }
+    p.part_splits = std::max(p.rows.n, p.big.n);
+    if (p.part_splits > 1) {
+        p.part_floats = (size_t)n_tokens * n_heads * p.part_splits * HD;
+        p.ml_floats = (size_t)n_tokens * n_heads * p.part_splits * 2;
     }
     return p;
 }
 
-hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s) {
-    const dim3 grid(a.tiles, a.map.n_kv, a.nsplit);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
-    if (fmt == FMT_Q8)
-        type == TYPE_F32 ? go(paged_rows_kernel<TYPE_F32, FMT_Q8>) : go(paged_rows_kernel<TYPE_F16, FMT_Q8>);
-    else
-        type == TYPE_F32 ? go(paged_rows_kernel<TYPE_F32, FMT_F16>) : go(paged_rows_kernel<TYPE_F16, FMT_F16>);
+template <int TYPE, int FMT>
+static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((paged_rows_kernel<TYPE, FMT>), dim3(a.n_seqs, a.map.n_kv, a.rows.n), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.nsplit == 1) return e;
-    const dim3 mgrid((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4));
-    if (type == TYPE_F32)
-        hipLaunchKernelGGL(paged_merge_kernel<TYPE_F32>, mgrid, dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(paged_merge_kernel<TYPE_F16>, mgrid, dim3(256), 0, s, a);
-    return hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.tiles) {
+        e = hipFuncSetAttribute((const void*)paged_chunk_kernel<TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, CH_LDS);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_chunk_kernel<TYPE, FMT>), dim3((unsigned)a.tiles * a.map.n_kv * a.big.n), dim3(512), CH_LDS, s, a);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (a.part_splits > 1) {
+        hipLaunchKernelGGL(paged_merge_kernel<TYPE>, dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s) {
+    if (fmt == FMT_Q8) return type == TYPE_F32 ? attention_of<TYPE_F32, FMT_Q8>(a, s) : attention_of<TYPE_F16, FMT_Q8>(a, s);
+    return type == TYPE_F32 ? attention_of<TYPE_F32, FMT_F16>(a, s) : attention_of<TYPE_F16, FMT_F16>(a, s);
 }
 
 }  // namespace icua

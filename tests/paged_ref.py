@@ -66,7 +66,7 @@ class Pool:
 
 
 def attention(pool, q, q_lens, kv_lens, tables, scale=None):
-    """(out, bound of |k| . |q| scale, largest |v|); q [T][heads][128], pages outside the pool take no part."""
+    """(out, bound of |k| . |q| |scale|, largest |v|); q [T][heads][128], pages outside the pool take no part."""
     scale = D ** -0.5 if scale is None else scale
     heads = q.shape[1]
     group = heads // pool.n_kv
@@ -87,7 +87,7 @@ def attention(pool, q, q_lens, kv_lens, tables, scale=None):
                 x = kk @ qq * scale
                 w = np.exp(x - x.max())
                 out[t + i, h] = w @ vv / w.sum()
-                reach = max(reach, float((np.abs(kk) @ np.abs(qq)).max() * scale))
+                reach = max(reach, float((np.abs(kk) @ np.abs(qq)).max() * abs(scale)))  # a scale may be negative
                 vmax = max(vmax, float(np.abs(vv).max()))
         t += m
     return out, reach, vmax
