@@ -190,15 +190,16 @@ __global__ __launch_bounds__(256) void paged_load_kernel(PagedLoadArgs a) {
 // A KV head's query rows are (token i, head of the group h), numbered i * group + h.  Products run
 // transposed on v_mfma_f32_16x16x32_f16, 16 query rows as columns: S^T = K Q^T leaves lane (column c,
 // q) with slots 4 q .. 4 q + 3 of a 16-slot tile, which is the B operand of O^T = V^T P^T when the V
-// operand takes its slots in that order.  Exponentials are taken of base-2 scores, shifted by 2^15 (of
-// numerator and denominator alike): fp16 probabilities down to 2^-39 of the largest keep their value,
-// where unshifted ones would round to nothing below 2^-24, which adds up over long caches.
+// operand takes its slots in that order.  Exponentials are taken of base-2 scores, shifted by 2^9 (of
+// numerator and denominator alike): fp16 probabilities down to 2^-33 of the largest keep their value,
+// where unshifted ones would round to nothing below 2^-24, which adds up over long caches.  The maximum
+// that is subtracted may lag 2^6 behind the true one, so accumulators are seldom rescaled.
 //
 // fp32 queries and probabilities are split into fp16 hi + lo parts, two products each; queries are
 // first scaled by a power of two that puts the row's largest value in [2^9, 2^10), so that neither
 // part leaves fp16's range.
 
-constexpr float P_SHIFT = 15.0f;
+constexpr float P_SHIFT = 9.0f, P_SLACK = 6.0f;
 
 // Max over the lanes l and l ^ 32.
 __device__ __forceinline__ float max_x2(float v) {
@@ -317,6 +318,9 @@ __device__ __forceinline__ void load_v(const PagedAttnArgs& a, int row, int lane
     }
 }
 
+// All ones for the bits of an infinity or no number, else zero.
+__device__ __forceinline__ uint32_t no_number(uint32_t x) { return (uint32_t)((int32_t)((x & 0x7F800000u) + 0x00800000u) >> 31); }
+
 // Four int8 codes as exact fp16 values: code + 128 under the exponent of 1024 is 1152 + code.
 __device__ __forceinline__ void codes_h2(uint32_t w, f16x2 y[2]) {
     const uint32_t u = w ^ 0x80808080u;
@@ -401,9 +405,9 @@ __device__ __forceinline__ void v_operands(const VTile<FMT>* t, VOps<TYPE, FMT>&
 
 // Value d of a row of V, as the products take it.
 template <int FMT>
-__device__ __forceinline__ float row_value(const PagedAttnArgs& a, int64_t row, int d) {
-    if constexpr (FMT == FMT_F16) return (float)((const f16*)a.v)[row * HD + d];
-    return (float)(f16)(h2f(((const uint16_t*)a.v_sb)[row * NG + d / QG]) * (float)((const int8_t*)a.v)[row * HD + d]);
+__device__ __forceinline__ float row_value(const void* v, const void* v_sb, int64_t row, int d) {
+    if constexpr (FMT == FMT_F16) return (float)((const f16*)v)[row * HD + d];
+    return (float)(f16)(h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d]);
 }
 
 template <int TYPE, int FMT>
@@ -511,12 +515,13 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
                     const int r = __builtin_amdgcn_readlane(rows, (at - sub + j) / PAGED_TILE);
                     if (r < 0 || at + j >= lim) continue;
                     const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
+                    const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int dt = 0; dt < 8; ++dt) {
-                            const float x = row_value<FMT>(a, vrow, 32 * q + 8 * i + dt);
-                            if (at + j <= row.last && !(fabsf(x) < __builtin_inff())) O[dt][i] += x;
+                            const uint32_t x = as_u32(row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * i + dt));
+                            O[dt][i] += as_f32(x & sees & no_number(x));
                         }
                 }
         }
@@ -579,7 +584,7 @@ constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
 constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
 // q8 with fp32 queries: a half's scales [K, V][group][slot] and the largest of V, [group][16-slot tile].
 constexpr int CH_SCALES = 8 * CH_HALF + 16;
-// And for the eight tiles of two stages whether they exist, and whether V has values that are no numbers.
+// And for the eight tiles of two stages whether V has values that are no numbers, and whether the page exists.
 constexpr int CH_LDS = 2 * CH_STAGE + 4 * CH_SCALES * 4 + 128;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -587,13 +592,26 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 __device__ __constant__ const u32x4 g_zeros = {0, 0, 0, 0};  // what slots that are not there are copied from
 
-__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
 __device__ __forceinline__ f32x16 mfma32(v8h a, v8h b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// All of this wave's copies to LDS and LDS writes are done, then all waves meet.
+// Each lane's 16 bytes from memory to LDS, lane l's to dst + 16 l (dst the same in all lanes).  As assembly
+// (it has no outputs): after the builtin the compiler waits for the copy before the next transposing read,
+// whatever stage that reads.
+__device__ __forceinline__ void copy_to_lds(const uint8_t* p, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(p) : "memory", "m0");
+}
+// The same from base + offset, base the same in all lanes.
+__device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory", "m0");
+}
+
+// This wave's LDS writes are done and of its copies and loads at most the last `pending` in flight (63: no
+// matter), then all waves meet.  The empty statements keep memory accesses on their side of the barrier.
+template <int pending>
 __device__ __forceinline__ void staged_barrier() {
-    __builtin_amdgcn_s_waitcnt(0);
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((pending & 15) | (7 << 4) | (0 << 8) | ((pending >> 4) << 14));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -631,7 +649,8 @@ template <int TYPE, int FMT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
     constexpr bool HL = TYPE == TYPE_F32, EXACT = HL && FMT == FMT_Q8;
     extern __shared__ __align__(1024) uint8_t lds[];
-    int* const tile_ok = (int*)(lds + 2 * CH_STAGE + 4 * CH_SCALES * 4);
+    int* const tile_odd = (int*)(lds + 2 * CH_STAGE + 4 * CH_SCALES * 4);
+    int* const tile_there = tile_odd + 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
     const int g = blockIdx.x % a.map.n_kv, at = blockIdx.x / a.map.n_kv, split = at % a.big.n;
@@ -647,7 +666,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
     const RowOf row = row_of(sp, r0 + c32, group, g);
     const int c0 = min(lim, split * a.big.chunk), c1 = min(lim, c0 + a.big.chunk);
-    const int it0 = c0 / 128, it1 = (c1 + 127) / 128;
+    const int it0 = c0 / 128, it1 = c1 > c0 ? (c1 + 127) / 128 : it0;
 
     // Query operands: dims 16 ks + 8 h .. + 7 of the column's row.
     // Scores are masked before they are scaled, so the scale is positive: a negative one's sign goes to
@@ -686,104 +705,116 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     qc = fmaxf(qc, 1e-37f);  // and not zero: products are below 2^40, so this makes scores of 2^-80 at most
 
+    // What the loop seldom needs is read again from the arguments where it is needed, so that it takes no
+    // registers in between.
+    auto arguments = []() __attribute__((always_inline)) {
+        auto p = (__attribute__((address_space(4))) const PagedAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(p));
+        return p;
+    };
     // Staging: wave w copies 16-slot tile w of an iteration's eight.  Lane i of `rows`: the pool row of this
     // wave's tile in iteration sub + i (-1: no such page).
-    const int32_t* table = a.tables + (int64_t)s * a.table_width;
+    bool bad_pages = false;
+    {
+        const int32_t* table = a.tables + (int64_t)s * a.table_width;
+        const int last_page = c1 > c0 ? (c1 - 1) / a.map.page_slots : -1;
+        for (int p = c0 / a.map.page_slots; p <= last_page; p += WAVE)
+            if (__ballot(p + lane <= last_page && page_row(a.map, table[min(p + lane, last_page)], 0) < 0)) bad_pages = true;
+    }
     int rows = -1, sub = it0 - WAVE;
-    // Row l / 16 (+ 4 j) of the tile, place l % 16.
-    int src_off[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) src_off[j] = (4 * j + lane / 16) * (HD * 2) + (((lane & 15) ^ swizzle(4 * j + lane / 16)) << 4);
-    auto tile_row = [&](int it) {
+    const int head_row = g * a.map.page_slots;
+    auto tile_row = [&](int it) __attribute__((always_inline)) {
         if (it >= sub + WAVE) {
+            auto b = arguments();
+            const PageMap map = {b->map.n_pages, b->map.n_kv, b->map.page_slots};
             sub = it;
             const int slot = (sub + lane) * 128 + 16 * wave;
-            rows = slot < c1 ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
+            rows = slot < c1 ? seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, slot) : -1;
         }
         return __builtin_amdgcn_readlane(rows, it - sub);
     };
-    auto issue = [&](int it) {
-        const int r = tile_row(it), slot0 = it * 128 + 16 * wave;
-        uint8_t* st = lds + (it & 1) * CH_STAGE + (wave >> 2) * 2 * CH_MAT + (wave & 3) * 16 * HD * 2;
-        if (lane == 0) tile_ok[(it & 1) * 8 + wave] = r >= 0;
-        const int64_t base = (int64_t)(max(r, 0) + g * a.map.page_slots) * (HD * 2);
-        const int n = r < 0 ? 0 : lim - slot0;  // rows of the tile that are there
+    const uint8_t *k_base = (const uint8_t*)a.k, *v_base = (const uint8_t*)a.v;
+    // LDS: half hb of K (kv = 0) or V (1) in stage st, and the scales of a half.
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    auto half_at = [&](int kv, int st, int hb) { return (uint32_t)((kv * 2 + st) * 2 + hb) * CH_MAT; };
+    auto scales_at = [&](int st, int hb) { return (float*)(lds + 2 * CH_STAGE) + (st * 2 + hb) * CH_SCALES; };
+    // fp16: this wave's tile of iteration it, pool row r, from memory to LDS; slots that are not there become
+    // zeros.  Row l / 16 (+ 4 j) of the tile, place l % 16.
+    int src_off[4];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            const uint8_t* src = (const uint8_t*)(kv ? a.v : a.k) + base;
+    for (int j = 0; j < 4; ++j) src_off[j] = (4 * j + lane / 16) * (HD * 2) + (((lane & 15) ^ swizzle(4 * j + lane / 16)) << 4);
+    auto copy = [&](int kv, int it, int r) __attribute__((always_inline)) {
+        const int n = r < 0 ? 0 : lim - (it * 128 + 16 * wave);
+        const uint32_t dst = lds0 + half_at(kv, it & 1, par) + wi * 16 * HD * 2;
+        const uint8_t* src = (kv ? v_base : k_base) + (int64_t)(max(r, 0) + head_row) * (HD * 2);
+        if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
+        if (n >= 16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) copy_to_lds(src, src_off[j], dst + j * 1024);
+        } else {
+            asm volatile("");
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint8_t* p = src + src_off[j & 1] + (j >> 1) * 8 * HD * 2;
-                if (n < 16 && 4 * j + lane / 16 >= n) p = (const uint8_t*)&g_zeros;
-                __builtin_amdgcn_global_load_lds(p, (__attribute__((address_space(3))) void*)(st + kv * CH_MAT + j * 1024), 16, 0, 0);
+                const uint8_t* p = 4 * j + lane / 16 < n ? src + src_off[j] : (const uint8_t*)&g_zeros;
+                copy_to_lds(p, dst + j * 1024);
             }
         }
     };
-
     // q8: lane l has row l / 4 of the tile and its group l % 4, fetched before the products and put to
     // LDS after them.
-    u32x4 kc[2], vc[2];
-    uint16_t ksc = 0, vsc = 0;
-    int fetched = -1;
-    auto fetch = [&](int it) {
-        fetched = tile_row(it);
-        const int n = fetched < 0 ? 0 : lim - (it * 128 + 16 * wave);
-        kc[0] = kc[1] = vc[0] = vc[1] = u32x4{0, 0, 0, 0};
-        ksc = vsc = 0;
+    u32x4 codes[2][2];
+    uint16_t scale[2] = {0, 0};
+    auto fetch = [&](int kv, int it, int r) __attribute__((always_inline)) {
+        const int n = r < 0 ? 0 : lim - (it * 128 + 16 * wave);
+        if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
+        codes[kv][0] = codes[kv][1] = u32x4{0, 0, 0, 0};
+        scale[kv] = 0;
         if (lane / 4 < n) {
-            const int64_t r = (int64_t)fetched + g * a.map.page_slots + lane / 4;
-            const uint8_t *k = (const uint8_t*)a.k + r * HD + 32 * (lane & 3), *v = (const uint8_t*)a.v + r * HD + 32 * (lane & 3);
-            kc[0] = *(const u32x4*)k;
-            kc[1] = *(const u32x4*)(k + 16);
-            vc[0] = *(const u32x4*)v;
-            vc[1] = *(const u32x4*)(v + 16);
-            ksc = ((const uint16_t*)a.k_sb)[r * NG + (lane & 3)];
-            vsc = ((const uint16_t*)a.v_sb)[r * NG + (lane & 3)];
+            const int64_t at = (int64_t)r + head_row + lane / 4;
+            const uint8_t* c = (kv ? v_base : k_base) + at * HD + 32 * (lane & 3);
+            codes[kv][0] = *(const u32x4*)c;
+            codes[kv][1] = *(const u32x4*)(c + 16);
+            scale[kv] = ((const uint16_t*)(kv ? a.v_sb : a.k_sb))[at * NG + (lane & 3)];
         }
     };
-    auto put = [&](int it) {
-        uint8_t* st = lds + (it & 1) * CH_STAGE + par * 2 * CH_MAT;
+    auto put = [&](int kv, int it) __attribute__((always_inline)) {
+        uint8_t* dst = lds + half_at(kv, it & 1, par);
         const int r = 16 * wi + lane / 4;
         // V with a scale that is no number, or (fp16 products) takes codes out of fp16's range: what is no
         // number is kept out of the products, for the rows that may not see it.
-        const bool odd = __ballot(!(h2f(vsc) <= (EXACT ? 65504.f : 65504.f / 127.f))) != 0;
-        if (lane == 0) {
-            tile_ok[(it & 1) * 8 + wave] = fetched >= 0;
-            tile_ok[16 + (it & 1) * 8 + wave] = odd;
-        }
-        if (EXACT && !(h2f(vsc) <= 65504.f)) vsc = 0;
+        const bool odd = kv && __ballot(!(h2f(scale[1]) <= (EXACT ? 65504.f : 65504.f / 127.f)));
+        if (kv && lane == 0) tile_odd[(it & 1) * 8 + wave] = odd;
+        if (EXACT && kv && !(h2f(scale[1]) <= 65504.f)) scale[1] = 0;
+        const f16 sc = __builtin_bit_cast(f16, scale[kv]);
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            const f16 sc = __builtin_bit_cast(f16, kv ? vsc : ksc);
+        for (int k = 0; k < 4; ++k) {
+            const u32x4 w = codes[kv][k / 2];
+            u32x4 y;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const u32x4 w = kv ? vc[k / 2] : kc[k / 2];
-                u32x4 y;
+            for (int x = 0; x < 2; ++x) {
+                f16x2 c[2];
+                codes_h2(w[2 * (k % 2) + x], c);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    f16x2 c[2];
-                    codes_h2(w[2 * (k % 2) + x], c);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) y[2 * x + e] = h2_bits(EXACT ? c[e] : c[e] * sc);
-                }
-                if (!EXACT && kv && odd) {
-                    v8h fin = __builtin_bit_cast(v8h, y);
-                    uint32_t some = 0;
-                    keep_finite(fin, some);
-                    y = __builtin_bit_cast(u32x4, fin);
-                }
-                *(u32x4*)(st + kv * CH_MAT + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
+                for (int e = 0; e < 2; ++e) y[2 * x + e] = h2_bits(EXACT ? c[e] : c[e] * sc);
             }
-            if constexpr (EXACT)
-                ((float*)(lds + 2 * CH_STAGE))[((it & 1) * 2 + par) * CH_SCALES + kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = (float)sc;
+            if (!EXACT && odd) {
+                v8h fin = __builtin_bit_cast(v8h, y);
+                uint32_t some = 0;
+                keep_finite(fin, some);
+                y = __builtin_bit_cast(u32x4, fin);
+            }
+            *(u32x4*)(dst + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
         }
         if constexpr (EXACT) {
-            // The largest scale of each group: over the lanes with the same l % 4.
-            float top = h2f(vsc);
-            top = fmaxf(top, dpp<0x124>(top));  // row_ror:4, 8: within rows of 16 lanes
-            top = fmaxf(top, dpp<0x128>(top));
-            top = max_x4(top);
-            if (lane < 4) ((float*)(lds + 2 * CH_STAGE))[((it & 1) * 2 + par) * CH_SCALES + 8 * CH_HALF + 4 * lane + wi] = top;
+            float* scales = scales_at(it & 1, par);
+            scales[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = (float)sc;
+            if (kv) {  // the largest scale of each group: over the lanes with the same l % 4
+                float top = (float)sc;
+                top = fmaxf(top, dpp<0x124>(top));  // row_ror:4, 8: within rows of 16 lanes
+                top = fmaxf(top, dpp<0x128>(top));
+                top = max_x4(top);
+                if (lane < 4) scales[8 * CH_HALF + 4 * lane + wi] = top;
+            }
         }
     };
 
@@ -791,197 +822,258 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
     float m = NEG_INF, l = 0.f;
-    if (it0 < it1) {
-        if constexpr (FMT == FMT_F16) {
-            issue(it0);
-        } else {
-            fetch(it0);
-            put(it0);
-        }
+    auto base_of = [&](int it) { return it * 128 + CH_HALF * par; };
+    // LDS addresses of operands in stage 0.  K of block 0: slot c32, dims 16 ks + 8 h .. + 7, at k_at ^ (ks <<
+    // 5).  V^T: dims 32 dt + c32 of slots 4 h + {0 .. 3} (k = 1: + 8, the operand's other half), at v_at[k] ^
+    // (dt << 6).  (A row's place in a stage is a multiple of its 256 bytes.)
+    const uint32_t k_at = lds0 + half_at(0, 0, par) + c32 * (HD * 2) + ((h ^ swizzle(c32)) << 4);
+    uint32_t v_at[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int r = 8 * k + 4 * h + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        v_at[k] = lds0 + half_at(1, 0, par) + r * (HD * 2) + ((chunk ^ swizzle(r)) << 4) + 8 * (lane & 1);
     }
-    for (int it = it0; it < it1; ++it) {
-        staged_barrier();
-        if (it + 1 < it1) {
-            if constexpr (FMT == FMT_F16)
-                issue(it + 1);
-            else
-                fetch(it + 1);
+    auto k_operand = [&](uint32_t block, int ks) __attribute__((always_inline)) {
+        return *(__attribute__((address_space(3))) const v8h*)((k_at + block) ^ (ks << 5));
+    };
+    auto v_operand = [&](uint32_t block, int c, int dt) __attribute__((always_inline)) {
+        v4s half[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(
+                ((v_at[k] + block) ^ (dt << 6)) + c * 16 * HD * 2));
+        return __builtin_bit_cast(v8h, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    // Scores of a block are unscaled; element i: slot 8 (i / 4) + 4 h + i % 4.
+    auto mask = [&](int it, int kt, f32x16& S) __attribute__((always_inline)) {
+        const int base = base_of(it) + 32 * kt;
+        if (base + 31 <= w_first && !bad_pages) return;
+        asm volatile("");  // keeps the branch: the selects are not made where they are not needed
+        const int seen = row.last - base - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (8 * (i / 4) + i % 4 > seen) S[i] = NEG_INF;
+        if (bad_pages) {
+            const int2 there = *(const int2*)(tile_there + (it & 1) * 8 + 4 * par + 2 * kt);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!(i < 8 ? there.x : there.y)) S[i] = NEG_INF;
         }
-        if constexpr (FMT == FMT_F16) {
-            // Slots that some rows of the workgroup see and others do not may hold values that are no numbers.
-            // In the iterations that have such slots each wave makes its tile of V finite.
-            if (it * 128 + 127 > before + tile * CH_ROWS / group) {
-                uint32_t odd = 0;
-                uint8_t* vt = lds + (it & 1) * CH_STAGE + (2 * par + 1) * CH_MAT + wi * 16 * HD * 2 + lane * 16;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v8h v = *(const v8h*)(vt + 1024 * k);
-                    keep_finite(v, odd);
-                    *(v8h*)(vt + 1024 * k) = v;
-                }
-                const bool any = __ballot(odd != 0) != 0;
-                if (lane == 0) tile_ok[16 + (it & 1) * 8 + wave] = any;
-                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the copies for the next iteration stay in flight
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-            }
-        }
-        const int base = it * 128 + CH_HALF * par;
-        if (active && base <= w_last) {
-        const uint8_t* Ks = lds + (it & 1) * CH_STAGE + par * 2 * CH_MAT;
-        const uint8_t* Vs = Ks + CH_MAT;
-        const float* scales = (const float*)(lds + 2 * CH_STAGE) + ((it & 1) * 2 + par) * CH_SCALES;
-        auto k_operand = [&](int kt, int ks) {
-            const int r = kt * 32 + c32;
-            return *(const v8h*)(Ks + r * (HD * 2) + (((2 * ks + h) ^ swizzle(r)) << 4));
-        };
-        f32x16 S[2] = {};
-        if constexpr (!EXACT) {
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    const v8h kf = k_operand(kt, ks);
-                    S[kt] = mfma32(kf, Qh[ks], S[kt]);
-                    if constexpr (HL) S[kt] = mfma32(kf, Ql[ks], S[kt]);
-                }
-        } else {  // a group's sum of codes takes its slot's scale
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr) {
-                    f32x16 y = {};
-#pragma unroll
-                    for (int ks = 2 * gr; ks < 2 * gr + 2; ++ks) {
-                        const v8h kf = k_operand(kt, ks);
-                        y = mfma32(kf, Qh[ks], y);
-                        y = mfma32(kf, Ql[ks], y);
-                    }
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const f32x4 sc = *(const f32x4*)(scales + gr * CH_HALF + 32 * kt + 8 * b + 4 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) S[kt][4 * b + e] += y[4 * b + e] * sc[e];
-                    }
-                }
-        }
-        // Element i of block kt: slot base + 32 kt + 8 (i / 4) + 4 h + i % 4.
-        const int4 ok = *(const int4*)(tile_ok + (it & 1) * 8 + 4 * par);
-        const bool all_there = (ok.x & ok.y & ok.z & ok.w) != 0;
-        const bool masked = __builtin_amdgcn_readfirstlane(base + CH_HALF - 1 > w_first || !all_there);
-        if (masked) {
-            const int there[4] = {ok.x, ok.y, ok.z, ok.w};
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (base + 32 * kt + 8 * (i / 4) + 4 * h + i % 4 > row.last || !there[2 * kt + i / 8]) S[kt][i] = NEG_INF;
-        }
+    };
+    auto block_max = [&](const f32x16& S) __attribute__((always_inline)) {
         float mb = NEG_INF;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mb = fmaxf(mb, S[kt][i] * qc);
-        mb = max_x2(mb);
-        const float m_new = fmaxf(m, mb);
-        const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-        const float sub_m = m_new == NEG_INF ? 0.f : m_new - P_SHIFT;
-        m = m_new;
-        l *= corr;
-        if (__builtin_amdgcn_ballot_w64(corr != 1.f)) {
+        for (int i = 0; i < 16; ++i) mb = fmaxf(mb, S[i]);
+        return mb;
+    };
+    // The maximum that is subtracted follows the true one when that is more than 2^P_SLACK ahead.
+    auto follow_max = [&](float mb) __attribute__((always_inline)) {
+        mb = max_x2(mb) * qc;
+        if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK)) {
+            asm volatile("");
+            const float m_new = fmaxf(m, mb);
+            const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= corr;
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) O[dt] *= corr;
         }
-        v8h Ph[EXACT ? 1 : 4], Pl[HL && !EXACT ? 4 : 1];
-        float P[EXACT ? 32 : 1];
+    };
+    // One half of an iteration: scores, their softmax, values, written in the order in which it is to be
+    // issued.  Operands are read six (K) and eight (V) products ahead, the exponentials of 16 slots are among
+    // the products of the 16 before; the denominator sums the probabilities as the products take them.
+    auto half_step = [&](int it) __attribute__((always_inline)) {
+        f32x16 S[2] = {f32x16{}, f32x16{}};
+        const uint32_t st = (it & 1) * 2 * CH_MAT;
+        v8h kf[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int k = 0; k < 6; ++k) kf[k] = k_operand(st + (k % 2) * 32 * HD * 2, k / 2);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            if (k + 6 < 16) kf[(k + 6) % 8] = k_operand(st + (k % 2) * 32 * HD * 2, (k + 6) / 2);
+            S[k % 2] = mfma32(kf[k % 8], Qh[k / 2], S[k % 2]);
+            if constexpr (HL) S[k % 2] = mfma32(kf[k % 8], Ql[k / 2], S[k % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        mask(it, 0, S[0]);
+        mask(it, 1, S[1]);
+        v8h vf[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) vf[k] = v_operand(st, k / 4, k % 4);
+        follow_max(fmaxf(block_max(S[0]), block_max(S[1])));
+        const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
+        const f16x2 ones = {(f16)1.f, (f16)1.f};
+        float sum[2] = {0.f, 0.f};
+        v8h hi[4], lo[HL ? 4 : 1];
+        auto exponentials = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float p = __builtin_amdgcn_exp2f(S[c / 2][8 * (c % 2) + e] * qc - sub_m);
-                l += p;
-                if constexpr (EXACT) {
-                    P[8 * c + e] = p;
-                } else {
-                    Ph[c][e] = (f16)p;
-                    if constexpr (HL) Pl[c][e] = (f16)(p - (float)Ph[c][e]);
-                }
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[c / 2][8 * (c % 2) + e], qc, -sub_m));
+                hi[c][e] = (f16)p;
+                if constexpr (HL) lo[c][e] = (f16)(p - (float)hi[c][e]);
             }
-        // V^T operand of dims 32 dt + c32 over slots 16 c + 4 h + {0 .. 3, 8 .. 11}.
-        auto v_operand = [&](int c, int dt) {
-            v4s half[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int r = 16 * c + 8 * k + 4 * h + ((lane & 15) >> 2);
-                const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(
-                    Vs + r * (HD * 2) + ((chunk ^ swizzle(r)) << 4) + 8 * (lane & 1)));
-            }
-            return __builtin_bit_cast(v8h, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
         };
-        if constexpr (!EXACT) {
+        exponentials(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+        for (int k = 0; k < 16; ++k) {
+            const int c = k / 4, dt = k % 4;
+            if (dt == 0 && c < 3) exponentials(c + 1);
+            O[dt] = mfma32(vf[k % 8], hi[c], O[dt]);
+            if constexpr (HL) O[dt] = mfma32(vf[k % 8], lo[c], O[dt]);
+            sum[dt % 2] = dot2(f16x2{hi[c][2 * dt], hi[c][2 * dt + 1]}, ones, sum[dt % 2]);
+            if constexpr (HL) sum[dt % 2] = dot2(f16x2{lo[c][2 * dt], lo[c][2 * dt + 1]}, ones, sum[dt % 2]);
+            if (k + 8 < 16) vf[k % 8] = v_operand(st, (k + 8) / 4, (k + 8) % 4);
+            if (dt == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum[0] + sum[1];
+    };
+    // q8 with fp32 queries.  Scores of 32-slot block kt of iteration it's half: a group's sum of codes takes
+    // its slot's scale.
+    auto exact_scores = [&](int it, int kt) __attribute__((always_inline)) {
+        const uint32_t Ks = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
+        const float* scales = scales_at(it & 1, par);
+        f32x16 S = {};
 #pragma unroll
-                for (int dt = 0; dt < 4; ++dt) {
-                    const v8h v = v_operand(c, dt);
-                    O[dt] = mfma32(v, Ph[c], O[dt]);
-                    if constexpr (HL) O[dt] = mfma32(v, Pl[c], O[dt]);
-                }
-        } else {
+        for (int gr = 0; gr < NG; ++gr) {
+            f32x16 y = {};
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-                // The tile's dims are one group: its scales, by the power of two that brings the half's largest
-                // below 1, go to the probabilities, and the power to the sum.
-                const f32x4 tops = *(const f32x4*)(scales + 8 * CH_HALF + 4 * dt);
-                const int e2 = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-                const float down = ldexpf(1.f, -e2), up = ldexpf(1.f, e2);
-                f32x16 y = {};
+            for (int ks = 2 * gr; ks < 2 * gr + 2; ++ks) {
+                const v8h kf = k_operand(Ks, ks);
+                y = mfma32(kf, Qh[ks], y);
+                y = mfma32(kf, Ql[HL ? ks : 0], y);
+            }
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    v8h ph, pl;
+            for (int b = 0; b < 4; ++b) {
+                const f32x4 sc = *(const f32x4*)(scales + gr * CH_HALF + 32 * kt + 8 * b + 4 * h);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const f32x4 sc = *(const f32x4*)(scales + 4 * CH_HALF + dt * CH_HALF + 16 * c + 8 * k + 4 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = P[8 * c + 4 * k + e] * (sc[e] * down);
-                            ph[4 * k + e] = (f16)x;
-                            pl[4 * k + e] = (f16)(x - (float)ph[4 * k + e]);
-                        }
-                    }
-                    const v8h v = v_operand(c, dt);
-                    y = mfma32(v, ph, y);
-                    y = mfma32(v, pl, y);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) O[dt][i] += up * y[i];
+                for (int e = 0; e < 4; ++e) S[4 * b + e] += y[4 * b + e] * sc[e];
             }
         }
-        // Values that are no numbers were kept out of the products: they go to the rows that see them.
-        if (base + CH_HALF - 1 > w_first || FMT == FMT_Q8) {
-            const int4 odd = *(const int4*)(tile_ok + 16 + (it & 1) * 8 + 4 * par);
-            if (__builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w))
-                for (int j = 0; j < CH_HALF && base + j < lim; ++j) {
-                    const int r = seq_slot_row(a.map, table, a.table_width, base + j);
-                    if (r < 0) continue;
+        return S;
+    };
+    // Its values: a block's dims 32 dt .. + 31 are one group, whose scales, by the power of two that brings the
+    // half's largest below 1, go to the probabilities, and the power to the sum.
+    auto exact_values = [&](int it, int kt, const f32x16& S) __attribute__((always_inline)) {
+        const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
+        const uint32_t Vs = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
+        const float* scales = scales_at(it & 1, par);
+        float p[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
+        for (int i = 0; i < 16; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], qc, -sub_m));
+            l += p[i];
+        }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = row_value<FMT>(a, (int64_t)r + g * a.map.page_slots, 32 * (k / 4) + 8 * (k % 4) + 4 * h + e);
-                            if (base + j <= row.last && !(fabsf(x) < __builtin_inff())) O[k / 4][4 * (k % 4) + e] += x;
-                        }
+        for (int dt = 0; dt < 4; ++dt) {
+            const f32x4 tops = *(const f32x4*)(scales + 8 * CH_HALF + 4 * dt);
+            const int e2 = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+            const float down = ldexpf(1.f, -e2), up = ldexpf(1.f, e2);
+            f32x16 y = {};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                v8h ph, pl;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f32x4 sc = *(const f32x4*)(scales + 4 * CH_HALF + dt * CH_HALF + 32 * kt + 16 * c + 8 * k + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = p[8 * c + 4 * k + e] * (sc[e] * down);
+                        ph[4 * k + e] = (f16)x;
+                        pl[4 * k + e] = (f16)(x - (float)ph[4 * k + e]);
+                    }
+                }
+                const v8h v = v_operand(Vs, c, dt);
+                y = mfma32(v, ph, y);
+                y = mfma32(v, pl, y);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[dt][i] += up * y[i];
+        }
+    };
+    // Values that are no numbers were kept out of the products: they go to the rows that see them.
+    auto add_odd_values = [&](int it) __attribute__((always_inline)) {
+        const int base = base_of(it);
+        if (FMT == FMT_F16 && base + CH_HALF - 1 <= w_first) return;
+        const int4 odd = *(const int4*)(tile_odd + (it & 1) * 8 + 4 * par);
+        if (!__builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w)) return;
+        auto b = arguments();
+        const PageMap map = {b->map.n_pages, b->map.n_kv, b->map.page_slots};
+        for (int j = 0; j < CH_HALF && base + j < lim; ++j) {
+            const int r = seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, base + j);
+            if (r < 0) continue;
+            const uint32_t sees = base + j <= row.last ? 0xFFFFFFFFu : 0;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = as_u32(row_value<FMT>(b->v, b->v_sb, (int64_t)r + head_row, 32 * (k / 4) + 8 * (k % 4) + 4 * h + e));
+                    O[k / 4][4 * (k % 4) + e] += as_f32(x & sees & no_number(x));
                 }
         }
+    };
+    // Slots that some rows of the workgroup see and others do not may hold values that are no numbers: in
+    // iterations that have such slots each wave makes its tile of V finite.  (q8: when it is put to LDS.)
+    auto clean_values = [&](int it) __attribute__((always_inline)) {
+        if (it * 128 + 127 <= before + tile * CH_ROWS / group) return;
+        asm volatile("");
+        uint32_t odd = 0;
+        uint8_t* vt = lds + half_at(1, it & 1, par) + wi * 16 * HD * 2 + lane * 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v8h v = *(const v8h*)(vt + 1024 * k);
+            keep_finite(v, odd);
+            *(v8h*)(vt + 1024 * k) = v;
         }
-        if constexpr (FMT == FMT_Q8)
-            if (it + 1 < it1) put(it + 1);
+        const bool any = __ballot(odd != 0) != 0;
+        if (lane == 0) tile_odd[(it & 1) * 8 + wave] = any;
+        staged_barrier<63>();
+    };
+    // Iterations whose half some row of this wave sees.
+    const int my1 = active && base_of(it0) <= w_last ? min(it1, (w_last - CH_HALF * par) / 128 + 1) : it0;
+    auto stage = [&](int it) __attribute__((always_inline)) {
+        const int r = tile_row(it);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            if constexpr (FMT == FMT_F16)
+                copy(kv, it, r);
+            else
+                fetch(kv, it, r);
+        }
+    };
+    auto staged = [&](int it) __attribute__((always_inline)) {
+        if constexpr (FMT == FMT_Q8) {
+            put(0, it);
+            put(1, it);
+        }
+    };
+    if (it0 < it1) {
+        stage(it0);
+        staged(it0);
+    }
+    for (int it = it0; it < it1; ++it) {
+        staged_barrier<0>();
+        if (it + 1 < it1) stage(it + 1);
+        if constexpr (FMT == FMT_F16) clean_values(it);
+        if (it < my1) {
+            if constexpr (!EXACT) {
+                half_step(it);
+            } else {
+                f32x16 S[2] = {exact_scores(it, 0), exact_scores(it, 1)};
+                mask(it, 0, S[0]);
+                mask(it, 1, S[1]);
+                follow_max(fmaxf(block_max(S[0]), block_max(S[1])));
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) exact_values(it, kt, S[kt]);
+            }
+            add_odd_values(it);
+        }
+        if (it + 1 < it1) staged(it + 1);
     }
 
     // The halves' states join: waves 4 .. 7 hand theirs to waves 0 .. 3.
-    staged_barrier();
+    staged_barrier<0>();
     f32x4* const mo = (f32x4*)lds;                          // [4 waves][16][64 lanes]
     float2* const mml = (float2*)(lds + 4 * 16 * 64 * 16);  // [4 waves][64 lanes]
     l = swap32_add(l, l);
@@ -991,7 +1083,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             mo[(wi * 16 + k) * 64 + lane] = f32x4{O[k / 4][4 * (k % 4)], O[k / 4][4 * (k % 4) + 1], O[k / 4][4 * (k % 4) + 2], O[k / 4][4 * (k % 4) + 3]};
         mml[wi * 64 + lane] = make_float2(m, l);
     }
-    staged_barrier();
+    staged_barrier<0>();
     if (par == 1 || row.t < 0) return;
     const float2 ml = mml[wi * 64 + lane];
     const float mt = fmaxf(m, ml.x);
