@@ -1743,6 +1743,7 @@ int icua_paged_store(const icua_pages_t* pages, const icua_paged_store_t* args, 
     if (!type_ok(args->type) || !type_ok(args->q_type)) return fail("paged_store: bad type");
     if (args->n_tokens < 0) return fail("paged_store: negative n_tokens");
     if (args->n_heads < 0 || args->n_heads > 16384) return fail("paged_store: n_heads must be in 0..16384");
+    if ((int64_t)args->n_tokens * (args->n_heads + 2 * a.map.n_kv) > (1 << 27)) return fail("paged_store: more than 2^27 (token, head) rows");
     a.n_tokens = args->n_tokens;
     a.n_heads = args->n_heads;
     a.qkv_stride = args->qkv_stride;
@@ -1791,7 +1792,8 @@ static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention
         return fail("paged_attention: n_heads must be a multiple of n_kv, at most 16 for each");
     if (args->n_seqs < 0 || args->n_tokens < 0 || args->max_q < 0 || args->max_kv < 0)
         return fail("paged_attention: negative size");
-    if (args->n_seqs > (1 << 20) || args->n_tokens > (1 << 24)) return fail("paged_attention: more than 2^20 sequences or 2^24 tokens");
+    if ((int64_t)args->n_seqs * a.map.n_kv > (1 << 21) || (int64_t)args->n_tokens * args->n_heads > (1 << 26))
+        return fail("paged_attention: more than 2^21 (sequence, KV head) pairs or 2^26 (token, head) rows");
     if (args->table_width < 1 || args->table_width > INT32_MAX / 2 / a.map.page_slots)
         return fail("paged_attention: table_width must be positive and its pages hold fewer than 2^30 slots");
     const int slots = args->table_width * a.map.page_slots;
@@ -1857,6 +1859,7 @@ int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, vo
     if (pages_check(pages, a.map, true)) return -1;
     if (!type_ok(args->type)) return fail("paged_load: bad type");
     if (args->n_rows < 0) return fail("paged_load: negative n_rows");
+    if ((int64_t)args->n_rows * a.map.n_kv > (1 << 27)) return fail("paged_load: more than 2^27 (row, head) pairs");
     a.token_stride = args->token_stride;
     a.head_stride = args->head_stride;
     if (a.token_stride == 0 && a.head_stride == 0) {

@@ -264,57 +264,41 @@ __device__ __forceinline__ Query<TYPE> load_query(const PagedAttnArgs& a, const 
 
 __device__ __forceinline__ f32x4 mfma(v8h a, v8h b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// Two 16-slot tiles of K or V as a lane reads them from memory (K: slot r16, dims 32 ks + 8 q .. + 7;
-// V: slots 4 q .. + 3, dims 8 r16 .. + 7), with a scale for each 8 values (q8).
+// A 16-slot tile of K or V as a lane reads it from memory (K: slot r16, dims 32 ks + 8 q .. + 7; V: slots
+// 4 q .. + 3, dims 8 r16 .. + 7), with q8 scales (K: slots 4 q .. + 3, four each; V: of its 8 dims).
 template <int FMT>
-struct KTile {
-    u32x4 w[4];
+struct Tile {
+    u32x4 k[4], v[4];
 };
 template <>
-struct KTile<FMT_Q8> {
-    u32x2 w[4];
-    u32x4 s[2];  // scales of slots 4 q .. + 3, four each
+struct Tile<FMT_Q8> {
+    u32x2 k[4], v[4];
+    u32x4 ks[2];
+    uint16_t vs[4];
 };
 template <int FMT>
-struct VTile {
-    u32x4 w[4];
-};
-template <>
-struct VTile<FMT_Q8> {
-    u32x2 w[4];
-    uint16_t s[4];
-};
-
-template <int FMT>
-__device__ __forceinline__ void load_k(const PagedAttnArgs& a, int row, int lane, KTile<FMT>& t) {
+__device__ __forceinline__ void load_tile(const PagedAttnArgs& a, int row, int lane, Tile<FMT>& t) {
     const int q = lane >> 4, r16 = lane & 15;
     if constexpr (FMT == FMT_F16) {
-        const uint8_t* p = (const uint8_t*)a.k + (int64_t)row * (HD * 2) + r16 * (HD * 2) + q * 16;
+        const uint8_t* k = (const uint8_t*)a.k + (int64_t)row * (HD * 2) + r16 * (HD * 2) + q * 16;
+        const uint8_t* v = (const uint8_t*)a.v + (int64_t)row * (HD * 2) + q * 4 * (HD * 2) + r16 * 16;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) t.w[ks] = *(const u32x4*)(p + 64 * ks);
+        for (int i = 0; i < 4; ++i) t.k[i] = *(const u32x4*)(k + 64 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t.v[i] = *(const u32x4*)(v + i * HD * 2);
     } else {
-        const uint8_t* p = (const uint8_t*)a.k + (int64_t)row * HD + r16 * HD + q * 8;
+        const uint8_t* k = (const uint8_t*)a.k + (int64_t)row * HD + r16 * HD + q * 8;
+        const uint8_t* ks = (const uint8_t*)a.k_sb + (int64_t)row * (NG * 2) + q * 32;
+        const uint8_t* v = (const uint8_t*)a.v + (int64_t)row * HD + q * 4 * HD + r16 * 8;
+        const uint16_t* vs = (const uint16_t*)a.v_sb + (int64_t)row * NG + q * 4 * NG + r16 / 4;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) t.w[ks] = *(const u32x2*)(p + 32 * ks);
-        const uint8_t* s = (const uint8_t*)a.k_sb + (int64_t)row * (NG * 2) + q * 32;
-        t.s[0] = *(const u32x4*)s;
-        t.s[1] = *(const u32x4*)(s + 16);
-    }
-}
-template <int FMT>
-__device__ __forceinline__ void load_v(const PagedAttnArgs& a, int row, int lane, VTile<FMT>& t) {
-    const int q = lane >> 4, r16 = lane & 15;
-    if constexpr (FMT == FMT_F16) {
-        const uint8_t* p = (const uint8_t*)a.v + (int64_t)row * (HD * 2) + q * 4 * (HD * 2) + r16 * 16;
+        for (int i = 0; i < 4; ++i) t.k[i] = *(const u32x2*)(k + 32 * i);
+        t.ks[0] = *(const u32x4*)ks;
+        t.ks[1] = *(const u32x4*)(ks + 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t.w[j] = *(const u32x4*)(p + j * HD * 2);
-    } else {
-        const uint8_t* p = (const uint8_t*)a.v + (int64_t)row * HD + q * 4 * HD + r16 * 8;
+        for (int i = 0; i < 4; ++i) t.v[i] = *(const u32x2*)(v + i * HD);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t.w[j] = *(const u32x2*)(p + j * HD);
-        const uint16_t* s = (const uint16_t*)a.v_sb + (int64_t)row * NG + q * 4 * NG + r16 / 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t.s[j] = s[j * NG];
+        for (int i = 0; i < 4; ++i) t.vs[i] = vs[i * NG];
     }
 }
 
@@ -337,70 +321,65 @@ __device__ __forceinline__ void keep_finite(v8h& v, uint32_t& odd) {
     v = fin;
 }
 
-// Eight int8 codes as exact fp16 values.
-__device__ __forceinline__ v8h codes_f16(u32x2 c) {
-    v8h y;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = (f16)(float)(int8_t)(c[k / 4] >> (8 * (k % 4)));
-    return y;
-}
-
 // Scores of a tile, products with the column's query: fp16 rows directly; q8 codes are exact in fp16
 // and a 32-value group is one product's depth, so each group's sum takes its scale in fp32.
 template <int TYPE, int FMT>
-__device__ __forceinline__ f32x4 tile_scores(const KTile<FMT>& t, const Query<TYPE>& y) {
+__device__ __forceinline__ f32x4 tile_scores(const Tile<FMT>& t, const Query<TYPE>& y) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
         if constexpr (FMT == FMT_F16) {
-            const v8h k = __builtin_bit_cast(v8h, t.w[ks]);
+            const v8h k = __builtin_bit_cast(v8h, t.k[ks]);
             s = mfma(k, y.hi[ks], s);
             if constexpr (TYPE == TYPE_F32) s = mfma(k, y.lo[ks], s);
         } else {
-            const v8h k = codes_f16(t.w[ks]);
+            f16x2 c[4];
+            codes_h2(t.k[ks][0], c);
+            codes_h2(t.k[ks][1], c + 2);
+            const v8h k = {c[0].x, c[0].y, c[1].x, c[1].y, c[2].x, c[2].y, c[3].x, c[3].y};
             f32x4 p = mfma(k, y.hi[ks], f32x4{0.f, 0.f, 0.f, 0.f});
             if constexpr (TYPE == TYPE_F32) p = mfma(k, y.lo[ks], p);
-            // The scale of slot 4 q + i, group ks: half 4 i + ks of t.s.
+            // The scale of slot 4 q + i, group ks: half 4 i + ks of t.ks.
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                s[i] += p[i] * h2f((uint16_t)(t.s[i / 2][2 * (i % 2) + ks / 2] >> (16 * (ks % 2))));
+                s[i] = __builtin_fmaf(p[i], h2f((uint16_t)(t.ks[i / 2][2 * (i % 2) + ks / 2] >> (16 * (ks % 2)))), s[i]);
         }
     }
     return s;
 }
 
-// The V^T operands of two tiles: dims 8 r16 + dt over this lane's eight slots (4 q .. + 3 of each tile),
-// hi and, for q8 with fp32 queries, lo parts of the exact products code x scale.
+// The V^T operand dims 8 r16 + dt of two tiles over this lane's eight slots (4 q .. + 3 of each tile), hi
+// and, for q8 with fp32 queries, the lo part of the exact product code x scale.
 template <int TYPE, int FMT>
-struct VOps {
+struct VOp {
     static constexpr bool LO = FMT == FMT_Q8 && TYPE == TYPE_F32;
-    v8h hi[8], lo[LO ? 8 : 1];
+    v8h hi, lo;
 };
 template <int TYPE, int FMT>
-__device__ __forceinline__ void v_operands(const VTile<FMT>* t, VOps<TYPE, FMT>& o) {
-    if constexpr (FMT == FMT_F16) {
-        // Word w of output dim 2 w (+ 1): the low (high) halves of word w of two rows, one byte select.
+__device__ __forceinline__ VOp<TYPE, FMT> v_operand(const Tile<FMT>* t, int dt) {
+    VOp<TYPE, FMT> o;
+    u32x4 hi, lo;
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-            u32x4 y;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                y[j] = __builtin_amdgcn_perm(t[j / 2].w[2 * (j % 2) + 1][dt / 2], t[j / 2].w[2 * (j % 2)][dt / 2],
-                                             dt % 2 ? 0x07060302u : 0x05040100u);
-            o.hi[dt] = __builtin_bit_cast(v8h, y);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float s = h2f(t[j / 4].s[j % 4]);
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt) {
-                const float v = s * (float)(int8_t)(t[j / 4].w[j % 4][dt / 4] >> (8 * (dt % 4)));
-                o.hi[dt][j] = (f16)v;
-                if constexpr (VOps<TYPE, FMT>::LO) o.lo[dt][j] = (f16)(v - (float)o.hi[dt][j]);
-            }
+    for (int j = 0; j < 4; ++j) {  // slots 2 j, 2 j + 1 of the eight
+        const Tile<FMT>& x = t[j / 2];
+        const int r = 2 * (j % 2);
+        if constexpr (FMT == FMT_F16) {
+            // The low (even dt) or high halves of a word of two rows: one byte select.
+            hi[j] = __builtin_amdgcn_perm(x.v[r + 1][dt / 2], x.v[r][dt / 2], dt % 2 ? 0x07060302u : 0x05040100u);
+        } else {
+            // Byte dt % 4 of both rows' words (sign flipped before) under the exponent of 1024, less 1152.
+            const uint32_t sel = 0x0C000C00u | (uint32_t)(dt % 4) | (uint32_t)(4 + dt % 4) << 16;
+            const f16x2 bias = {(f16)1152.f, (f16)1152.f};
+            const f16x2 c = as_h2(__builtin_amdgcn_perm(x.v[r + 1][dt / 4], x.v[r][dt / 4], sel) | 0x64006400u) - bias;
+            const f16x2 s = as_h2((uint32_t)x.vs[r] | (uint32_t)x.vs[r + 1] << 16);
+            const f16x2 h = c * s;
+            hi[j] = h2_bits(h);
+            if constexpr (VOp<TYPE, FMT>::LO) lo[j] = h2_bits(__builtin_elementwise_fma(c, s, -h));  // exact
         }
     }
+    o.hi = __builtin_bit_cast(v8h, hi);
+    if constexpr (VOp<TYPE, FMT>::LO) o.lo = __builtin_bit_cast(v8h, lo);
+    return o;
 }
 
 // Value d of a row of V, as the products take it.
@@ -410,162 +389,192 @@ __device__ __forceinline__ float row_value(const void* v, const void* v_sb, int6
     return (float)(f16)(h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d]);
 }
 
-template <int TYPE, int FMT>
-__device__ __forceinline__ f32x4 pv(const VOps<TYPE, FMT>& v, int dt, v8h ph, v8h pl, f32x4 c) {
-    c = mfma(v.hi[dt], ph, c);
-    if constexpr (TYPE == TYPE_F32) c = mfma(v.hi[dt], pl, c);
-    if constexpr (VOps<TYPE, FMT>::LO) c = mfma(v.lo[dt], ph, c);
-    return c;
-}
+// Sequences with at most 16 query rows a KV head (single tokens, drafts): a workgroup of NW waves has a
+// (sequence, KV head) and a range of its slots, its waves take 32-slot steps of it in turn and join
+// through LDS.  K and V go from memory to registers, as each is used by one tile alone, a step ahead of
+// its products.  Bound by memory.
+constexpr int ROWS_TILE = 16, ROWS_STEP = 32;
+template <int NW>
+constexpr size_t rows_lds() { return NW * (8 * WAVE * 16 + 16 * 8); }
 
-// Sequences with at most 16 query rows a KV head (single tokens, drafts): a workgroup has a (sequence, KV
-// head) and a range of its slots, its four waves take 32-slot steps of it in turn and join through LDS.
-// K and V go from memory to registers: each is used by one tile alone.  Bound by memory.
-constexpr int ROWS_TILE = 16, ROWS_STEP = 32, ROWS_SUB = WAVE * PAGED_TILE;
-
-template <int TYPE, int FMT>
-__global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a) {
-    __shared__ f32x4 so[4][8][WAVE];
-    __shared__ float sm[4][16], sl[4][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r16 = lane & 15;
-    const int g = blockIdx.y, split = blockIdx.z, group = a.n_heads / a.map.n_kv;
-    const int s = blockIdx.x;
+template <int TYPE, int FMT, int NW>
+__device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uint8_t* lds) {
+    // fp32 probabilities and, so that only the output's rounding counts, those of q8 in two parts.
+    constexpr bool PLO = TYPE == TYPE_F32 || FMT == FMT_Q8, VLO = VOp<TYPE, FMT>::LO;
+    f32x4* const so = (f32x4*)lds;                        // [NW][8][64]
+    float2* const sml = (float2*)(lds + NW * 8 * WAVE * 16);  // [NW][16]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
+    const int split = index % a.rows.n, g = index / a.rows.n % a.map.n_kv, s = index / a.rows.n / a.map.n_kv;
+    const int group = a.n_heads / a.map.n_kv;
+    const int32_t* table = a.tables + (int64_t)s * a.table_width;
+    // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).  Looked up
+    // before the sequence's lengths are there.
+    auto step_slot = [&](int sub, int i) { return sub + ROWS_STEP * (wave + NW * i); };
+    auto lookup = [&](int sub) {
+        const int slot = step_slot(sub, lane / 2) + PAGED_TILE * (lane % 2);
+        return slot < a.max_kv ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
+    };
+    constexpr int SUB = NW * ROWS_STEP * (WAVE / 2);
+    const int start = split * a.rows.chunk;
+    int rows = lookup(start);
     const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
-    if (sp.n_q == 0 || sp.n_q * group > ROWS_TILE) return;  // the others are paged_chunk_kernel's
+    if (sp.n_q == 0 || sp.n_q * group > ROWS_TILE) return;  // the others are the chunk kernel's
     const RowOf row = row_of(sp, r16, group, g);
     // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
-    const int lim = sp.n_kv, all = sp.n_kv - sp.n_q;
-    const int c0 = min(lim, split * a.rows.chunk), c1 = min(lim, c0 + a.rows.chunk);
+    const int lim = sp.n_kv, all = sp.n_kv - sp.n_q, c1 = min(lim, start + a.rows.chunk);
 
-    const Query<TYPE> y = load_query<TYPE>(a, row, q);
     f32x4 O[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = NEG_INF, l = 0.f;
-    const int32_t* table = a.tables + (int64_t)s * a.table_width;
-    for (int sub = c0; sub < c1; sub += ROWS_SUB) {
-        // Lane i: the pool row of the range's tile i (-1: beyond the range, or no such page).
-        int rows = -1;
-        if (sub + lane * PAGED_TILE < c1) rows = seq_slot_row(a.map, table, a.table_width, sub + lane * PAGED_TILE);
-        const int end = min(c1, sub + ROWS_SUB);
-        for (int at = sub + wave * ROWS_STEP; at < end; at += 4 * ROWS_STEP) {
-            KTile<FMT> kt[2];
-            VTile<FMT> vt[2];
-            int ok[2];
+    int sub = start;
+    auto fetch = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int r = __builtin_amdgcn_readlane(rows, (at - sub) / PAGED_TILE + t);
-                ok[t] = r < 0 ? 0 : lim;  // slots from here on are not there
-                const int base = max(r, 0) + g * a.map.page_slots;
-                load_k<FMT>(a, base, lane, kt[t]);
-                load_v<FMT>(a, base, lane, vt[t]);
-            }
-            float p[8], mb = NEG_INF;
+        for (int k = 0; k < 2; ++k)
+            load_tile<FMT>(a, max(__builtin_amdgcn_readlane(rows, 2 * i + k), 0) + g * a.map.page_slots, lane, t[k]);
+    };
+    const Query<TYPE> y = load_query<TYPE>(a, row, q);
+    auto step = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
+        const int at = step_slot(sub, i);
+        const int ok[2] = {__builtin_amdgcn_readlane(rows, 2 * i) < 0 ? 0 : lim, __builtin_amdgcn_readlane(rows, 2 * i + 1) < 0 ? 0 : lim};
+        float p[8];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const f32x4 sc = tile_scores<TYPE, FMT>(kt[t], y);
+        for (int k = 0; k < 2; ++k) {
+            const f32x4 sc = tile_scores<TYPE, FMT>(t[k], y);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int slot = at + 16 * t + 4 * q + i;
-                    p[4 * t + i] = slot > row.last || slot >= ok[t] ? NEG_INF : sc[i] * y.c;
-                    mb = fmaxf(mb, p[4 * t + i]);
+            for (int e = 0; e < 4; ++e) p[4 * k + e] = sc[e] * y.c;
+        }
+        uint32_t odd = 0;
+        const bool masked = at + ROWS_STEP - 1 > all || ok[0] == 0 || ok[1] == 0;
+        if (masked) {
+            asm volatile("");
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int slot = at + 16 * k + 4 * q + e;
+                    if (slot > row.last || slot >= ok[k]) p[4 * k + e] = NEG_INF;
+                    // Values of slots that no row sees may be anything: they take no part.
+                    if (slot >= ok[k]) {
+                        t[k].v[e] = 0;
+                        if constexpr (FMT == FMT_Q8) t[k].vs[e] = 0;
+                    }
                 }
-            }
-            mb = max_x4(mb);
+        }
+        float mb = NEG_INF;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mb = fmaxf(mb, p[e]);
+        mb = max_x4(mb);
+        if (__ballot(mb > m + P_SLACK)) {
+            asm volatile("");
             const float m_new = fmaxf(m, mb);
             const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-            const float base = m_new == NEG_INF ? 0.f : m_new - P_SHIFT;
             m = m_new;
-            v8h ph, pl;
             l *= corr;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = __builtin_amdgcn_exp2f(p[i] - base);
-                l += e;
-                ph[i] = (f16)e;
-                pl[i] = TYPE == TYPE_F32 ? (f16)(e - (float)ph[i]) : (f16)0.f;
-            }
-            // Values of slots that no row sees may be anything: they take no part.
-            if (at + ROWS_STEP > min(ok[0], ok[1]))
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (at + 16 * t + 4 * q + j >= ok[t]) {
-                            vt[t].w[j] = 0;
-                            if constexpr (FMT == FMT_Q8) vt[t].s[j] = 0;
-                        }
-            VOps<TYPE, FMT> vo;
-            v_operands<TYPE, FMT>(vt, vo);
-#pragma unroll
             for (int dt = 0; dt < 8; ++dt) O[dt] *= corr;
-            // Slots that some rows see and others do not: values there that are no numbers are kept out of the
-            // products and go to the rows that see them.
-            uint32_t odd = 0;
-            if (at + ROWS_STEP - 1 > all)
+        }
+        const float base = m == NEG_INF ? 0.f : m - P_SHIFT;
+        v8h ph, pl;
 #pragma unroll
-                for (int dt = 0; dt < 8; ++dt) {
-                    keep_finite(vo.hi[dt], odd);
-                    if constexpr (VOps<TYPE, FMT>::LO) keep_finite(vo.lo[dt], odd);
-                }
+        for (int e = 0; e < 8; ++e) {
+            const float x = __builtin_amdgcn_exp2f(p[e] - base);
+            l += x;
+            ph[e] = (f16)x;
+            if constexpr (PLO) pl[e] = (f16)(x - (float)ph[e]);
+        }
+        if constexpr (FMT == FMT_Q8)
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) O[dt] = pv<TYPE, FMT>(vo, dt, ph, pl, O[dt]);
-            if (__ballot(odd != 0))
-                for (int j = 0; j < ROWS_STEP; ++j) {
-                    const int r = __builtin_amdgcn_readlane(rows, (at - sub + j) / PAGED_TILE);
-                    if (r < 0 || at + j >= lim) continue;
-                    const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
-                    const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                for (int e = 0; e < 4; ++e) t[k].v[e] ^= 0x80808080u;
+        // Slots that some rows see and others do not: values there that are no numbers are kept out of the
+        // products and go to the rows that see them.
 #pragma unroll
-                        for (int dt = 0; dt < 8; ++dt) {
-                            const uint32_t x = as_u32(row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * i + dt));
-                            O[dt][i] += as_f32(x & sees & no_number(x));
-                        }
-                }
+        for (int dt = 0; dt < 8; ++dt) {
+            VOp<TYPE, FMT> v = v_operand<TYPE, FMT>(t, dt);
+            if (masked) {
+                keep_finite(v.hi, odd);
+                if constexpr (VLO) keep_finite(v.lo, odd);
+            }
+            O[dt] = mfma(v.hi, ph, O[dt]);
+            if constexpr (PLO) O[dt] = mfma(v.hi, pl, O[dt]);
+            if constexpr (VLO) O[dt] = mfma(v.lo, ph, O[dt]);
+        }
+        if (__ballot(odd != 0))
+            for (int j = 0; j < ROWS_STEP; ++j) {
+                const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);
+                if (r < 0 || at + j >= lim) continue;
+                const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
+                const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int dt = 0; dt < 8; ++dt) {
+                        const uint32_t x = as_u32(row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * e + dt));
+                        O[dt][e] += as_f32(x & sees & no_number(x));
+                    }
+            }
+    };
+    for (; sub < c1; sub += SUB) {
+        if (sub != start) rows = lookup(sub);
+        // This wave's steps of the window that begin below c1.
+        const int left = c1 - step_slot(sub, 0);
+        const int n = left <= 0 ? 0 : min(WAVE / 2, (left + NW * ROWS_STEP - 1) / (NW * ROWS_STEP));
+        Tile<FMT> A[2], B[2];
+        if (n > 0) fetch(0, A);
+        for (int i = 0; i < n; i += 2) {
+            if (i + 1 < n) fetch(i + 1, B);
+            step(i, A);
+            if (i + 1 < n) {
+                if (i + 2 < n) fetch(i + 2, A);
+                step(i + 1, B);
+            }
         }
     }
     // Join the waves: lane (r16, q) of each has dims 8 (4 q + i) + dt of row r16.
     l = sum_x4(l);
-    if (q == 0) {
-        sm[wave][r16] = m;
-        sl[wave][r16] = l;
-    }
+    if (q == 0) sml[wave * 16 + r16] = make_float2(m, l);
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) so[wave][dt][lane] = O[dt];
+    for (int dt = 0; dt < 8; ++dt) so[(wave * 8 + dt) * WAVE + lane] = O[dt];
     __syncthreads();
-    float mt = NEG_INF, lt = 0.f, f[4];
+    float mt = NEG_INF, lt = 0.f, f[NW];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, sm[w][r16]);
+    for (int w = 0; w < NW; ++w) mt = fmaxf(mt, sml[w * 16 + r16].x);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = sm[w][r16] == mt ? 1.f : __builtin_amdgcn_exp2f(sm[w][r16] - mt);
-        lt += sl[w][r16] * f[w];
+    for (int w = 0; w < NW; ++w) {
+        const float2 ml = sml[w * 16 + r16];
+        f[w] = ml.x == mt ? 1.f : __builtin_amdgcn_exp2f(ml.x - mt);
+        lt += ml.y * f[w];
     }
     if (row.t < 0) return;
-    // Wave w writes dims 8 (4 q + i) + 2 w, + 1.
-    const float inv = a.rows.n > 1 ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+    // Wave w writes dims 8 (4 q + i) + dt, its 8 / NW of dt.
+    const bool whole = a.rows.n == 1;
+    const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
     const int64_t out_row = (int64_t)row.t * a.n_heads + row.head;
+    constexpr int ND = 8 / NW;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float y2[2] = {0.f, 0.f};
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int k = 0; k < ND; ++k) {
+            const int dt = ND * wave + k, d = 8 * (4 * q + i) + dt;
+            float x = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) y2[h] += so[w][2 * wave + h][lane][i] * f[w];
-        const int d = 8 * (4 * q + i) + 2 * wave;
-        if (a.rows.n > 1) {
-            *(float2*)(a.part + (out_row * a.part_splits + split) * HD + d) = make_float2(y2[0], y2[1]);
-        } else {
-            const int64_t o = (int64_t)row.t * a.out_stride + row.head * HD + d;
-            if constexpr (TYPE == TYPE_F32)
-                *(float2*)((float*)a.out + o) = make_float2(y2[0] * inv, y2[1] * inv);
+            for (int w = 0; w < NW; ++w) x += so[(w * 8 + dt) * WAVE + lane][i] * f[w];
+            if (!whole)
+                a.part[(out_row * a.part_splits + split) * HD + d] = x;
+            else if constexpr (TYPE == TYPE_F32)
+                ((float*)a.out)[(int64_t)row.t * a.out_stride + row.head * HD + d] = x * inv;
             else
-                *(f16x2*)((f16*)a.out + o) = f16x2{(f16)(y2[0] * inv), (f16)(y2[1] * inv)};
+                ((f16*)a.out)[(int64_t)row.t * a.out_stride + row.head * HD + d] = (f16)(x * inv);
         }
-    }
-    if (a.rows.n > 1 && wave == 0 && q == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
+    if (!whole && wave == 0 && q == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
+}
+
+template <int TYPE, int FMT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows_kernel(PagedAttnArgs a) {
+    __shared__ __align__(16) uint8_t lds[rows_lds<4>()];
+    rows_work<TYPE, FMT, 4>(a, blockIdx.x, lds);
 }
 
 // Sequences with more query rows: flash attention on 128 rows of a (sequence, KV head) a workgroup, eight
@@ -616,31 +625,30 @@ __device__ __forceinline__ void staged_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// The sequence and tile (of `rows` query rows a KV head) that workgroup tile `index` stands for, over the
-// sequences with more than ROWS_TILE rows; false past the last one.  One wave looks at 64 sequences at a time.
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int group, int rows, int index, int& s, int& tile, int& tiles) {
+// The sequence and tile (of `rows` query rows a KV head) that number `index` stands for, over the
+// sequences with more than ROWS_TILE rows; false past the last one.  A wave looks at 64 sequences at a time.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int group, int rows, int index, int& s, int& tile, int& tiles, SeqSpan& sp) {
     const int lane = threadIdx.x & 63;
     for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
-        int n = 0;
-        if (s0 + lane < a.n_seqs) {
-            n = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv).n_q * group;
-            n = n > ROWS_TILE ? (n + rows - 1) / rows : 0;
-        }
+        SeqSpan x = {0, 0, 0};
+        if (s0 + lane < a.n_seqs) x = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
+        const int n = x.n_q * group > ROWS_TILE ? (x.n_q * group + rows - 1) / rows : 0;
         int end = n;
 #pragma unroll
         for (int o = 1; o < WAVE; o <<= 1) {
-            const int x = __shfl_up(end, o);
-            if (lane >= o) end += x;
+            const int y = __shfl_up(end, o);
+            if (lane >= o) end += y;
         }
         const uint64_t past = __ballot(end > index);
         if (past) {
             const int first = __ffsll((unsigned long long)past) - 1;
-            tile = index - __shfl(end - n, first);
-            tiles = __shfl(n, first);
+            tile = index - __builtin_amdgcn_readlane(end - n, first);
+            tiles = __builtin_amdgcn_readlane(n, first);
+            sp = {__builtin_amdgcn_readlane(x.t0, first), __builtin_amdgcn_readlane(x.n_q, first), __builtin_amdgcn_readlane(x.n_kv, first)};
             s = s0 + first;
             return true;
         }
-        index -= __shfl(end, WAVE - 1);
+        index -= __builtin_amdgcn_readlane(end, WAVE - 1);
     }
     return false;
 }
@@ -653,12 +661,17 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int* const tile_there = tile_odd + 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
-    const int g = blockIdx.x % a.map.n_kv, at = blockIdx.x / a.map.n_kv, split = at % a.big.n;
+    // The first workgroups have the sequences of few rows: their reads run beside the others' products.
+    const int few = a.n_seqs * a.map.n_kv * a.rows.n, index = (int)blockIdx.x - few;
+    if (index < 0) {
+        rows_work<TYPE, FMT, 8>(a, blockIdx.x, lds);
+        return;
+    }
+    const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % a.big.n;
     int s, tile, tiles;
-    if (!find_tile(a, group, CH_ROWS, at / a.big.n, s, tile, tiles)) return;
-    s = __builtin_amdgcn_readfirstlane(s);
-    tile = __builtin_amdgcn_readfirstlane(tiles - 1 - tile);  // those that see the most slots first
-    const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
+    SeqSpan sp;
+    if (!find_tile(a, group, CH_ROWS, at / a.big.n, s, tile, tiles, sp)) return;
+    tile = tiles - 1 - tile;  // those that see the most slots first
     const int before = sp.n_kv - sp.n_q;  // token i sees slots up to before + i
     const int r0 = tile * CH_ROWS + 32 * wi;
     const bool active = r0 < sp.n_q * group;
@@ -1106,42 +1119,66 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (a.big.n > 1 && h == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
 }
 
-// Joins the splits of a row: one wave a row, two dims a lane.
+// Joins the splits of a row: 32 lanes have a split's 128 values, four each, so a wave reads two splits at a
+// time, eight loads in flight; all of them are independent of the weights.
+template <int TYPE>
+__device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int head, int nsplit) {
+    const int lane = threadIdx.x & 63, d = 4 * (lane & 31);
+    const int64_t row = (int64_t)t * a.n_heads + head;
+    const float* part = a.part + row * a.part_splits * HD + d;
+    float2 ml = make_float2(NEG_INF, 0.f);
+    if (lane < nsplit) ml = a.part_ml[row * a.part_splits + lane];
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float f = 0.f, m = 0.f, l = 0.f;
+    for (int i0 = 0; i0 < nsplit; i0 += 16) {
+        f32x4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = *(const f32x4*)(part + (int64_t)min(i0 + 2 * k + (lane >> 5), nsplit - 1) * HD);
+        if (i0 == 0) {
+            m = wave_max(ml.x);
+            f = ml.x == NEG_INF ? 0.f : ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+            l = wave_sum(ml.y * f);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + 2 * k + (lane >> 5);
+            const float w = i < nsplit ? __shfl(f, i) : 0.f;
+            if (w != 0.f) o += x[k] * w;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = swap32_add(o[e], o[e]);
+    const float inv = m == NEG_INF && l == 0.f ? 0.f : 1.f / l;
+    if (lane < 32) store4<TYPE>(a.out, (int64_t)t * a.out_stride + head * HD + d, o * inv);
+}
+
+// Where only sequences of few rows are split: a workgroup has a (sequence, KV head), a wave a row.
+template <int TYPE>
+__global__ __launch_bounds__(256) void paged_merge_rows_kernel(PagedAttnArgs a) {
+    const int s = blockIdx.x / a.map.n_kv, g = blockIdx.x % a.map.n_kv, group = a.n_heads / a.map.n_kv;
+    const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
+    const int rows = sp.n_q * group;
+    if (rows > ROWS_TILE) return;
+    for (int r = threadIdx.x >> 6; r < rows; r += 4) merge_row<TYPE>(a, sp.t0 + r / group, g * group + r % group, a.rows.n);
+}
+
+// Else a wave a row, over all tokens; rows of no sequence stay as they are.
 template <int TYPE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
     const int lane = threadIdx.x & 63;
     if (row >= (int64_t)a.n_tokens * a.n_heads) return;
     const int t = (int)(row / a.n_heads), head = (int)(row - (int64_t)t * a.n_heads);
-    // The row's sequence, 64 at a time; rows of none stay as they are.
-    int n_q = 0;
+    int n_q = 0;  // of the row's sequence, looked for 64 at a time
     for (int s0 = 0; s0 < a.n_seqs && !n_q; s0 += WAVE) {
         SeqSpan sp = {0, 0, 0};
         if (s0 + lane < a.n_seqs) sp = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
         const uint64_t mine = __ballot(t >= sp.t0 && t < sp.t0 + sp.n_q);
-        if (mine) n_q = __shfl(sp.n_q, __ffsll((unsigned long long)mine) - 1);
+        if (mine) n_q = __builtin_amdgcn_readlane(sp.n_q, __ffsll((unsigned long long)mine) - 1);
     }
     const int nsplit = n_q * (a.n_heads / a.map.n_kv) <= ROWS_TILE ? a.rows.n : a.big.n;
     if (n_q == 0 || nsplit == 1) return;  // unsplit: written already
-    float2 ml = make_float2(NEG_INF, 0.f);
-    if (lane < nsplit) ml = a.part_ml[row * a.part_splits + lane];
-    const float m = wave_max(ml.x);
-    const float f = ml.x == NEG_INF ? 0.f : ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
-    const float l = wave_sum(ml.y * f);
-    float2 o = make_float2(0.f, 0.f);
-    for (int i = 0; i < nsplit; ++i) {
-        const float w = as_f32(__builtin_amdgcn_readlane(as_u32(f), i));
-        if (w == 0.f) continue;
-        const float2 p = *(const float2*)(a.part + (row * a.part_splits + i) * HD + 2 * lane);
-        o.x += w * p.x;
-        o.y += w * p.y;
-    }
-    const float inv = m == NEG_INF && l == 0.f ? 0.f : 1.f / l;
-    const int64_t at = (int64_t)t * a.out_stride + head * HD + 2 * lane;
-    if constexpr (TYPE == TYPE_F32)
-        *(float2*)((float*)a.out + at) = make_float2(o.x * inv, o.y * inv);
-    else
-        *(f16x2*)((f16*)a.out + at) = f16x2{(f16)(o.x * inv), (f16)(o.y * inv)};
+    merge_row<TYPE>(a, t, head, nsplit);
 }
 
 }  // namespace
@@ -1203,21 +1240,22 @@ PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q,
 
 template <int TYPE, int FMT>
 static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((paged_rows_kernel<TYPE, FMT>), dim3(a.n_seqs, a.map.n_kv, a.rows.n), dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const unsigned few = (unsigned)a.n_seqs * a.map.n_kv * a.rows.n;
+    hipError_t e;
     if (a.tiles) {
         e = hipFuncSetAttribute((const void*)paged_chunk_kernel<TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, CH_LDS);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_chunk_kernel<TYPE, FMT>), dim3((unsigned)a.tiles * a.map.n_kv * a.big.n), dim3(512), CH_LDS, s, a);
-        e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_chunk_kernel<TYPE, FMT>), dim3(few + (unsigned)a.tiles * a.map.n_kv * a.big.n), dim3(512), CH_LDS, s, a);
+    } else {
+        hipLaunchKernelGGL((paged_rows_kernel<TYPE, FMT>), dim3(few), dim3(256), 0, s, a);
     }
-    if (a.part_splits > 1) {
+    e = hipGetLastError();
+    if (e != hipSuccess || a.part_splits == 1) return e;
+    if (a.big.n > 1)
         hipLaunchKernelGGL(paged_merge_kernel<TYPE>, dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a);
-        e = hipGetLastError();
-    }
-    return e;
+    else
+        hipLaunchKernelGGL(paged_merge_rows_kernel<TYPE>, dim3((unsigned)a.n_seqs * a.map.n_kv), dim3(256), 0, s, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s) {

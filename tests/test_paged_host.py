@@ -61,7 +61,7 @@ def test_pools_are_checked_by_the_wrapper():
 
 @pytest.mark.parametrize("kw,match", [
     (dict(type=2), "type"), (dict(q_type=-1), "type"), (dict(n_tokens=-1), "negative"), (dict(n_heads=-1), "n_heads"),
-    (dict(qkv_stride=32 * 128 - 8), "qkv_stride"), (dict(qkv_stride=32 * 128 + 4), "qkv_stride"),
+    (dict(n_tokens=(1 << 22) + 1), "2\\^27"), (dict(qkv_stride=32 * 128 - 8), "qkv_stride"), (dict(qkv_stride=32 * 128 + 4), "qkv_stride"),
     (dict(q_stride=16 * 128 - 8), "q_stride"), (dict(qkv=At(4)), "qkv"), (dict(qkv=None), "qkv"), (dict(q=None), "q must"),
     (dict(q_norm=At(4)), "q_norm"), (dict(k_norm=At(4)), "k_norm"), (dict(slots=None), "slots"),
     (dict(rot_dim=12), "rot_dim"), (dict(rot_dim=136), "rot_dim"), (dict(rot_dim=-8), "rot_dim"),
@@ -79,7 +79,7 @@ def test_store_refuses(kw, match):
 @pytest.mark.parametrize("kw,match", [
     (dict(type=2), "type"), (dict(n_heads=12), "n_heads"), (dict(n_heads=0), "n_heads"), (dict(n_heads=136), "n_heads"),
     (dict(n_seqs=-1), "negative"), (dict(n_tokens=-1), "negative"), (dict(max_q=-1), "negative"),
-    (dict(max_kv=-1), "negative"), (dict(n_seqs=(1 << 20) + 1), "2\\^20"), (dict(n_tokens=(1 << 24) + 1), "2\\^24"),
+    (dict(max_kv=-1), "negative"), (dict(n_seqs=(1 << 18) + 1), "2\\^21"), (dict(n_tokens=(1 << 22) + 1), "2\\^26"),
     (dict(table_width=0), "table_width"), (dict(table_width=1 << 24), "table_width"), (dict(q_stride=8), "q_stride"),
     (dict(out_stride=16 * 128 + 4), "out_stride"), (dict(scale=float("inf")), "scale"), (dict(q=At(2)), "q and out"),
     (dict(out=None), "q and out"), (dict(q_start=None), "q_start"), (dict(kv_len=None), "q_start"),
@@ -95,7 +95,7 @@ def test_attention_refuses(kw, match):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(type=3), "type"), (dict(n_rows=-1), "negative"), (dict(k=At(4)), "aligned"), (dict(slots=None), "slots"),
+    (dict(type=3), "type"), (dict(n_rows=-1), "negative"), (dict(n_rows=(1 << 24) + 1), "2\\^27"), (dict(k=At(4)), "aligned"), (dict(slots=None), "slots"),
     (dict(token_stride=8, head_stride=128), "strides"), (dict(token_stride=128), "strides"),
     (dict(token_stride=132, head_stride=1024), "strides"),
 ])
