@@ -1802,11 +1802,13 @@ static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention
     a.n_tokens = args->n_tokens;
     a.table_width = args->table_width;
     a.max_kv = args->max_kv ? std::min(args->max_kv, slots) : slots;
+    if ((int64_t)a.n_seqs * ((a.max_kv + 127) / 128) > (1 << 29))
+        return fail("paged_attention: more than 2^36 slots in all");
     const int max_q = args->max_q ? std::min(args->max_q, args->n_tokens) : args->n_tokens;
     plan = paged_plan(a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv);
     return 0;
 }
-static size_t plan_bytes(const PagedPlan& p) { return (p.part_floats + p.ml_floats) * sizeof(float); }
+static size_t plan_bytes(const PagedPlan& p) { return (p.few_rows + p.part_rows) * (HD + 2) * sizeof(float); }
 
 int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, size_t* bytes) {
     PagedAttnArgs a{};
@@ -1843,12 +1845,16 @@ int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t
     a.q_start = args->q_start;
     a.kv_len = args->kv_len;
     a.tables = args->tables;
-    a.rows = plan.rows;
+    a.few = plan.few;
     a.big = plan.big;
     a.tiles = plan.tiles;
-    a.part_splits = plan.part_splits;
-    a.part = (float*)args->work;
-    a.part_ml = (float2*)(a.part + plan.part_floats);
+    float* const few_part = (float*)args->work;
+    float* const part = few_part + plan.few_rows * HD;
+    float2* const ml = (float2*)(part + plan.part_rows * HD);
+    a.few_part = plan.few_rows ? few_part : nullptr;
+    a.few_ml = ml;
+    a.part = plan.part_rows ? part : nullptr;
+    a.part_ml = ml + plan.few_rows;
     HIPCK(launch_paged_attention(pages->fmt, args->type, a, (hipStream_t)stream));
     return 0;
 }

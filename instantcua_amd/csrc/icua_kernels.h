@@ -247,11 +247,15 @@ hipError_t launch_paged_load(int fmt, int type, const PagedLoadArgs& a, hipStrea
 struct PagedSplit {
     int n, chunk;                   // a sequence's slots in n ranges of chunk slots
 };
+struct PagedFew {
+    int n, unit, least;             // n workgroups a KV head, each with a share of `least` or more units of slots
+    int rows;                       // upper bound of a sequence's query rows a KV head
+};
 struct PagedPlan {
-    PagedSplit rows, big;           // for sequences of at most 16 query rows a KV head, and of more
+    PagedFew few;                   // sequences of at most 16 query rows a KV head
+    PagedSplit big;                 // those of more
     int tiles;                      // upper bound of the 128-row tiles of the latter (0: none)
-    int part_splits;                // ranges of a row's partials, > 1 if any sequence's slots are split
-    size_t part_floats, ml_floats;  // partial rows and their (maximum, denominator) pairs
+    size_t few_rows, part_rows;     // partial rows of the two (0: none is split)
 };
 constexpr int PAGED_MAX_SPLITS = 64;
 PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv);
@@ -267,10 +271,13 @@ struct PagedAttnArgs {
     const int32_t *q_start;         // [n_seqs + 1] first token of every sequence
     const int32_t *kv_len;          // [n_seqs] slots, the new tokens' included
     const int32_t* tables;          // [n_seqs][table_width] pages
-    PagedSplit rows, big;
-    int tiles, part_splits;
-    float* part;                    // [n_tokens][n_heads][part_splits][128]
-    float2* part_ml;                // [n_tokens][n_heads][part_splits]
+    PagedFew few;
+    PagedSplit big;
+    int tiles;
+    float* few_part;                // [workgroup][KV head][2][few.rows][128], null: none
+    float2* few_ml;                 // (maximum, denominator) of each
+    float* part;                    // [n_tokens][n_heads][big.n][128], null: none
+    float2* part_ml;
 };
 hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s);
 

@@ -229,23 +229,38 @@ struct Query {
     v8h hi[4], lo[TYPE == TYPE_F32 ? 4 : 1];
     float c;
 };
+// Its values as they are in memory, and the operands made of them: what is loaded in between is under way
+// meanwhile.
 template <int TYPE>
-__device__ __forceinline__ Query<TYPE> load_query(const PagedAttnArgs& a, const RowOf& r, int q) {
-    Query<TYPE> y;
-    y.c = a.scale * 1.4426950408889634f;
+struct QueryRow {
+    u32x4 x[TYPE == TYPE_F32 ? 8 : 4];
+};
+template <int TYPE>
+__device__ __forceinline__ QueryRow<TYPE> load_query(const PagedAttnArgs& a, const RowOf& r, int q) {
+    QueryRow<TYPE> y;
     const int64_t at = (int64_t)r.t * a.q_stride + r.head * HD + 8 * q;
     if constexpr (TYPE == TYPE_F16) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) y.hi[ks] = r.t < 0 ? v8h{} : *(const v8h*)((const f16*)a.q + at + 32 * ks);
+        for (int ks = 0; ks < 4; ++ks) y.x[ks] = r.t < 0 ? u32x4{} : *(const u32x4*)((const f16*)a.q + at + 32 * ks);
     } else {
-        f32x4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y.x[k] = r.t < 0 ? u32x4{} : *(const u32x4*)((const float*)a.q + at + 32 * (k / 2) + 4 * (k % 2));
+    }
+    return y;
+}
+template <int TYPE>
+__device__ __forceinline__ Query<TYPE> query_of(const QueryRow<TYPE>& r, float scale) {
+    Query<TYPE> y;
+    y.c = scale * 1.4426950408889634f;
+    if constexpr (TYPE == TYPE_F16) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) y.hi[ks] = __builtin_bit_cast(v8h, r.x[ks]);
+    } else {
         float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            x[k] = r.t < 0 ? f32x4{} : *(const f32x4*)((const float*)a.q + at + 32 * (k / 2) + 4 * (k % 2));
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
-        }
+            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(as_f32(r.x[k][e])));
         amax = max_x4(amax);
         const int k2 = query_shift(amax);
         y.c = ldexpf(y.c, -k2);
@@ -253,7 +268,7 @@ __device__ __forceinline__ Query<TYPE> load_query(const PagedAttnArgs& a, const 
         for (int k = 0; k < 8; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float v = ldexpf(x[k][e], k2);
+                const float v = ldexpf(as_f32(r.x[k][e]), k2);
                 const f16 h = (f16)v;
                 y.hi[k / 2][4 * (k % 2) + e] = h;
                 y.lo[k / 2][4 * (k % 2) + e] = (f16)(v - (float)h);
@@ -276,6 +291,21 @@ struct Tile<FMT_Q8> {
     u32x4 ks[2];
     uint16_t vs[4];
 };
+// Any values: those of a tile of before need not be kept.
+template <int FMT>
+__device__ __forceinline__ void no_tile(Tile<FMT>* t) {
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            t[j].k[i] = __builtin_nondeterministic_value(t[j].k[i]);
+            t[j].v[i] = __builtin_nondeterministic_value(t[j].v[i]);
+            if constexpr (FMT == FMT_Q8) t[j].vs[i] = __builtin_nondeterministic_value(t[j].vs[i]);
+        }
+        if constexpr (FMT == FMT_Q8)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) t[j].ks[i] = __builtin_nondeterministic_value(t[j].ks[i]);
+    }
+}
 template <int FMT>
 __device__ __forceinline__ void load_tile(const PagedAttnArgs& a, int row, int lane, Tile<FMT>& t) {
     const int q = lane >> 4, r16 = lane & 15;
@@ -389,39 +419,87 @@ __device__ __forceinline__ float row_value(const void* v, const void* v_sb, int6
     return (float)(f16)(h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d]);
 }
 
-// Sequences with at most 16 query rows a KV head (single tokens, drafts): a workgroup of NW waves has a
-// (sequence, KV head) and a range of its slots, its waves take 32-slot steps of it in turn and join
-// through LDS.  K and V go from memory to registers, as each is used by one tile alone, a step ahead of
-// its products.  Bound by memory.
+// Sequences with at most 16 query rows a KV head (single tokens, drafts).  Their slots, in units of a step
+// of all waves of a workgroup, are dealt out evenly: workgroup w of a KV head's `few.n` has units w * per ..
+// of all sequences in a row, whatever the sequences' lengths.  A sequence that lies in one workgroup is
+// done there; of the others each workgroup leaves a partial, at most two: a sequence's end, or a part from
+// its middle, as the first and a beginning as the second.
+//
+// One workgroup a (sequence, KV head, range of slots) instead, as even as the longest sequence allows, takes
+// half again as long for lengths that differ by factors of up to 8.
 constexpr int ROWS_TILE = 16, ROWS_STEP = 32;
+constexpr int ROWS_PITCH = 80;  // 16-byte places of a wave's results of one dt
 template <int NW>
-constexpr size_t rows_lds() { return NW * (8 * WAVE * 16 + 16 * 8); }
+constexpr size_t rows_lds() { return NW * (8 * ROWS_PITCH * 16 + 16 * 8); }
 
+// Lane i: sequence s0 + i, its units (0: the chunk kernel's, or none) and those up to its end since s0; `sum`:
+// of all 64.
+struct FewUnits {
+    SeqSpan sp;
+    int n, end, sum;
+};
+__device__ __forceinline__ FewUnits few_units(const PagedAttnArgs& a, int group, int s0) {
+    const int lane = threadIdx.x & 63;
+    FewUnits u = {{0, 0, 0}, 0, 0, 0};
+    if (s0 + lane < a.n_seqs) u.sp = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
+    if (u.sp.n_q > 0 && u.sp.n_q * group <= ROWS_TILE) u.n = max(1, (u.sp.n_kv + a.few.unit - 1) / a.few.unit);
+    u.end = u.n;
+    for (int o = 1; o < min(WAVE, a.n_seqs); o <<= 1) {
+        const int y = __shfl_up(u.end, o);
+        if (lane >= o) u.end += y;
+    }
+    u.sum = __builtin_amdgcn_readlane(u.end, min(WAVE, a.n_seqs) - 1);
+    return u;
+}
+// Units a workgroup takes, of this many.
+__device__ __forceinline__ int few_per(const PagedAttnArgs& a, int total) {
+    return max(a.few.least, (total + a.few.n - 1) / a.few.n);
+}
+
+// A workgroup of NW waves: its waves take 32-slot steps of a sequence in turn and join through LDS.  K and V
+// go from memory to registers, as each is used by one tile alone, a step ahead of its products.  Bound by
+// memory.
 template <int TYPE, int FMT, int NW>
 __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uint8_t* lds) {
     // fp32 probabilities and, so that only the output's rounding counts, those of q8 in two parts.
     constexpr bool PLO = TYPE == TYPE_F32 || FMT == FMT_Q8, VLO = VOp<TYPE, FMT>::LO;
-    f32x4* const so = (f32x4*)lds;                        // [NW][8][64]
-    float2* const sml = (float2*)(lds + NW * 8 * WAVE * 16);  // [NW][16]
+    f32x4* const so = (f32x4*)lds;                                  // [NW][8][ROWS_PITCH]
+    float2* const sml = (float2*)(lds + NW * 8 * ROWS_PITCH * 16);  // [NW][16]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
-    const int split = index % a.rows.n, g = index / a.rows.n % a.map.n_kv, s = index / a.rows.n / a.map.n_kv;
-    const int group = a.n_heads / a.map.n_kv;
-    const int32_t* table = a.tables + (int64_t)s * a.table_width;
-    // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).  Looked up
-    // before the sequence's lengths are there.
+    const int g = index % a.map.n_kv, w = index / a.map.n_kv, group = a.n_heads / a.map.n_kv;
+    FewUnits u = few_units(a, group, 0);
+    int total = u.sum;
+    for (int s0 = WAVE; s0 < a.n_seqs; s0 += WAVE) total += few_units(a, group, s0).sum;
+    const int per = few_per(a, total), end = min(total, (w + 1) * per);
+    int pos = w * per, s0 = 0, before = 0;
+    while (pos < end) {
+    // The sequence that has unit pos, and where its units begin.
+    const uint64_t past = __ballot(before + u.end > pos);
+    if (!past) {
+        before += u.sum;
+        s0 += WAVE;
+        if (s0 >= a.n_seqs) return;
+        u = few_units(a, group, s0);
+        continue;
+    }
+    const int at_lane = __ffsll((unsigned long long)past) - 1, seq_end = before + __builtin_amdgcn_readlane(u.end, at_lane);
+    const int seq_units = __builtin_amdgcn_readlane(u.n, at_lane), first = pos - (seq_end - seq_units), count = min(end, seq_end) - pos;
+    const SeqSpan sp = {__builtin_amdgcn_readlane(u.sp.t0, at_lane), __builtin_amdgcn_readlane(u.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.sp.n_kv, at_lane)};
+    const bool whole = count == seq_units;
+    pos += count;
+    const RowOf row = row_of(sp, r16, group, g);
+    // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
+    const int start = first * a.few.unit;
+    const int lim = sp.n_kv, all = sp.n_kv - sp.n_q, c1 = min(lim, start + count * a.few.unit);
+    const int32_t* table = a.tables + (int64_t)(s0 + at_lane) * a.table_width;
+    // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).
     auto step_slot = [&](int sub, int i) { return sub + ROWS_STEP * (wave + NW * i); };
     auto lookup = [&](int sub) {
         const int slot = step_slot(sub, lane / 2) + PAGED_TILE * (lane % 2);
-        return slot < a.max_kv ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
+        return slot < c1 ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
     };
     constexpr int SUB = NW * ROWS_STEP * (WAVE / 2);
-    const int start = split * a.rows.chunk;
     int rows = lookup(start);
-    const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
-    if (sp.n_q == 0 || sp.n_q * group > ROWS_TILE) return;  // the others are the chunk kernel's
-    const RowOf row = row_of(sp, r16, group, g);
-    // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
-    const int lim = sp.n_kv, all = sp.n_kv - sp.n_q, c1 = min(lim, start + a.rows.chunk);
 
     f32x4 O[8];
 #pragma unroll
@@ -433,7 +511,18 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
         for (int k = 0; k < 2; ++k)
             load_tile<FMT>(a, max(__builtin_amdgcn_readlane(rows, 2 * i + k), 0) + g * a.map.page_slots, lane, t[k]);
     };
-    const Query<TYPE> y = load_query<TYPE>(a, row, q);
+    // This wave's steps of the window that begin below c1.
+    auto steps = [&]() {
+        const int left = c1 - step_slot(sub, 0);
+        return left <= 0 ? 0 : min(WAVE / 2, (left + NW * ROWS_STEP - 1) / (NW * ROWS_STEP));
+    };
+    const QueryRow<TYPE> qrow = load_query<TYPE>(a, row, q);
+    Tile<FMT> A[2], B[2];
+    no_tile<FMT>(A);
+    no_tile<FMT>(B);
+    int n = steps();
+    if (n > 0) fetch(0, A);
+    const Query<TYPE> y = query_of<TYPE>(qrow, a.scale);
     auto step = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
         const int at = step_slot(sub, i);
         const int ok[2] = {__builtin_amdgcn_readlane(rows, 2 * i) < 0 ? 0 : lim, __builtin_amdgcn_readlane(rows, 2 * i + 1) < 0 ? 0 : lim};
@@ -490,17 +579,25 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                 for (int e = 0; e < 4; ++e) t[k].v[e] ^= 0x80808080u;
         // Slots that some rows see and others do not: values there that are no numbers are kept out of the
         // products and go to the rows that see them.
+        auto values = [&](auto finite) __attribute__((always_inline)) {
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-            VOp<TYPE, FMT> v = v_operand<TYPE, FMT>(t, dt);
-            if (masked) {
-                keep_finite(v.hi, odd);
-                if constexpr (VLO) keep_finite(v.lo, odd);
+            for (int dt = 0; dt < 8; ++dt) {
+                VOp<TYPE, FMT> v = v_operand<TYPE, FMT>(t, dt);
+                if (finite) {
+                    keep_finite(v.hi, odd);
+                    if constexpr (VLO) keep_finite(v.lo, odd);
+                }
+                O[dt] = mfma(v.hi, ph, O[dt]);
+                if constexpr (PLO) O[dt] = mfma(v.hi, pl, O[dt]);
+                if constexpr (VLO) O[dt] = mfma(v.lo, ph, O[dt]);
             }
-            O[dt] = mfma(v.hi, ph, O[dt]);
-            if constexpr (PLO) O[dt] = mfma(v.hi, pl, O[dt]);
-            if constexpr (VLO) O[dt] = mfma(v.lo, ph, O[dt]);
-        }
+        };
+        if constexpr (VLO)
+            values(masked);  // one copy: two take more registers than there are
+        else if (masked)
+            values(std::true_type());
+        else
+            values(std::false_type());
         if (__ballot(odd != 0))
             for (int j = 0; j < ROWS_STEP; ++j) {
                 const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);
@@ -516,13 +613,7 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                     }
             }
     };
-    for (; sub < c1; sub += SUB) {
-        if (sub != start) rows = lookup(sub);
-        // This wave's steps of the window that begin below c1.
-        const int left = c1 - step_slot(sub, 0);
-        const int n = left <= 0 ? 0 : min(WAVE / 2, (left + NW * ROWS_STEP - 1) / (NW * ROWS_STEP));
-        Tile<FMT> A[2], B[2];
-        if (n > 0) fetch(0, A);
+    while (n > 0) {
         for (int i = 0; i < n; i += 2) {
             if (i + 1 < n) fetch(i + 1, B);
             step(i, A);
@@ -531,44 +622,54 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                 step(i + 1, B);
             }
         }
+        sub += SUB;
+        if (sub >= c1) break;
+        rows = lookup(sub);
+        n = steps();
+        if (n > 0) fetch(0, A);
     }
-    // Join the waves: lane (r16, q) of each has dims 8 (4 q + i) + dt of row r16.
+    // Join the waves: lane (r16, q) of each has dims 32 q + 8 i + dt of row r16.  They go through LDS, [wave][dt]
+    // [q][r16][i], the rows of q padded by four so that the lanes that read it meet no bank twice.
     l = sum_x4(l);
+    __syncthreads();  // the sequence before is read
     if (q == 0) sml[wave * 16 + r16] = make_float2(m, l);
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) so[(wave * 8 + dt) * WAVE + lane] = O[dt];
+    for (int dt = 0; dt < 8; ++dt) so[(wave * 8 + dt) * ROWS_PITCH + q * 20 + r16] = O[dt];
     __syncthreads();
-    float mt = NEG_INF, lt = 0.f, f[NW];
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mt = fmaxf(mt, sml[w * 16 + r16].x);
+    // A thread writes DIMS values of a row.
+    constexpr int DIMS = 8 * 4 / NW;
+    const int at = threadIdx.x * DIMS, d0 = at % HD, orow = at / HD;
+    const RowOf out = row_of(sp, orow, group, g);
+    if (out.t >= 0 && (whole || orow < a.few.rows)) {
+    float mt = NEG_INF, lt = 0.f;
+    float2 ml[NW];
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-        const float2 ml = sml[w * 16 + r16];
-        f[w] = ml.x == mt ? 1.f : __builtin_amdgcn_exp2f(ml.x - mt);
-        lt += ml.y * f[w];
+        ml[w] = sml[w * 16 + orow];
+        mt = fmaxf(mt, ml[w].x);
     }
-    if (row.t < 0) return;
-    // Wave w writes dims 8 (4 q + i) + dt, its 8 / NW of dt.
-    const bool whole = a.rows.n == 1;
+    float x[DIMS] = {};
+    const float* src = (const float*)so + (d0 % 8) * ROWS_PITCH * 4 + (d0 / 32) * 80 + orow * 4 + d0 / 8 % 4;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const float f = ml[w].x == mt ? 1.f : __builtin_amdgcn_exp2f(ml[w].x - mt);
+        lt += ml[w].y * f;
+#pragma unroll
+        for (int k = 0; k < DIMS; ++k) x[k] += src[(w * 8 + k) * ROWS_PITCH * 4] * f;
+    }
     const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
-    const int64_t out_row = (int64_t)row.t * a.n_heads + row.head;
-    constexpr int ND = 8 / NW;
+    const int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < ND; ++k) {
-            const int dt = ND * wave + k, d = 8 * (4 * q + i) + dt;
-            float x = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) x += so[(w * 8 + dt) * WAVE + lane][i] * f[w];
-            if (!whole)
-                a.part[(out_row * a.part_splits + split) * HD + d] = x;
-            else if constexpr (TYPE == TYPE_F32)
-                ((float*)a.out)[(int64_t)row.t * a.out_stride + row.head * HD + d] = x * inv;
-            else
-                ((f16*)a.out)[(int64_t)row.t * a.out_stride + row.head * HD + d] = (f16)(x * inv);
-        }
-    if (!whole && wave == 0 && q == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
+    for (int k = 0; k < DIMS; k += 4) {
+        const f32x4 y = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]} * inv;
+        if (!whole)
+            *(f32x4*)(a.few_part + part * HD + d0 + k) = y;
+        else
+            store4<TYPE>(a.out, (int64_t)out.t * a.out_stride + out.head * HD + d0 + k, y);
+    }
+    if (!whole && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
+    }
+    }
 }
 
 template <int TYPE, int FMT>
@@ -662,7 +763,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
     // The first workgroups have the sequences of few rows: their reads run beside the others' products.
-    const int few = a.n_seqs * a.map.n_kv * a.rows.n, index = (int)blockIdx.x - few;
+    const int few = a.few.n * a.map.n_kv, index = (int)blockIdx.x - few;
     if (index < 0) {
         rows_work<TYPE, FMT, 8>(a, blockIdx.x, lds);
         return;
@@ -1112,28 +1213,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int e = 0; e < 4; ++e) y[e] = (O[k / 4][4 * (k % 4) + e] * f0 + o1[e] * f1) * inv;
         const int d = 32 * (k / 4) + 8 * (k % 4) + 4 * h;
         if (a.big.n > 1)
-            *(f32x4*)(a.part + (out_row * a.part_splits + split) * HD + d) = y;
+            *(f32x4*)(a.part + (out_row * a.big.n + split) * HD + d) = y;
         else
             store4<TYPE>(a.out, (int64_t)row.t * a.out_stride + row.head * HD + d, y);
     }
-    if (a.big.n > 1 && h == 0) a.part_ml[out_row * a.part_splits + split] = make_float2(mt, lt);
+    if (a.big.n > 1 && h == 0) a.part_ml[out_row * a.big.n + split] = make_float2(mt, lt);
 }
 
-// Joins the splits of a row: 32 lanes have a split's 128 values, four each, so a wave reads two splits at a
-// time, eight loads in flight; all of them are independent of the weights.
-template <int TYPE>
-__device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int head, int nsplit) {
+// Joins the partials of a row, at part_at(0 .. n - 1): 32 lanes have a partial's 128 values, four each, so a
+// wave reads two at a time, eight loads in flight; all of them are independent of the weights.
+template <int TYPE, typename AT>
+__device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int head, const float* part, const float2* part_ml, int n, AT part_at) {
     const int lane = threadIdx.x & 63, d = 4 * (lane & 31);
-    const int64_t row = (int64_t)t * a.n_heads + head;
-    const float* part = a.part + row * a.part_splits * HD + d;
     float2 ml = make_float2(NEG_INF, 0.f);
-    if (lane < nsplit) ml = a.part_ml[row * a.part_splits + lane];
+    if (lane < n) ml = part_ml[part_at(lane)];
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float f = 0.f, m = 0.f, l = 0.f;
-    for (int i0 = 0; i0 < nsplit; i0 += 16) {
+    for (int i0 = 0; i0 < n; i0 += 16) {
         f32x4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = *(const f32x4*)(part + (int64_t)min(i0 + 2 * k + (lane >> 5), nsplit - 1) * HD);
+        for (int k = 0; k < 8; ++k) x[k] = *(const f32x4*)(part + part_at(min(i0 + 2 * k + (lane >> 5), n - 1)) * HD + d);
         if (i0 == 0) {
             m = wave_max(ml.x);
             f = ml.x == NEG_INF ? 0.f : ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
@@ -1142,7 +1241,7 @@ __device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int hea
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int i = i0 + 2 * k + (lane >> 5);
-            const float w = i < nsplit ? __shfl(f, i) : 0.f;
+            const float w = i < n ? __shfl(f, i) : 0.f;
             if (w != 0.f) o += x[k] * w;
         }
     }
@@ -1152,33 +1251,58 @@ __device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int hea
     if (lane < 32) store4<TYPE>(a.out, (int64_t)t * a.out_stride + head * HD + d, o * inv);
 }
 
-// Where only sequences of few rows are split: a workgroup has a (sequence, KV head), a wave a row.
+// Row r of a few-row sequence s and KV head g, if workgroups share the sequence.
+template <int TYPE>
+__device__ __forceinline__ void merge_few(const PagedAttnArgs& a, int s, const SeqSpan& sp, int g, int r) {
+    const int group = a.n_heads / a.map.n_kv;
+    int total = 0, begin = 0, n = 0;  // units of all sequences, those before s, its own
+    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
+        const FewUnits u = few_units(a, group, s0);
+        if (s >= s0 && s < s0 + WAVE) {
+            n = __builtin_amdgcn_readlane(u.n, s - s0);
+            begin = total + __builtin_amdgcn_readlane(u.end, s - s0) - n;
+        }
+        total += u.sum;
+    }
+    const int per = few_per(a, total), w0 = begin / per, parts = (begin + n - 1) / per - w0 + 1;
+    if (parts < 2 || r >= a.few.rows) return;
+    merge_row<TYPE>(a, sp.t0 + r / group, g * group + r % group, a.few_part, a.few_ml, parts, [&](int i) {
+        return (((int64_t)(w0 + i) * a.map.n_kv + g) * 2 + (i == 0)) * a.few.rows + r;
+    });
+}
+
+// Where only sequences of few rows are split: a workgroup has four of the at most 16 rows of a (sequence, KV
+// head), a wave one.
 template <int TYPE>
 __global__ __launch_bounds__(256) void paged_merge_rows_kernel(PagedAttnArgs a) {
-    const int s = blockIdx.x / a.map.n_kv, g = blockIdx.x % a.map.n_kv, group = a.n_heads / a.map.n_kv;
+    const int r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = blockIdx.x / a.map.n_kv, g = blockIdx.x % a.map.n_kv;
     const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
-    const int rows = sp.n_q * group;
-    if (rows > ROWS_TILE) return;
-    for (int r = threadIdx.x >> 6; r < rows; r += 4) merge_row<TYPE>(a, sp.t0 + r / group, g * group + r % group, a.rows.n);
+    const int rows = sp.n_q * (a.n_heads / a.map.n_kv);
+    if (rows > ROWS_TILE || r >= rows) return;
+    merge_few<TYPE>(a, s, sp, g, r);
 }
 
 // Else a wave a row, over all tokens; rows of no sequence stay as they are.
 template <int TYPE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lane = threadIdx.x & 63, group = a.n_heads / a.map.n_kv;
     if (row >= (int64_t)a.n_tokens * a.n_heads) return;
     const int t = (int)(row / a.n_heads), head = (int)(row - (int64_t)t * a.n_heads);
-    int n_q = 0;  // of the row's sequence, looked for 64 at a time
-    for (int s0 = 0; s0 < a.n_seqs && !n_q; s0 += WAVE) {
-        SeqSpan sp = {0, 0, 0};
-        if (s0 + lane < a.n_seqs) sp = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
-        const uint64_t mine = __ballot(t >= sp.t0 && t < sp.t0 + sp.n_q);
-        if (mine) n_q = __builtin_amdgcn_readlane(sp.n_q, __ffsll((unsigned long long)mine) - 1);
+    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {  // its sequence, looked for 64 at a time
+        SeqSpan x = {0, 0, 0};
+        if (s0 + lane < a.n_seqs) x = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
+        const uint64_t mine = __ballot(t >= x.t0 && t < x.t0 + x.n_q);
+        if (!mine) continue;
+        const int i = __ffsll((unsigned long long)mine) - 1;
+        const SeqSpan sp = {__builtin_amdgcn_readlane(x.t0, i), __builtin_amdgcn_readlane(x.n_q, i), __builtin_amdgcn_readlane(x.n_kv, i)};
+        if (sp.n_q * group <= ROWS_TILE)
+            merge_few<TYPE>(a, s0 + i, sp, head / group, (t - sp.t0) * group + head % group);
+        else
+            merge_row<TYPE>(a, t, head, a.part, a.part_ml, a.big.n, [&](int k) { return row * a.big.n + k; });
+        return;
     }
-    const int nsplit = n_q * (a.n_heads / a.map.n_kv) <= ROWS_TILE ? a.rows.n : a.big.n;
-    if (n_q == 0 || nsplit == 1) return;  // unsplit: written already
-    merge_row<TYPE>(a, t, head, nsplit);
 }
 
 }  // namespace
@@ -1221,26 +1345,32 @@ static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv) {
     return {std::max(1, (max_kv + chunk - 1) / chunk), chunk};
 }
 
+// Units of few-row sequences among `want` workgroups: no sequence in more than PAGED_MAX_SPLITS of them.
+static PagedFew few_of(int64_t want, int unit, int n_kv, int n_seqs, int rows, int max_kv) {
+    const int most = std::max(1, (max_kv + unit - 1) / unit);
+    const int n = (int)std::min(std::max<int64_t>(1, want / n_kv), (int64_t)n_seqs * most);
+    return {n, unit, most < 2 ? 1 : (most - 2) / (PAGED_MAX_SPLITS - 1) + 1, rows};
+}
+
 PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv) {
     PagedPlan p{};
-    const int group = n_heads / n_kv;
-    p.rows = split_slots((int64_t)n_seqs * n_kv, 1024, max_kv);
+    const int group = n_heads / n_kv, few = (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
     p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
     if ((int64_t)max_q * group > ROWS_TILE) {
         p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
         p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv);
+        p.few = few_of(256, 8 * ROWS_STEP, n_kv, n_seqs, few, max_kv);
+    } else {
+        p.few = few_of(512, 4 * ROWS_STEP, n_kv, n_seqs, few, max_kv);
     }
-    p.part_splits = std::max(p.rows.n, p.big.n);
-    if (p.part_splits > 1) {
-        p.part_floats = (size_t)n_tokens * n_heads * p.part_splits * HD;
-        p.ml_floats = (size_t)n_tokens * n_heads * p.part_splits * 2;
-    }
+    if (p.big.n > 1) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
+    if (p.few.n > 1 && max_kv > p.few.unit) p.few_rows = (size_t)p.few.n * n_kv * 2 * few;
     return p;
 }
 
 template <int TYPE, int FMT>
 static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
-    const unsigned few = (unsigned)a.n_seqs * a.map.n_kv * a.rows.n;
+    const unsigned few = (unsigned)a.few.n * a.map.n_kv;
     hipError_t e;
     if (a.tiles) {
         e = hipFuncSetAttribute((const void*)paged_chunk_kernel<TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, CH_LDS);
@@ -1250,11 +1380,11 @@ static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
         hipLaunchKernelGGL((paged_rows_kernel<TYPE, FMT>), dim3(few), dim3(256), 0, s, a);
     }
     e = hipGetLastError();
-    if (e != hipSuccess || a.part_splits == 1) return e;
-    if (a.big.n > 1)
+    if (e != hipSuccess) return e;
+    if (a.part)
         hipLaunchKernelGGL(paged_merge_kernel<TYPE>, dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(paged_merge_rows_kernel<TYPE>, dim3((unsigned)a.n_seqs * a.map.n_kv), dim3(256), 0, s, a);
+    else if (a.few_part)
+        hipLaunchKernelGGL(paged_merge_rows_kernel<TYPE>, dim3((unsigned)a.n_seqs * a.map.n_kv, (unsigned)(a.few.rows + 3) / 4), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
