@@ -1805,7 +1805,7 @@ static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention
     if ((int64_t)a.n_seqs * ((a.max_kv + 127) / 128) > (1 << 29))
         return fail("paged_attention: more than 2^36 slots in all");
     const int max_q = args->max_q ? std::min(args->max_q, args->n_tokens) : args->n_tokens;
-    plan = paged_plan(a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv);
+    plan = paged_plan(pages->fmt, a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv);
     return 0;
 }
 static size_t plan_bytes(const PagedPlan& p) { return (p.few_rows + p.part_rows) * (HD + 2) * sizeof(float); }

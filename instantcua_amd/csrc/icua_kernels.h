@@ -248,7 +248,8 @@ struct PagedSplit {
     int n, chunk;                   // a sequence's slots in n ranges of chunk slots
 };
 struct PagedFew {
-    int n, unit, least;             // n workgroups a KV head, each with a share of `least` or more units of slots
+    int n, unit, least, twice;      // n workgroups a KV head, each with a share of `least` or more units of slots,
+                                    // shares above `twice` doubled
     int rows;                       // upper bound of a sequence's query rows a KV head
 };
 struct PagedPlan {
@@ -258,7 +259,7 @@ struct PagedPlan {
     size_t few_rows, part_rows;     // partial rows of the two (0: none is split)
 };
 constexpr int PAGED_MAX_SPLITS = 64;
-PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv);
+PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv);
 struct PagedAttnArgs {
     PageMap map;
     const void *k, *v, *k_sb, *v_sb;

@@ -453,7 +453,8 @@ __device__ __forceinline__ FewUnits few_units(const PagedAttnArgs& a, int group,
 }
 // Units a workgroup takes, of this many.
 __device__ __forceinline__ int few_per(const PagedAttnArgs& a, int total) {
-    return max(a.few.least, (total + a.few.n - 1) / a.few.n);
+    const int per = max(a.few.least, (int)(((unsigned)total + a.few.n - 1) / (unsigned)a.few.n));
+    return per > a.few.twice ? 2 * per : per;
 }
 
 // A workgroup of NW waves: its waves take 32-slot steps of a sequence in turn and join through LDS.  K and V
@@ -692,10 +693,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 constexpr int CH_ROWS = 128, CH_HALF = 64;
 constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
 constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
-// q8 with fp32 queries: a half's scales [K, V][group][slot] and the largest of V, [group][16-slot tile].
-constexpr int CH_SCALES = 8 * CH_HALF + 16;
-// And for the eight tiles of two stages whether V has values that are no numbers, and whether the page exists.
-constexpr int CH_LDS = 2 * CH_STAGE + 4 * CH_SCALES * 4 + 128;
+// q8: a half's scales [K, V][group][slot] and the largest of V, [group][16-slot tile].
+constexpr int CH_SCALES = 8 * CH_HALF * 2 + 16 * 4;
+// And for the eight tiles of two stages whether V has values that are no numbers, whether the page exists, and
+// the power of two that V's scales are below.
+constexpr int CH_FLAGS = 2 * CH_STAGE + 4 * CH_SCALES, CH_LDS = CH_FLAGS + 192;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -727,45 +729,47 @@ __device__ __forceinline__ void staged_barrier() {
 }
 
 // The sequence and tile (of `rows` query rows a KV head) that number `index` stands for, over the
-// sequences with more than ROWS_TILE rows; false past the last one.  A wave looks at 64 sequences at a time.
+// sequences with more than ROWS_TILE rows; false past the last one.  A wave looks at 64 sequences at a time,
+// and takes those with the most slots first, so that the last workgroups to run are short.
 __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int group, int rows, int index, int& s, int& tile, int& tiles, SeqSpan& sp) {
     const int lane = threadIdx.x & 63;
     for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
+        const int count = min(WAVE, a.n_seqs - s0);
         SeqSpan x = {0, 0, 0};
-        if (s0 + lane < a.n_seqs) x = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
+        if (lane < count) x = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
         const int n = x.n_q * group > ROWS_TILE ? (x.n_q * group + rows - 1) / rows : 0;
-        int end = n;
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const int y = __shfl_up(end, o);
-            if (lane >= o) end += y;
+        int begin = 0, sum = 0;  // tiles of the sequences that come before lane's, of all
+        for (int j = 0; j < count; ++j) {
+            const int kv = __builtin_amdgcn_readlane(x.n_kv, j), add = __builtin_amdgcn_readlane(n, j);
+            if (kv > x.n_kv || (kv == x.n_kv && j < lane)) begin += add;
+            sum += add;
         }
-        const uint64_t past = __ballot(end > index);
-        if (past) {
-            const int first = __ffsll((unsigned long long)past) - 1;
-            tile = index - __builtin_amdgcn_readlane(end - n, first);
-            tiles = __builtin_amdgcn_readlane(n, first);
-            sp = {__builtin_amdgcn_readlane(x.t0, first), __builtin_amdgcn_readlane(x.n_q, first), __builtin_amdgcn_readlane(x.n_kv, first)};
-            s = s0 + first;
+        const uint64_t mine = __ballot(index >= begin && index < begin + n);
+        if (mine) {
+            const int i = __ffsll((unsigned long long)mine) - 1;
+            tile = index - __builtin_amdgcn_readlane(begin, i);
+            tiles = __builtin_amdgcn_readlane(n, i);
+            sp = {__builtin_amdgcn_readlane(x.t0, i), __builtin_amdgcn_readlane(x.n_q, i), __builtin_amdgcn_readlane(x.n_kv, i)};
+            s = s0 + i;
             return true;
         }
-        index -= __builtin_amdgcn_readlane(end, WAVE - 1);
+        index -= sum;
     }
     return false;
 }
 
 template <int TYPE, int FMT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
-    constexpr bool HL = TYPE == TYPE_F32, EXACT = HL && FMT == FMT_Q8;
+    constexpr bool HL = TYPE == TYPE_F32, CODES = FMT == FMT_Q8;
     extern __shared__ __align__(1024) uint8_t lds[];
-    int* const tile_odd = (int*)(lds + 2 * CH_STAGE + 4 * CH_SCALES * 4);
-    int* const tile_there = tile_odd + 16;
+    int* const tile_odd = (int*)(lds + CH_FLAGS);
+    int *const tile_there = tile_odd + 16, *const tile_top = tile_odd + 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
-    // The first workgroups have the sequences of few rows: their reads run beside the others' products.
-    const int few = a.few.n * a.map.n_kv, index = (int)blockIdx.x - few;
-    if (index < 0) {
-        rows_work<TYPE, FMT, 8>(a, blockIdx.x, lds);
+    // The last workgroups have the sequences of few rows: they are short, and bound by memory.
+    const int index = blockIdx.x, few = index - a.tiles * a.map.n_kv * a.big.n;
+    if (few >= 0) {
+        rows_work<TYPE, FMT, 8>(a, few, lds);
         return;
     }
     const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % a.big.n;
@@ -851,7 +855,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // LDS: half hb of K (kv = 0) or V (1) in stage st, and the scales of a half.
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     auto half_at = [&](int kv, int st, int hb) { return (uint32_t)((kv * 2 + st) * 2 + hb) * CH_MAT; };
-    auto scales_at = [&](int st, int hb) { return (float*)(lds + 2 * CH_STAGE) + (st * 2 + hb) * CH_SCALES; };
+    auto scales_at = [&](int st, int hb) { return (f16*)(lds + 2 * CH_STAGE + (st * 2 + hb) * CH_SCALES); };
+    auto tops_at = [&](int st, int hb) { return (float*)(scales_at(st, hb) + 8 * CH_HALF); };
     // fp16: this wave's tile of iteration it, pool row r, from memory to LDS; slots that are not there become
     // zeros.  Row l / 16 (+ 4 j) of the tile, place l % 16.
     int src_off[4];
@@ -894,11 +899,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto put = [&](int kv, int it) __attribute__((always_inline)) {
         uint8_t* dst = lds + half_at(kv, it & 1, par);
         const int r = 16 * wi + lane / 4;
-        // V with a scale that is no number, or (fp16 products) takes codes out of fp16's range: what is no
-        // number is kept out of the products, for the rows that may not see it.
-        const bool odd = kv && __ballot(!(h2f(scale[1]) <= (EXACT ? 65504.f : 65504.f / 127.f)));
+        // V with a scale that is no number is kept out of the products, for the rows that may not see it.
+        const bool odd = kv && __ballot(!(fabsf(h2f(scale[1])) <= 65504.f));
         if (kv && lane == 0) tile_odd[(it & 1) * 8 + wave] = odd;
-        if (EXACT && kv && !(h2f(scale[1]) <= 65504.f)) scale[1] = 0;
+        if (kv && !(fabsf(h2f(scale[1])) <= 65504.f)) scale[1] = 0;
         const f16 sc = __builtin_bit_cast(f16, scale[kv]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -909,25 +913,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 f16x2 c[2];
                 codes_h2(w[2 * (k % 2) + x], c);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) y[2 * x + e] = h2_bits(EXACT ? c[e] : c[e] * sc);
-            }
-            if (!EXACT && odd) {
-                v8h fin = __builtin_bit_cast(v8h, y);
-                uint32_t some = 0;
-                keep_finite(fin, some);
-                y = __builtin_bit_cast(u32x4, fin);
+                for (int e = 0; e < 2; ++e) y[2 * x + e] = h2_bits(c[e]);
             }
             *(u32x4*)(dst + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
         }
-        if constexpr (EXACT) {
-            float* scales = scales_at(it & 1, par);
-            scales[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = (float)sc;
-            if (kv) {  // the largest scale of each group: over the lanes with the same l % 4
-                float top = (float)sc;
-                top = fmaxf(top, dpp<0x124>(top));  // row_ror:4, 8: within rows of 16 lanes
-                top = fmaxf(top, dpp<0x128>(top));
-                top = max_x4(top);
-                if (lane < 4) scales[8 * CH_HALF + 4 * lane + wi] = top;
+        scales_at(it & 1, par)[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = sc;
+        if (kv) {  // the largest scale of each group: over the lanes with the same l % 4
+            int top = scale[1] & 0x7FFF;  // fp16 bits rise with the value
+            top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x124, 0xF, 0xF, true));  // row_ror:4, 8: within 16 lanes
+            top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x128, 0xF, 0xF, true));
+            auto r16 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = max((int)r16[0], (int)r16[1]);
+            auto r32 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max((int)r32[0], (int)r32[1]);
+            if constexpr (HL) {
+                if (lane < 4) tops_at(it & 1, par)[4 * lane + wi] = h2f((uint16_t)top);
+            } else {
+                top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR1, 0xF, 0xF, true));
+                top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR2, 0xF, 0xF, true));
+                if (lane == 0) tile_top[(it & 1) * 8 + wave] = (top >> 10) - 14;
             }
         }
     };
@@ -981,8 +985,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         return mb;
     };
     // The maximum that is subtracted follows the true one when that is more than 2^P_SLACK ahead.
-    auto follow_max = [&](float mb) __attribute__((always_inline)) {
-        mb = max_x2(mb) * qc;
+    auto follow_max = [&](float mb, float up) __attribute__((always_inline)) {
+        mb = max_x2(mb) * qc + up;
         if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK)) {
             asm volatile("");
             const float m_new = fmaxf(m, mb);
@@ -1015,7 +1019,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         v8h vf[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) vf[k] = v_operand(st, k / 4, k % 4);
-        follow_max(fmaxf(block_max(S[0]), block_max(S[1])));
+        follow_max(fmaxf(block_max(S[0]), block_max(S[1])), 0.f);
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
         const f16x2 ones = {(f16)1.f, (f16)1.f};
         float sum[2] = {0.f, 0.f};
@@ -1043,36 +1047,79 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         l += sum[0] + sum[1];
     };
-    // q8 with fp32 queries.  Scores of 32-slot block kt of iteration it's half: a group's sum of codes takes
-    // its slot's scale.
-    auto exact_scores = [&](int it, int kt) __attribute__((always_inline)) {
-        const uint32_t Ks = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
-        const float* scales = scales_at(it & 1, par);
-        f32x16 S = {};
+    // q8: codes are exact in fp16, and scales go to the sums of a group's products, in fp32, and to the
+    // probabilities.  Block kt's sums of group gr take their slots' scales.
+    auto scale_scores = [&](int it, int kt, int gr, const f32x16& y, f32x16& S) __attribute__((always_inline)) {
+        const f16* scales = scales_at(it & 1, par) + gr * CH_HALF + 32 * kt + 4 * h;
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-            f32x16 y = {};
+        for (int b = 0; b < 4; ++b) {
+            const v4h sc = *(const v4h*)(scales + 8 * b);
 #pragma unroll
-            for (int ks = 2 * gr; ks < 2 * gr + 2; ++ks) {
-                const v8h kf = k_operand(Ks, ks);
-                y = mfma32(kf, Qh[ks], y);
-                y = mfma32(kf, Ql[HL ? ks : 0], y);
-            }
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const f32x4 sc = *(const f32x4*)(scales + gr * CH_HALF + 32 * kt + 8 * b + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) S[4 * b + e] += y[4 * b + e] * sc[e];
-            }
+            for (int e = 0; e < 4; ++e) S[4 * b + e] = __builtin_fmaf(y[4 * b + e], (float)sc[e], S[4 * b + e]);
         }
-        return S;
     };
-    // Its values: a block's dims 32 dt .. + 31 are one group, whose scales, by the power of two that brings the
-    // half's largest below 1, go to the probabilities, and the power to the sum.
+    auto codes_scores = [&](int it, f32x16 S[2]) __attribute__((always_inline)) {
+        const uint32_t st = (it & 1) * 2 * CH_MAT;
+        f32x16 y[2];
+        S[0] = S[1] = f32x16{};
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                y[kt] = f32x16{};
+#pragma unroll
+                for (int ks = 2 * gr; ks < 2 * gr + 2; ++ks) {
+                    const v8h kf = k_operand(st + kt * 32 * HD * 2, ks);
+                    y[kt] = mfma32(kf, Qh[ks], y[kt]);
+                    if constexpr (HL) y[kt] = mfma32(kf, Ql[ks], y[kt]);
+                }
+                // Under these products, those of the block before are scaled.
+                if (2 * gr + kt) scale_scores(it, 1 - kt, gr - 1 + kt, y[1 - kt], S[1 - kt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        scale_scores(it, 1, NG - 1, y[1], S[1]);
+    };
+    // Values, fp16 queries: the maximum that was subtracted was raised by the power of two that brings the
+    // half's largest scale to 1, so probabilities times scales stay in fp16's range.
+    auto codes_values = [&](int it, const f32x16 S[2]) __attribute__((always_inline)) {
+        const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
+        const uint32_t st = (it & 1) * 2 * CH_MAT;
+        const f16* scales = scales_at(it & 1, par) + 4 * CH_HALF + 4 * h;
+        const f16x2 ones = {(f16)1.f, (f16)1.f};
+        float sum[2] = {0.f, 0.f};
+        f16x2 p[2][4];
+        auto exponentials = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                p[c % 2][e / 2][e % 2] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(S[c / 2][8 * (c % 2) + e], qc, -sub_m));
+        };
+        exponentials(0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                u32x4 ph;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const u32x2 sc = *(const u32x2*)(scales + dt * CH_HALF + 16 * c + 8 * k);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) ph[2 * k + e] = h2_bits(p[c % 2][2 * k + e] * as_h2(sc[e]));
+                }
+                O[dt] = mfma32(v_operand(st, c, dt), __builtin_bit_cast(v8h, ph), O[dt]);
+                sum[dt % 2] = dot2(p[c % 2][dt], ones, sum[dt % 2]);
+                if (dt == 1 && c < 3) exponentials(c + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum[0] + sum[1];
+    };
+    // fp32 queries: a block's dims 32 dt .. + 31 are one group, whose scales, by the power of two that brings
+    // the half's largest below 1, go to the probabilities, and the power to the sum.
     auto exact_values = [&](int it, int kt, const f32x16& S) __attribute__((always_inline)) {
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
         const uint32_t Vs = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
-        const float* scales = scales_at(it & 1, par);
+        const f16* scales = scales_at(it & 1, par);
+        const float* all_tops = tops_at(it & 1, par);
         float p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1081,7 +1128,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) {
-            const f32x4 tops = *(const f32x4*)(scales + 8 * CH_HALF + 4 * dt);
+            const f32x4 tops = *(const f32x4*)(all_tops + 4 * dt);
             const int e2 = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
             const float down = ldexpf(1.f, -e2), up = ldexpf(1.f, e2);
             f32x16 y = {};
@@ -1090,10 +1137,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 v8h ph, pl;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const f32x4 sc = *(const f32x4*)(scales + 4 * CH_HALF + dt * CH_HALF + 32 * kt + 16 * c + 8 * k + 4 * h);
+                    const v4h sc = *(const v4h*)(scales + 4 * CH_HALF + dt * CH_HALF + 32 * kt + 16 * c + 8 * k + 4 * h);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = p[8 * c + 4 * k + e] * (sc[e] * down);
+                        const float x = p[8 * c + 4 * k + e] * ((float)sc[e] * down);
                         ph[4 * k + e] = (f16)x;
                         pl[4 * k + e] = (f16)(x - (float)ph[4 * k + e]);
                     }
@@ -1171,15 +1218,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (it + 1 < it1) stage(it + 1);
         if constexpr (FMT == FMT_F16) clean_values(it);
         if (it < my1) {
-            if constexpr (!EXACT) {
+            if constexpr (!CODES) {
                 half_step(it);
             } else {
-                f32x16 S[2] = {exact_scores(it, 0), exact_scores(it, 1)};
+                f32x16 S[2];
+                codes_scores(it, S);
                 mask(it, 0, S[0]);
                 mask(it, 1, S[1]);
-                follow_max(fmaxf(block_max(S[0]), block_max(S[1])));
+                int up = 0;
+                if constexpr (!HL) {
+                    const int4 tops = *(const int4*)(tile_top + (it & 1) * 8 + 4 * par);
+                    up = max(max(max(tops.x, tops.y), max(tops.z, tops.w)), 0);
+                }
+                follow_max(fmaxf(block_max(S[0]), block_max(S[1])), (float)up);
+                if constexpr (HL) {
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) exact_values(it, kt, S[kt]);
+                    for (int kt = 0; kt < 2; ++kt) exact_values(it, kt, S[kt]);
+                } else {
+                    codes_values(it, S);
+                }
             }
             add_odd_values(it);
         }
@@ -1346,22 +1403,26 @@ static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv) {
 }
 
 // Units of few-row sequences among `want` workgroups: no sequence in more than PAGED_MAX_SPLITS of them.
-static PagedFew few_of(int64_t want, int unit, int n_kv, int n_seqs, int rows, int max_kv) {
+//
+// 512 workgroups are what the registers let run at once.  fp16 steps are twice a q8 step's bytes, and half as
+// many workgroups read long caches faster: eight sequences of up to 32768 slots 115 us, 124 with 512; 64 q8
+// ones of up to 8192 108 us with 512, 141 with 256, 116 with 1024.
+static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, int rows, int max_kv) {
     const int most = std::max(1, (max_kv + unit - 1) / unit);
     const int n = (int)std::min(std::max<int64_t>(1, want / n_kv), (int64_t)n_seqs * most);
-    return {n, unit, most < 2 ? 1 : (most - 2) / (PAGED_MAX_SPLITS - 1) + 1, rows};
+    return {n, unit, most < 2 ? 1 : (most - 2) / (PAGED_MAX_SPLITS - 1) + 1, twice, rows};
 }
 
-PagedPlan paged_plan(int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv) {
+PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv) {
     PagedPlan p{};
     const int group = n_heads / n_kv, few = (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
     p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
     if ((int64_t)max_q * group > ROWS_TILE) {
         p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
         p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv);
-        p.few = few_of(256, 8 * ROWS_STEP, n_kv, n_seqs, few, max_kv);
+        p.few = few_of(256, 8 * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv);
     } else {
-        p.few = few_of(512, 4 * ROWS_STEP, n_kv, n_seqs, few, max_kv);
+        p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, n_seqs, few, max_kv);
     }
     if (p.big.n > 1) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
     if (p.few.n > 1 && max_kv > p.few.unit) p.few_rows = (size_t)p.few.n * n_kv * 2 * few;
