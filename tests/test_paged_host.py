@@ -80,7 +80,7 @@ def test_store_refuses(kw, match):
     (dict(type=2), "type"), (dict(n_heads=12), "n_heads"), (dict(n_heads=0), "n_heads"), (dict(n_heads=136), "n_heads"),
     (dict(n_seqs=-1), "negative"), (dict(n_tokens=-1), "negative"), (dict(max_q=-1), "negative"),
     (dict(max_kv=-1), "negative"), (dict(n_seqs=(1 << 18) + 1), "2\\^21"), (dict(n_tokens=(1 << 22) + 1), "2\\^26"),
-    (dict(table_width=0), "table_width"), (dict(table_width=1 << 24), "table_width"), (dict(q_stride=8), "q_stride"),
+    (dict(n_seqs=1 << 18, table_width=1 << 13, max_kv=0), "2\\^36"), (dict(table_width=0), "table_width"), (dict(table_width=1 << 24), "table_width"), (dict(q_stride=8), "q_stride"),
     (dict(out_stride=16 * 128 + 4), "out_stride"), (dict(scale=float("inf")), "scale"), (dict(q=At(2)), "q and out"),
     (dict(out=None), "q and out"), (dict(q_start=None), "q_start"), (dict(kv_len=None), "q_start"),
     (dict(tables=None), "q_start"), (dict(work=None), "work"), (dict(work=At(nbytes=64)), "work"),
