@@ -786,42 +786,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int c0 = min(lim, split * a.big.chunk), c1 = min(lim, c0 + a.big.chunk);
     const int it0 = c0 / 128, it1 = c1 > c0 ? (c1 + 127) / 128 : it0;
 
-    // Query operands: dims 16 ks + 8 h .. + 7 of the column's row.
-    // Scores are masked before they are scaled, so the scale is positive: a negative one's sign goes to
-    // the query.
-    v8h Qh[8], Ql[HL ? 8 : 1];
-    const float sign = a.scale < 0.f ? -1.f : 1.f;
-    float qc = fabsf(a.scale) * 1.4426950408889634f;
+    // Query operands: dims 16 ks + 8 h .. + 7 of the column's row.  Loaded first, then the first K and V are
+    // asked for, and what both take is waited for once.
+    u32x4 qrow[HL ? 16 : 8];
     {
         const int64_t qa = (int64_t)row.t * a.q_stride + row.head * HD + 8 * h;
-        if constexpr (!HL) {
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) Qh[ks] = row.t < 0 ? v8h{} : *(const v8h*)((const f16*)a.q + qa + 16 * ks) * (f16)sign;
-        } else {
-            f32x4 x[16];
-            float amax = 0.f;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                x[k] = row.t < 0 ? f32x4{} : *(const f32x4*)((const float*)a.q + qa + 16 * (k / 2) + 4 * (k % 2));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
-            }
-            amax = max_x2(amax);
-            const int k2 = query_shift(amax);
-            qc = ldexpf(qc, -k2);
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = sign * ldexpf(x[k][e], k2);
-                    const f16 hi = (f16)v;
-                    Qh[k / 2][4 * (k % 2) + e] = hi;
-                    Ql[k / 2][4 * (k % 2) + e] = (f16)(v - (float)hi);
-                }
-        }
+        for (int k = 0; k < (HL ? 16 : 8); ++k)
+            qrow[k] = row.t < 0 ? u32x4{} : HL ? *(const u32x4*)((const float*)a.q + qa + 16 * (k / 2) + 4 * (k % 2)) : *(const u32x4*)((const f16*)a.q + qa + 16 * k);
     }
-
-    qc = fmaxf(qc, 1e-37f);  // and not zero: products are below 2^40, so this makes scores of 2^-80 at most
 
     // What the loop seldom needs is read again from the arguments where it is needed, so that it takes no
     // registers in between.
@@ -832,13 +805,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     // Staging: wave w copies 16-slot tile w of an iteration's eight.  Lane i of `rows`: the pool row of this
     // wave's tile in iteration sub + i (-1: no such page).
-    bool bad_pages = false;
-    {
-        const int32_t* table = a.tables + (int64_t)s * a.table_width;
-        const int last_page = c1 > c0 ? (c1 - 1) / a.map.page_slots : -1;
-        for (int p = c0 / a.map.page_slots; p <= last_page; p += WAVE)
-            if (__ballot(p + lane <= last_page && page_row(a.map, table[min(p + lane, last_page)], 0) < 0)) bad_pages = true;
-    }
     int rows = -1, sub = it0 - WAVE;
     const int head_row = g * a.map.page_slots;
     auto tile_row = [&](int it) __attribute__((always_inline)) {
@@ -935,6 +901,62 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
         }
     };
+
+    auto stage = [&](int it) __attribute__((always_inline)) {
+        const int r = tile_row(it);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            if constexpr (FMT == FMT_F16)
+                copy(kv, it, r);
+            else
+                fetch(kv, it, r);
+        }
+    };
+    auto staged = [&](int it) __attribute__((always_inline)) {
+        if constexpr (FMT == FMT_Q8) {
+            put(0, it);
+            put(1, it);
+        }
+    };
+    if (it0 < it1) stage(it0);
+    // Scores are masked before they are scaled, so the scale is positive: a negative one's sign goes to
+    // the query.
+    v8h Qh[8], Ql[HL ? 8 : 1];
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    float qc = fabsf(a.scale) * 1.4426950408889634f;
+    if constexpr (!HL) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) Qh[ks] = __builtin_bit_cast(v8h, qrow[ks]) * (f16)sign;
+    } else {
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(as_f32(qrow[k][e])));
+        amax = max_x2(amax);
+        const int k2 = query_shift(amax);
+        qc = ldexpf(qc, -k2);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = sign * ldexpf(as_f32(qrow[k][e]), k2);
+                const f16 hi = (f16)v;
+                Qh[k / 2][4 * (k % 2) + e] = hi;
+                Ql[k / 2][4 * (k % 2) + e] = (f16)(v - (float)hi);
+            }
+    }
+    qc = fmaxf(qc, 1e-37f);  // and not zero: products are below 2^40, so this makes scores of 2^-80 at most
+
+    // Whether the table has pages outside the pool.
+    bool bad_pages = false;
+    {
+        const int32_t* table = a.tables + (int64_t)s * a.table_width;
+        const int last_page = c1 > c0 ? (c1 - 1) / a.map.page_slots : -1;
+        for (int p = c0 / a.map.page_slots; p <= last_page; p += WAVE)
+            if (__ballot(p + lane <= last_page && page_row(a.map, table[min(p + lane, last_page)], 0) < 0)) bad_pages = true;
+    }
+    if (it0 < it1) staged(it0);
 
     f32x16 O[4];
 #pragma unroll
@@ -1193,26 +1215,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     // Iterations whose half some row of this wave sees.
     const int my1 = active && base_of(it0) <= w_last ? min(it1, (w_last - CH_HALF * par) / 128 + 1) : it0;
-    auto stage = [&](int it) __attribute__((always_inline)) {
-        const int r = tile_row(it);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            if constexpr (FMT == FMT_F16)
-                copy(kv, it, r);
-            else
-                fetch(kv, it, r);
-        }
-    };
-    auto staged = [&](int it) __attribute__((always_inline)) {
-        if constexpr (FMT == FMT_Q8) {
-            put(0, it);
-            put(1, it);
-        }
-    };
-    if (it0 < it1) {
-        stage(it0);
-        staged(it0);
-    }
     for (int it = it0; it < it1; ++it) {
         staged_barrier<0>();
         if (it + 1 < it1) stage(it + 1);
