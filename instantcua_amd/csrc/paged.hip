@@ -79,7 +79,8 @@ __device__ __forceinline__ f32x4 rotate4(f32x4 x, f32x4 o, int d, int rot, bool 
 }
 
 // 16 lanes a (token, head) vector, 16 vectors a workgroup.  Bound by memory: a token's row is read once
-// and its queries, keys and values written once.
+// and its queries, keys and values written once.  4096 tokens of 16 + 8 + 8 heads, fp32 in, fp16 out: 101 MB in
+// 24 us, 4.2 TB/s, four fifths of what a copy reaches; eight tokens: 3.5 us, a launch.
 template <int TYPE, int QTYPE, int FMT>
 __global__ __launch_bounds__(256) void paged_store_kernel(PagedStoreArgs a) {
     const int nvec = a.n_heads + 2 * a.map.n_kv;
@@ -148,7 +149,8 @@ __global__ __launch_bounds__(256) void paged_store_kernel(PagedStoreArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------
-// Read-back: 16 lanes a (row, KV head), 8 values a lane, K and V by one lane.
+// Read-back: 16 lanes a (row, KV head), 8 values a lane, K and V by one lane.  Bound by memory: 16 sessions of up
+// to 16384 fp16 slots in 186 us, 5.8 TB/s of reads and writes; 4096 q8 slots, 26 MB, in 7 us.
 template <int TYPE, int FMT>
 __global__ __launch_bounds__(256) void paged_load_kernel(PagedLoadArgs a) {
     const int64_t i = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
@@ -458,8 +460,12 @@ __device__ __forceinline__ int few_per(const PagedAttnArgs& a, int total) {
 }
 
 // A workgroup of NW waves: its waves take 32-slot steps of a sequence in turn and join through LDS.  K and V
-// go from memory to registers, as each is used by one tile alone, a step ahead of its products.  Bound by
-// memory.
+// go from memory to registers, as each is used by one tile alone, a step ahead of its products: two waves a SIMD
+// with a step in flight each; three or four without one are no faster, and a step ahead with three does not fit
+// the registers.  A step's latency is 2.4 us from memory, the queries' and tables' before it some 2 us, so a
+// single token over 4096 slots is bound by latency: 9 us, and 4 to join.  Long caches are bound by memory: eight
+// tokens over up to 32768 fp16 slots 115 us, 5.4 TB/s; 64 tokens over up to 8192 q8 slots 108 us, 4.6 TB/s (a q8
+// step is some 450 instructions, 2.7 us of a wave).
 template <int TYPE, int FMT, int NW>
 __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uint8_t* lds) {
     // fp32 probabilities and, so that only the output's rounding counts, those of q8 in two parts.
@@ -474,202 +480,202 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
     const int per = few_per(a, total), end = min(total, (w + 1) * per);
     int pos = w * per, s0 = 0, before = 0;
     while (pos < end) {
-    // The sequence that has unit pos, and where its units begin.
-    const uint64_t past = __ballot(before + u.end > pos);
-    if (!past) {
-        before += u.sum;
-        s0 += WAVE;
-        if (s0 >= a.n_seqs) return;
-        u = few_units(a, group, s0);
-        continue;
-    }
-    const int at_lane = __ffsll((unsigned long long)past) - 1, seq_end = before + __builtin_amdgcn_readlane(u.end, at_lane);
-    const int seq_units = __builtin_amdgcn_readlane(u.n, at_lane), first = pos - (seq_end - seq_units), count = min(end, seq_end) - pos;
-    const SeqSpan sp = {__builtin_amdgcn_readlane(u.sp.t0, at_lane), __builtin_amdgcn_readlane(u.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.sp.n_kv, at_lane)};
-    const bool whole = count == seq_units;
-    pos += count;
-    const RowOf row = row_of(sp, r16, group, g);
-    // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
-    const int start = first * a.few.unit;
-    const int lim = sp.n_kv, all = sp.n_kv - sp.n_q, c1 = min(lim, start + count * a.few.unit);
-    const int32_t* table = a.tables + (int64_t)(s0 + at_lane) * a.table_width;
-    // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).
-    auto step_slot = [&](int sub, int i) { return sub + ROWS_STEP * (wave + NW * i); };
-    auto lookup = [&](int sub) {
-        const int slot = step_slot(sub, lane / 2) + PAGED_TILE * (lane % 2);
-        return slot < c1 ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
-    };
-    constexpr int SUB = NW * ROWS_STEP * (WAVE / 2);
-    int rows = lookup(start);
-
-    f32x4 O[8];
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = NEG_INF, l = 0.f;
-    int sub = start;
-    auto fetch = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            load_tile<FMT>(a, max(__builtin_amdgcn_readlane(rows, 2 * i + k), 0) + g * a.map.page_slots, lane, t[k]);
-    };
-    // This wave's steps of the window that begin below c1.
-    auto steps = [&]() {
-        const int left = c1 - step_slot(sub, 0);
-        return left <= 0 ? 0 : min(WAVE / 2, (left + NW * ROWS_STEP - 1) / (NW * ROWS_STEP));
-    };
-    const QueryRow<TYPE> qrow = load_query<TYPE>(a, row, q);
-    Tile<FMT> A[2], B[2];
-    no_tile<FMT>(A);
-    no_tile<FMT>(B);
-    int n = steps();
-    if (n > 0) fetch(0, A);
-    const Query<TYPE> y = query_of<TYPE>(qrow, a.scale);
-    auto step = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
-        const int at = step_slot(sub, i);
-        const int ok[2] = {__builtin_amdgcn_readlane(rows, 2 * i) < 0 ? 0 : lim, __builtin_amdgcn_readlane(rows, 2 * i + 1) < 0 ? 0 : lim};
-        float p[8];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const f32x4 sc = tile_scores<TYPE, FMT>(t[k], y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[4 * k + e] = sc[e] * y.c;
+        // The sequence that has unit pos, and where its units begin.
+        const uint64_t past = __ballot(before + u.end > pos);
+        if (!past) {
+            before += u.sum;
+            s0 += WAVE;
+            if (s0 >= a.n_seqs) return;
+            u = few_units(a, group, s0);
+            continue;
         }
-        uint32_t odd = 0;
-        const bool masked = at + ROWS_STEP - 1 > all || ok[0] == 0 || ok[1] == 0;
-        if (masked) {
-            asm volatile("");
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int slot = at + 16 * k + 4 * q + e;
-                    if (slot > row.last || slot >= ok[k]) p[4 * k + e] = NEG_INF;
-                    // Values of slots that no row sees may be anything: they take no part.
-                    if (slot >= ok[k]) {
-                        t[k].v[e] = 0;
-                        if constexpr (FMT == FMT_Q8) t[k].vs[e] = 0;
-                    }
-                }
-        }
-        float mb = NEG_INF;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mb = fmaxf(mb, p[e]);
-        mb = max_x4(mb);
-        if (__ballot(mb > m + P_SLACK)) {
-            asm volatile("");
-            const float m_new = fmaxf(m, mb);
-            const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-            m = m_new;
-            l *= corr;
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt) O[dt] *= corr;
-        }
-        const float base = m == NEG_INF ? 0.f : m - P_SHIFT;
-        v8h ph, pl;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = __builtin_amdgcn_exp2f(p[e] - base);
-            l += x;
-            ph[e] = (f16)x;
-            if constexpr (PLO) pl[e] = (f16)(x - (float)ph[e]);
-        }
-        if constexpr (FMT == FMT_Q8)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) t[k].v[e] ^= 0x80808080u;
-        // Slots that some rows see and others do not: values there that are no numbers are kept out of the
-        // products and go to the rows that see them.
-        auto values = [&](auto finite) __attribute__((always_inline)) {
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt) {
-                VOp<TYPE, FMT> v = v_operand<TYPE, FMT>(t, dt);
-                if (finite) {
-                    keep_finite(v.hi, odd);
-                    if constexpr (VLO) keep_finite(v.lo, odd);
-                }
-                O[dt] = mfma(v.hi, ph, O[dt]);
-                if constexpr (PLO) O[dt] = mfma(v.hi, pl, O[dt]);
-                if constexpr (VLO) O[dt] = mfma(v.lo, ph, O[dt]);
-            }
+        const int at_lane = __ffsll((unsigned long long)past) - 1, seq_end = before + __builtin_amdgcn_readlane(u.end, at_lane);
+        const int seq_units = __builtin_amdgcn_readlane(u.n, at_lane), first = pos - (seq_end - seq_units), count = min(end, seq_end) - pos;
+        const SeqSpan sp = {__builtin_amdgcn_readlane(u.sp.t0, at_lane), __builtin_amdgcn_readlane(u.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.sp.n_kv, at_lane)};
+        const bool whole = count == seq_units;
+        pos += count;
+        const RowOf row = row_of(sp, r16, group, g);
+        // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
+        const int start = first * a.few.unit;
+        const int lim = sp.n_kv, all = sp.n_kv - sp.n_q, c1 = min(lim, start + count * a.few.unit);
+        const int32_t* table = a.tables + (int64_t)(s0 + at_lane) * a.table_width;
+        // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).
+        auto step_slot = [&](int sub, int i) { return sub + ROWS_STEP * (wave + NW * i); };
+        auto lookup = [&](int sub) {
+            const int slot = step_slot(sub, lane / 2) + PAGED_TILE * (lane % 2);
+            return slot < c1 ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
         };
-        if constexpr (VLO)
-            values(masked);  // one copy: two take more registers than there are
-        else if (masked)
-            values(std::true_type());
-        else
-            values(std::false_type());
-        if (__ballot(odd != 0))
-            for (int j = 0; j < ROWS_STEP; ++j) {
-                const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);
-                if (r < 0 || at + j >= lim) continue;
-                const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
-                const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+        constexpr int SUB = NW * ROWS_STEP * (WAVE / 2);
+        int rows = lookup(start);
+
+        f32x4 O[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+        for (int dt = 0; dt < 8; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = NEG_INF, l = 0.f;
+        int sub = start;
+        auto fetch = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int dt = 0; dt < 8; ++dt) {
-                        const uint32_t x = as_u32(row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * e + dt));
-                        O[dt][e] += as_f32(x & sees & no_number(x));
+            for (int k = 0; k < 2; ++k)
+                load_tile<FMT>(a, max(__builtin_amdgcn_readlane(rows, 2 * i + k), 0) + g * a.map.page_slots, lane, t[k]);
+        };
+        // This wave's steps of the window that begin below c1.
+        auto steps = [&]() {
+            const int left = c1 - step_slot(sub, 0);
+            return left <= 0 ? 0 : min(WAVE / 2, (left + NW * ROWS_STEP - 1) / (NW * ROWS_STEP));
+        };
+        const QueryRow<TYPE> qrow = load_query<TYPE>(a, row, q);
+        Tile<FMT> A[2], B[2];
+        no_tile<FMT>(A);
+        no_tile<FMT>(B);
+        int n = steps();
+        if (n > 0) fetch(0, A);
+        const Query<TYPE> y = query_of<TYPE>(qrow, a.scale);
+        auto step = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
+            const int at = step_slot(sub, i);
+            const int ok[2] = {__builtin_amdgcn_readlane(rows, 2 * i) < 0 ? 0 : lim, __builtin_amdgcn_readlane(rows, 2 * i + 1) < 0 ? 0 : lim};
+            float p[8];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const f32x4 sc = tile_scores<TYPE, FMT>(t[k], y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[4 * k + e] = sc[e] * y.c;
+            }
+            uint32_t odd = 0;
+            const bool masked = at + ROWS_STEP - 1 > all || ok[0] == 0 || ok[1] == 0;
+            if (masked) {
+                asm volatile("");
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int slot = at + 16 * k + 4 * q + e;
+                        if (slot > row.last || slot >= ok[k]) p[4 * k + e] = NEG_INF;
+                        // Values of slots that no row sees may be anything: they take no part.
+                        if (slot >= ok[k]) {
+                            t[k].v[e] = 0;
+                            if constexpr (FMT == FMT_Q8) t[k].vs[e] = 0;
+                        }
                     }
             }
-    };
-    while (n > 0) {
-        for (int i = 0; i < n; i += 2) {
-            if (i + 1 < n) fetch(i + 1, B);
-            step(i, A);
-            if (i + 1 < n) {
-                if (i + 2 < n) fetch(i + 2, A);
-                step(i + 1, B);
+            float mb = NEG_INF;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mb = fmaxf(mb, p[e]);
+            mb = max_x4(mb);
+            if (__ballot(mb > m + P_SLACK)) {
+                asm volatile("");
+                const float m_new = fmaxf(m, mb);
+                const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                l *= corr;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) O[dt] *= corr;
             }
+            const float base = m == NEG_INF ? 0.f : m - P_SHIFT;
+            v8h ph, pl;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = __builtin_amdgcn_exp2f(p[e] - base);
+                l += x;
+                ph[e] = (f16)x;
+                if constexpr (PLO) pl[e] = (f16)(x - (float)ph[e]);
+            }
+            if constexpr (FMT == FMT_Q8)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[k].v[e] ^= 0x80808080u;
+            // Slots that some rows see and others do not: values there that are no numbers are kept out of the
+            // products and go to the rows that see them.
+            auto values = [&](auto finite) __attribute__((always_inline)) {
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) {
+                    VOp<TYPE, FMT> v = v_operand<TYPE, FMT>(t, dt);
+                    if (finite) {
+                        keep_finite(v.hi, odd);
+                        if constexpr (VLO) keep_finite(v.lo, odd);
+                    }
+                    O[dt] = mfma(v.hi, ph, O[dt]);
+                    if constexpr (PLO) O[dt] = mfma(v.hi, pl, O[dt]);
+                    if constexpr (VLO) O[dt] = mfma(v.lo, ph, O[dt]);
+                }
+            };
+            if constexpr (VLO)
+                values(masked);  // one copy: two take more registers than there are
+            else if (masked)
+                values(std::true_type());
+            else
+                values(std::false_type());
+            if (__ballot(odd != 0))
+                for (int j = 0; j < ROWS_STEP; ++j) {
+                    const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);
+                    if (r < 0 || at + j >= lim) continue;
+                    const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
+                    const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int dt = 0; dt < 8; ++dt) {
+                            const uint32_t x = as_u32(row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * e + dt));
+                            O[dt][e] += as_f32(x & sees & no_number(x));
+                        }
+                }
+        };
+        while (n > 0) {
+            for (int i = 0; i < n; i += 2) {
+                if (i + 1 < n) fetch(i + 1, B);
+                step(i, A);
+                if (i + 1 < n) {
+                    if (i + 2 < n) fetch(i + 2, A);
+                    step(i + 1, B);
+                }
+            }
+            sub += SUB;
+            if (sub >= c1) break;
+            rows = lookup(sub);
+            n = steps();
+            if (n > 0) fetch(0, A);
         }
-        sub += SUB;
-        if (sub >= c1) break;
-        rows = lookup(sub);
-        n = steps();
-        if (n > 0) fetch(0, A);
-    }
-    // Join the waves: lane (r16, q) of each has dims 32 q + 8 i + dt of row r16.  They go through LDS, [wave][dt]
-    // [q][r16][i], the rows of q padded by four so that the lanes that read it meet no bank twice.
-    l = sum_x4(l);
-    __syncthreads();  // the sequence before is read
-    if (q == 0) sml[wave * 16 + r16] = make_float2(m, l);
+        // Join the waves: lane (r16, q) of each has dims 32 q + 8 i + dt of row r16.  They go through LDS, [wave][dt]
+        // [q][r16][i], the rows of q padded by four so that the lanes that read it meet no bank twice.
+        l = sum_x4(l);
+        __syncthreads();  // the sequence before is read
+        if (q == 0) sml[wave * 16 + r16] = make_float2(m, l);
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) so[(wave * 8 + dt) * ROWS_PITCH + q * 20 + r16] = O[dt];
-    __syncthreads();
-    // A thread writes DIMS values of a row.
-    constexpr int DIMS = 8 * 4 / NW;
-    const int at = threadIdx.x * DIMS, d0 = at % HD, orow = at / HD;
-    const RowOf out = row_of(sp, orow, group, g);
-    if (out.t >= 0 && (whole || orow < a.few.rows)) {
-    float mt = NEG_INF, lt = 0.f;
-    float2 ml[NW];
+        for (int dt = 0; dt < 8; ++dt) so[(wave * 8 + dt) * ROWS_PITCH + q * 20 + r16] = O[dt];
+        __syncthreads();
+        // A thread writes DIMS values of a row.
+        constexpr int DIMS = 8 * 4 / NW;
+        const int at = threadIdx.x * DIMS, d0 = at % HD, orow = at / HD;
+        const RowOf out = row_of(sp, orow, group, g);
+        if (out.t >= 0 && (whole || orow < a.few.rows)) {
+        float mt = NEG_INF, lt = 0.f;
+        float2 ml[NW];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        ml[w] = sml[w * 16 + orow];
-        mt = fmaxf(mt, ml[w].x);
-    }
-    float x[DIMS] = {};
-    const float* src = (const float*)so + (d0 % 8) * ROWS_PITCH * 4 + (d0 / 32) * 80 + orow * 4 + d0 / 8 % 4;
+        for (int w = 0; w < NW; ++w) {
+            ml[w] = sml[w * 16 + orow];
+            mt = fmaxf(mt, ml[w].x);
+        }
+        float x[DIMS] = {};
+        const float* src = (const float*)so + (d0 % 8) * ROWS_PITCH * 4 + (d0 / 32) * 80 + orow * 4 + d0 / 8 % 4;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const float f = ml[w].x == mt ? 1.f : __builtin_amdgcn_exp2f(ml[w].x - mt);
-        lt += ml[w].y * f;
+        for (int w = 0; w < NW; ++w) {
+            const float f = ml[w].x == mt ? 1.f : __builtin_amdgcn_exp2f(ml[w].x - mt);
+            lt += ml[w].y * f;
 #pragma unroll
-        for (int k = 0; k < DIMS; ++k) x[k] += src[(w * 8 + k) * ROWS_PITCH * 4] * f;
-    }
-    const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
-    const int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
+            for (int k = 0; k < DIMS; ++k) x[k] += src[(w * 8 + k) * ROWS_PITCH * 4] * f;
+        }
+        const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+        const int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
 #pragma unroll
-    for (int k = 0; k < DIMS; k += 4) {
-        const f32x4 y = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]} * inv;
-        if (!whole)
-            *(f32x4*)(a.few_part + part * HD + d0 + k) = y;
-        else
-            store4<TYPE>(a.out, (int64_t)out.t * a.out_stride + out.head * HD + d0 + k, y);
-    }
-    if (!whole && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
-    }
+        for (int k = 0; k < DIMS; k += 4) {
+            const f32x4 y = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]} * inv;
+            if (!whole)
+                *(f32x4*)(a.few_part + part * HD + d0 + k) = y;
+            else
+                store4<TYPE>(a.out, (int64_t)out.t * a.out_stride + out.head * HD + d0 + k, y);
+        }
+        if (!whole && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
+        }
     }
 }
 
@@ -679,17 +685,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     rows_work<TYPE, FMT, 4>(a, blockIdx.x, lds);
 }
 
-// Sequences with more query rows: flash attention on 128 rows of a (sequence, KV head) a workgroup, eight
-// waves.  Wave w has rows 32 (w & 3) .. + 31 and of each 128 slots the half w >> 2; the two halves keep
-// softmax states of their own, joined through LDS at the end.  K and V are staged in LDS, two stages of
-// 128 slots, by copies that run under the products (fp16: memory to LDS directly; q8 through registers:
-// dequantised to fp16 for fp16 queries, for fp32 ones as exact codes, whose scales go to the sums of a
-// group's products and to the probabilities in fp32).  v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns, lane (column, h)
-// has slots 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major V by
-// transposing LDS reads.
+// Sequences with more query rows: 128 rows of a (sequence, KV head) a workgroup, eight waves.  Wave w has
+// rows 32 (w & 3) .. + 31 and of each 128 slots the half w >> 2; the two halves keep softmax states of their
+// own, joined through LDS at the end.  v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns,
+// lane (column, h) has slots 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major
+// V by transposing LDS reads.
 //
-// A staged row is 16 chunks of 16 bytes, chunk c at place c ^ swizzle(row): both the operand reads of K
-// (8 rows at one chunk) and of V (4 rows at two chunks) then spread over all banks.
+// K and V are staged in LDS, two stages of 128 slots, by copies that run under the products: fp16 from memory
+// to LDS directly; q8 through registers, as the exact codes in fp16, whose scales go to the groups' sums in fp32
+// and to the probabilities.  (Dequantised K, rounded to fp16, doubles the error of a batch of prompts, 4.8e-4
+// for 2.9e-4; it takes 107 us where this takes 138.)
+//
+// A staged row is 16 chunks of 16 bytes, chunk c at place c ^ swizzle(row): the operand reads of K (16 rows
+// at one chunk) and of V (4 rows at four chunks) then spread over all banks.  With only the low three bits
+// of the place changed they met in half of them, and the reads took twice as long.
+//
+// Bound by the issue of instructions: for 128 slots a SIMD's two waves issue 470 vector instructions (64 of them
+// exponentials, 64 products of 32 cycles), 200 scalar ones and 100 of LDS, in some 4300 cycles; products fill 38 %
+// of them, vector instructions 41 %, LDS 20 %.  Wave priorities and a start of half the waves apart change nothing.
+// A workgroup's first K and V are there 5 us after it starts, and 3 us join and write its rows.  A prompt of 4096
+// tokens, 16 heads: 95 us, 0.73 PFLOP/s of the causal half.
 constexpr int CH_ROWS = 128, CH_HALF = 64;
 constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
 constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
