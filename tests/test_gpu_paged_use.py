@@ -11,8 +11,8 @@ import pytest
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import paged_ref as ref  # noqa: E402
 from instantcua_amd import engine as eng  # noqa: E402
-from instantcua_amd import paged  # noqa: E402
-from instantcua_amd.modelfile import WeightFormat  # noqa: E402
+from instantcua_amd import paged, synth  # noqa: E402
+from instantcua_amd.modelfile import Dims, TensorID, WeightFormat  # noqa: E402
 from test_gpu_paged import D, FMTS, NP, TYPES, dev, download, filled, run_attention, tables_of, upload  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -309,3 +309,45 @@ def test_one_page_may_hold_a_whole_session(fmt):
     got = run_attention(pool, q, (1,), (777,), table, paged.F32)
     want, reach, vmax = ref.attention(pool, q, (1,), (777,), table)
     assert np.abs(got - want).max() <= ref.attention_tol(False, pool.q8, reach, vmax)
+
+
+@pytest.mark.parametrize("pos,n", [(29, 3), (700, 1), (1000, 8)])
+def test_the_operators_compute_the_engines_layer(pos, n):
+    """The engine's fused q|k|v rows of a layer pass, through store and attention on a pool of one page that holds
+    its cache: the engine's K/V rows and attention output.
+
+    Values are rounded from the same fp32 on both sides.  Keys go through the norm's sum and the table's angles
+    first, which differ in their last bits, so some lie on the other side of a rounding: one fp16 step, in at
+    most 2 % of them, and the attention over them within 1e-4 of its largest magnitude, as the engine's own
+    stages are held to their oracle."""
+    img = synth.build_model_image(WeightFormat.Q4, n_layers=2, tag="q4-small")
+    ctx, layer = 1024, 1
+    kc, vc = (synth.fp16_normal((8, pos, D), f"pu-{k}", pos) for k in "kv")
+    x = synth.fp16_normal((n, Dims.hidden), "pu-x", n).astype(np.float32)
+    with eng.Engine(flags=0, image=img, max_context=ctx) as e:
+        e.write_kv(layer, 0, 0, kc)
+        e.write_kv(layer, 1, 0, vc)
+        e.layer_step(layer, x, pos)
+        qkv, want = e.read_buffer("qkv")[:n], e.read_buffer("attn")[:n].reshape(n, 16, D)
+        rows = [e.read_kv(layer, kind, pos, n) for kind in range(2)]
+    pool = ref.Pool(WeightFormat.F16, 8, ctx, 1)
+    pool.data[0][0, :, :pos], pool.data[1][0, :, :pos] = kc, vc
+    cache = upload(pool)
+    norms = [dev(synth.tensor_view(img, TensorID.llm_layer(layer, i)).view(np.float32).copy()) for i in (TensorID.q_norm, TensorID.k_norm)]
+    # The engine's table: the angle is a product in fp32 (Engine.swift:121-125), up to 2^-14 off at slot 1000.
+    angle = (np.arange(ctx, dtype=np.float32)[:, None] * (Dims.rope_theta ** -(np.arange(0, D, 2) / D)).astype(np.float32)).astype(np.float64)
+    rope = np.stack([np.cos(angle), np.sin(angle)], axis=-1).astype(np.float32)
+    at, q, out = np.arange(pos, pos + n, dtype=np.int32), eng.DeviceBuffer(n * 16 * D * 4), eng.DeviceBuffer(n * 16 * D * 4)
+    cache.store(dev(qkv), n, dev(at), n_heads=16, q=q, q_norm=norms[0], k_norm=norms[1], rope=dev(rope), rope_rows=ctx, pos=dev(at))
+    sizes = dict(max_q=n, max_kv=ctx)
+    work = eng.DeviceBuffer(max(16, cache.attention_work(16, 1, n, table_width=1, **sizes)))
+    cache.attention(q, out, 16, dev(np.array([0, n], np.int32)), dev(np.array([pos + n], np.int32)), dev(np.zeros((1, 1), np.int32)),
+                    1, n, 1, work=work, **sizes)
+    after = download(cache, pool)
+    got_k, got_v = (after.data[i][0, :, pos:pos + n] for i in range(2))
+    assert np.array_equal(got_v.view(np.uint16), rows[1].view(np.uint16))
+    k, w = got_k.astype(np.float32), rows[0].astype(np.float32)
+    step = np.spacing(np.abs(rows[0])).astype(np.float32)
+    assert (np.abs(k - w) <= step + 1e-6 * np.abs(w).max()).all() and (k != w).mean() < 2e-2
+    got = out.to_array(np.float32, (n, 16, D))
+    assert np.abs(got - want).max() <= 1e-4 * np.abs(want).max()
