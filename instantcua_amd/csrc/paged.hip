@@ -1178,7 +1178,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     const v4h sc = *(const v4h*)(scales + 4 * CH_HALF + dt * CH_HALF + 32 * kt + 16 * c + 8 * k + 4 * h);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = p[8 * c + 4 * k + e] * ((float)sc[e] * down);
+                        float x = p[8 * c + 4 * k + e] * ((float)sc[e] * down);
+                        // One value for both parts: else the compiler rounds the product itself to fp16 for one
+                        // of them, which next to a tie is not its fp32 value rounded.
+                        asm("" : "+v"(x));
                         ph[4 * k + e] = (f16)x;
                         pl[4 * k + e] = (f16)(x - (float)ph[4 * k + e]);
                     }

@@ -351,3 +351,18 @@ def test_the_operators_compute_the_engines_layer(pos, n):
     assert (np.abs(k - w) <= step + 1e-6 * np.abs(w).max()).all() and (k != w).mean() < 2e-2
     got = out.to_array(np.float32, (n, 16, D))
     assert np.abs(got - want).max() <= 1e-4 * np.abs(want).max()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [8, 33])
+def test_fp32_probabilities_keep_both_parts(fmt, m):
+    """Flat softmaxes over few slots, where a probability whose fp16 parts do not add up to it would show: the
+    outputs are within the fp32 bound (2^-12 / 8 of a value, for a part rounded otherwise than the other
+    expects among eight slots, is ten times as much), over enough rows for roundings next to a tie."""
+    rng = np.random.default_rng(35)
+    lens = (m,) * 60
+    pool, table = filled(fmt, 4, 48, lens, rng)
+    q = rng.standard_normal((60 * m, 8, D)).astype(np.float32)
+    got = run_attention(pool, q, lens, lens, table, paged.F32, scale=1e-3)
+    want, reach, vmax = ref.attention(pool, q, lens, lens, table, scale=1e-3)
+    assert np.abs(got - want).max() <= ref.attention_tol(False, pool.q8, reach, vmax)
