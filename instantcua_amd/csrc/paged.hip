@@ -1319,7 +1319,7 @@ __device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int hea
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int i = i0 + 2 * k + (lane >> 5);
-            const float w = i < n ? __shfl(f, i) : 0.f;
+            const float w = __shfl(f, i);  // 0 past the last; by all lanes, as an inactive one hands nothing over
             if (w != 0.f) o += x[k] * w;
         }
     }

@@ -366,3 +366,19 @@ def test_fp32_probabilities_keep_both_parts(fmt, m):
     got = run_attention(pool, q, lens, lens, table, paged.F32, scale=1e-3)
     want, reach, vmax = ref.attention(pool, q, lens, lens, table, scale=1e-3)
     assert np.abs(got - want).max() <= ref.attention_tol(False, pool.q8, reach, vmax)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [1, 20])
+def test_attention_joins_any_number_of_partials(fmt, type_, m):
+    """Sequences of 1 .. 64 units of 128 slots, each alone in a call, so that every number of partials is joined."""
+    rng = np.random.default_rng(36)
+    pool, table = filled(fmt, 1, 128, (64 * 128,), rng)
+    q = rng.standard_normal((m, 2, D)).astype(NP[type_])
+    cache = upload(pool)
+    for units in (1, 2, 3, 16, 17, 31, 32, 33, 34, 35, 47, 48, 49, 62, 63, 64):
+        kv = 128 * units - 5
+        got = run_attention(pool, q, (m,), (kv,), table, type_, cache=cache)
+        want, reach, vmax = ref.attention(pool, q, (m,), (kv,), table)
+        assert np.abs(got - want).max() <= ref.attention_tol(type_ == paged.F16, pool.q8, reach, vmax), units
