@@ -382,10 +382,10 @@ __device__ __forceinline__ f32x4 tile_scores(const Tile<FMT>& t, const Query<TYP
 }
 
 // The V^T operand dims 8 r16 + dt of two tiles over this lane's eight slots (4 q .. + 3 of each tile), hi
-// and, for q8 with fp32 queries, the lo part of the exact product code x scale.
+// and, for q8, the lo part of the exact product code x scale.
 template <int TYPE, int FMT>
 struct VOp {
-    static constexpr bool LO = FMT == FMT_Q8 && TYPE == TYPE_F32;
+    static constexpr bool LO = FMT == FMT_Q8;
     v8h hi, lo;
 };
 template <int TYPE, int FMT>
@@ -465,12 +465,13 @@ __device__ __forceinline__ int few_per(const PagedAttnArgs& a, int total) {
 // with a step in flight each; three or four without one are no faster, and a step ahead with three does not fit
 // the registers.  A step's latency is 2.4 us from memory, the queries' and tables' before it some 2 us, so a
 // single token over 4096 slots is bound by latency: 9 us, and 4 to join.  Long caches are bound by memory: eight
-// tokens over up to 32768 fp16 slots 115 us, 5.4 TB/s; 64 tokens over up to 8192 q8 slots 108 us, 4.6 TB/s (a q8
+// tokens over up to 32768 fp16 slots 115 us, 5.4 TB/s; 64 tokens over up to 8192 q8 slots 111 us, 4.5 TB/s (a q8
 // step is some 450 instructions, 2.7 us of a wave).
 template <int TYPE, int FMT, int NW>
 __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uint8_t* lds) {
-    // fp32 probabilities and, so that only the output's rounding counts, those of q8 in two parts.
-    constexpr bool PLO = TYPE == TYPE_F32 || FMT == FMT_Q8, VLO = VOp<TYPE, FMT>::LO;
+    // fp32 probabilities in two parts.  With fp16 queries and q8, two parts of V cost as much as two of the
+    // probabilities and leave the smaller error (2.5e-4 for 2.9e-4 of the outputs' rms, 2.1e-4 the output's own).
+    constexpr bool PLO = TYPE == TYPE_F32, VLO = VOp<TYPE, FMT>::LO;
     f32x4* const so = (f32x4*)lds;                                  // [NW][8][ROWS_PITCH]
     float2* const sml = (float2*)(lds + NW * 8 * ROWS_PITCH * 16);  // [NW][16]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
@@ -601,7 +602,7 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                 }
             };
             if constexpr (VLO)
-                values(masked);  // one copy: two take more registers than there are
+                values(masked);  // one copy: two take more registers than there are (134 us for 111)
             else if (masked)
                 values(std::true_type());
             else
