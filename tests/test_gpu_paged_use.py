@@ -382,3 +382,30 @@ def test_attention_joins_any_number_of_partials(fmt, type_, m):
         got = run_attention(pool, q, (m,), (kv,), table, type_, cache=cache)
         want, reach, vmax = ref.attention(pool, q, (m,), (kv,), table)
         assert np.abs(got - want).max() <= ref.attention_tol(type_ == paged.F16, pool.q8, reach, vmax), units
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("q_lens", [(1, 0, 1, 2), (1, 0, 60, 2)])
+def test_bounds_may_be_loose(fmt, type_, q_lens):
+    """A padded batch: sequences without tokens or slots behind the others, tables wider than any sequence with
+    anything in the unused entries, no bound on tokens or slots given."""
+    rng = np.random.default_rng(37)
+    kv_lens = (900, 40, 333, 2)
+    pool, table = filled(fmt, 2, 32, kv_lens, rng)
+    wide = rng.integers(-2 ** 31, 2 ** 31 - 1, (7, 200)).astype(np.int32)
+    for i, n in enumerate(kv_lens):
+        wide[i, :-(-n // 32)] = table[i, :-(-n // 32)]
+    T, room = sum(q_lens), sum(q_lens) + 30
+    q = np.full((room, 4, D), np.nan, NP[type_])
+    q[:T] = rng.standard_normal((T, 4, D))
+    cache, out = upload(pool), dev(np.full((room, 4, D), 7, NP[type_]))
+    start = np.concatenate([[0], np.cumsum(q_lens), [T] * 3]).astype(np.int32)
+    n = cache.attention_work(4, 7, room, table_width=200)
+    work = dev(np.full(n + 64, 0xFF, np.uint8))
+    cache.attention(dev(q), out, 4, dev(start), dev(np.array(kv_lens + (0, 50, 0), np.int32)), dev(wide), 7, room, 200,
+                    type=type_, work=work)
+    got = out.to_array(NP[type_], (room, 4, D))
+    assert (got[T:] == 7).all() and (work.to_array(np.uint8, (n + 64,))[n:] == 0xFF).all()
+    want, reach, vmax = ref.attention(pool, q[:T], q_lens, kv_lens, table)
+    assert np.abs(got[:T] - want).max() <= ref.attention_tol(type_ == paged.F16, pool.q8, reach, vmax)
