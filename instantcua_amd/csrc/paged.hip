@@ -1195,10 +1195,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int i = 0; i < 16; ++i) O[dt][i] += up * y[i];
         }
     };
+    // Whether some row of the workgroup does not see all of an iteration: of an f16 pool, all of its values are
+    // made finite then, also for waves whose rows see them.
+    auto cleaned = [&](int it) __attribute__((always_inline)) { return it * 128 + 127 > before + tile * CH_ROWS / group; };
     // Values that are no numbers were kept out of the products: they go to the rows that see them.
     auto add_odd_values = [&](int it) __attribute__((always_inline)) {
         const int base = base_of(it);
-        if (FMT == FMT_F16 && base + CH_HALF - 1 <= w_first) return;
+        if (FMT == FMT_F16 && !cleaned(it)) return;
         const int4 odd = *(const int4*)(tile_odd + (it & 1) * 8 + 4 * par);
         if (!__builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w)) return;
         auto b = arguments();
@@ -1219,7 +1222,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // Slots that some rows of the workgroup see and others do not may hold values that are no numbers: in
     // iterations that have such slots each wave makes its tile of V finite.  (q8: when it is put to LDS.)
     auto clean_values = [&](int it) __attribute__((always_inline)) {
-        if (it * 128 + 127 <= before + tile * CH_ROWS / group) return;
+        if (!cleaned(it)) return;
         asm volatile("");
         uint32_t odd = 0;
         uint8_t* vt = lds + half_at(1, it & 1, par) + wi * 16 * HD * 2 + lane * 16;
