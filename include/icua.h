@@ -251,8 +251,9 @@ typedef struct {
  * head (norm NULL: y = x), then the rotation of the first rot_dim values by the table row of the
  * token's position, pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`.  Queries go to q,
  * keys and values to the pool: rounded to fp16, or quantised with the bytes that icua_quantize gives.
- * Arithmetic is fp32.  Keys and values are at most 65504 in magnitude, the largest fp16 (larger ones become
- * infinities).
+ * Arithmetic is fp32.  In an f16 pool keys and values are at most 65504 in magnitude, the largest fp16 (larger
+ * ones become infinities).  A q8 pool holds groups of up to 127 * 65504; code times scale may be half a step
+ * above the value (65532 for 65504), which fp32 outputs hold and fp16 ones round to an infinity.
  * A token whose slot is outside the pool (-1, say) has its queries made and is not stored; one whose
  * position is outside the table gets NaN queries and is not stored.  The slots of one call differ. */
 typedef struct {

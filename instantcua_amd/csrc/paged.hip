@@ -381,8 +381,12 @@ __device__ __forceinline__ f32x4 tile_scores(const Tile<FMT>& t, const Query<TYP
     return s;
 }
 
+// q8: the largest scale (its fp16 bits) whose products with codes are all fp16 numbers: 256.
+constexpr uint16_t V_TOP = 0x5C00;
+__device__ __forceinline__ bool beyond_fp16(uint16_t scale) { return (scale & 0x7FFF) > V_TOP; }
+
 // The V^T operand dims 8 r16 + dt of two tiles over this lane's eight slots (4 q .. + 3 of each tile), hi
-// and, for q8, the lo part of the exact product code x scale.
+// and, for q8, the lo part of the exact product code x scale (scales up to V_TOP).
 template <int TYPE, int FMT>
 struct VOp {
     static constexpr bool LO = FMT == FMT_Q8;
@@ -415,11 +419,11 @@ __device__ __forceinline__ VOp<TYPE, FMT> v_operand(const Tile<FMT>* t, int dt) 
     return o;
 }
 
-// Value d of a row of V, as the products take it.
+// Value d of a row of V.
 template <int FMT>
 __device__ __forceinline__ float row_value(const void* v, const void* v_sb, int64_t row, int d) {
     if constexpr (FMT == FMT_F16) return (float)((const f16*)v)[row * HD + d];
-    return (float)(f16)(h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d]);
+    return h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d];
 }
 
 // Sequences with at most 16 query rows a KV head (single tokens, drafts).  Their slots, in units of a step
@@ -581,32 +585,72 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                 ph[e] = (f16)x;
                 if constexpr (PLO) pl[e] = (f16)(x - (float)ph[e]);
             }
-            if constexpr (FMT == FMT_Q8)
+            // q8: groups of slots with scales beyond V_TOP, or that are no numbers, are kept out of the products
+            // (scale 0) and added in fp32.
+            bool beyond = false;
+            if constexpr (FMT == FMT_Q8) {
+                typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                u16x2 top = {0, 0};
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) t[k].v[e] ^= 0x80808080u;
-            // Slots that some rows see and others do not: values there that are no numbers are kept out of the
-            // products and go to the rows that see them.
+                    for (int e = 0; e < 4; ++e) {
+                        t[k].v[e] ^= 0x80808080u;
+                        if (e % 2 == 0)
+                            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, ((uint32_t)t[k].vs[e] | (uint32_t)t[k].vs[e + 1] << 16) & 0x7FFF7FFFu));
+                    }
+                beyond = __ballot(max(top.x, top.y) > V_TOP) != 0;
+                if (beyond) {
+                    asm volatile("");
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (beyond_fp16(t[k].vs[e])) t[k].vs[e] = 0;
+                }
+            }
+            // f16, slots that some rows see and others do not: values there that are no numbers are kept out of
+            // the products and go to the rows that see them.
             auto values = [&](auto finite) __attribute__((always_inline)) {
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt) {
                     VOp<TYPE, FMT> v = v_operand<TYPE, FMT>(t, dt);
-                    if (finite) {
-                        keep_finite(v.hi, odd);
-                        if constexpr (VLO) keep_finite(v.lo, odd);
-                    }
+                    if constexpr (finite) keep_finite(v.hi, odd);
                     O[dt] = mfma(v.hi, ph, O[dt]);
                     if constexpr (PLO) O[dt] = mfma(v.hi, pl, O[dt]);
                     if constexpr (VLO) O[dt] = mfma(v.lo, ph, O[dt]);
                 }
             };
-            if constexpr (VLO)
-                values(masked);  // one copy: two take more registers than there are (134 us for 111)
+            if constexpr (FMT == FMT_Q8)
+                values(std::false_type());
             else if (masked)
                 values(std::true_type());
             else
                 values(std::false_type());
+            if (beyond)
+                for (int j = 0; j < ROWS_STEP; ++j) {
+                    const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);
+                    if (r < 0 || at + j >= lim) continue;
+                    // The row's probability is lane (r16, j % 16 / 4)'s, element 4 (j / 16) + j % 4.
+                    auto of_slot = [&](const v8h& p8) __attribute__((always_inline)) {
+                        const u32x4 w = __builtin_bit_cast(u32x4, p8);
+                        const uint32_t two = j & 16 ? (j & 2 ? w[3] : w[2]) : (j & 2 ? w[1] : w[0]);
+                        return h2f((uint16_t)(__shfl((int)two, r16 + 16 * (j % 16 / 4)) >> (16 * (j & 1))));
+                    };
+                    float pj = of_slot(ph);
+                    if constexpr (PLO) pj += of_slot(pl);
+                    const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
+                    const uint16_t scale = ((const uint16_t*)a.v_sb)[vrow * NG + q];  // dims 32 q .. + 31 are group q
+                    const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+                    if (!beyond_fp16(scale)) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int dt = 0; dt < 8; ++dt) {
+                            const float x = row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * e + dt);
+                            O[dt][e] += no_number(as_u32(x)) ? as_f32(as_u32(x) & sees) : pj * x;
+                        }
+                }
             if (__ballot(odd != 0))
                 for (int j = 0; j < ROWS_STEP; ++j) {
                     const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);

@@ -6,9 +6,11 @@ import numpy as np
 import pytest
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import paged_bounds as bounds  # noqa: E402
 import paged_ref as ref  # noqa: E402
 from instantcua_amd import paged  # noqa: E402
-from test_gpu_paged import D, FMTS, NP, TYPES, filled, run_attention  # noqa: E402
+from instantcua_amd.modelfile import WeightFormat  # noqa: E402
+from test_gpu_paged import D, FMTS, NP, TYPES, dev, download, filled, run_attention, upload  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +57,73 @@ def test_values_that_are_no_numbers_reach_the_rows_that_see_them(fmt, type_, wha
             pool.scales[1][at] = kept
         else:
             pool.data[1][at] = kept
+
+
+def by_group(x):
+    return x.reshape(*x.shape[:-1], 4, 32)
+
+
+def of_sequences(pool, q, q_lens, kv_lens, table, got, floor=0.0, scale=None, type_=paged.F32):
+    """Outputs of every sequence against the definition, groups of 32 dims by themselves."""
+    group, at = q.shape[1] // pool.n_kv, 0
+    for s, (m, n) in enumerate(zip(q_lens, kv_lens)):
+        want, reach, _ = ref.attention(pool, q[at:at + m], (m,), (n,), table[s:s + 1], scale=scale)
+        bound = bounds.rms_bound(type_ == paged.F16, pool.q8, bounds.chunked(m, group), reach, n)
+        out = got[at:at + m].copy()
+        if type_ == paged.F16:  # outputs that round to infinities; next to the border (2^-9 are two and more bounds) either may be
+            assert (out == np.copysign(np.inf, want))[np.abs(want) > 65520 * (1 + 2.0 ** -9)].all()
+            big = np.abs(want) > 65520 * (1 - 2.0 ** -9)
+            out[big] = want[big] = 0
+        bounds.check(by_group(out), by_group(want), bound, floor)
+        at += m
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m", [1, 6])
+@pytest.mark.parametrize("size", [516.0, -516.0, 3000.0, 65504.0])
+def test_q8_values_beyond_fp16(type_, m, size):
+    """Groups whose values (code times scale) are beyond what fp16 holds are exact for single tokens and drafts,
+    also for tokens that do not see them."""
+    q8_values_beyond_fp16(type_, m, size)
+
+
+def q8_values_beyond_fp16(type_, m, size):
+    rng = np.random.default_rng(52)
+    q_lens, kv_lens = (m, 2), (300, 64)
+    pool, table = filled(WeightFormat.Q8, 2, 32, kv_lens, rng)
+    for slot, g in ((20, 1), (299 - m // 2, 2), (299, 0)):
+        at = table[0, slot // 32], slice(None), slot % 32
+        pool.scales[1][at][..., g] = size
+        pool.data[1][at][..., 32 * g:32 * g + 32:5] = 127
+        pool.data[1][at][..., 32 * g + 1:32 * g + 32:5] = -127
+    q = (0.3 * rng.standard_normal((m + 2, 4, D))).astype(NP[type_])
+    got = run_attention(pool, q, q_lens, kv_lens, table, type_)
+    of_sequences(pool, q, q_lens, kv_lens, table, got, type_=type_)
+
+
+def test_a_stored_value_of_65504_is_read_alike():
+    """The largest value that the store takes, from a q8 pool: single tokens, drafts, chunks and an fp32 load
+    have what code and scale say; an fp16 load rounds it."""
+    rng = np.random.default_rng(53)
+    T, page = 60, 16
+    pool = ref.Pool(WeightFormat.Q8, 2, page, 4)
+    cache = upload(pool)
+    x = rng.standard_normal((T, 4, D)).astype(np.float32)
+    x[7, 2:, 3], x[9, 2:, 40], x[59, 2:, 100] = 65504, -65500, 65469
+    x[11, 2:, 64:96] = np.where(np.arange(32) % 2, -65504, 65504)
+    slots = np.arange(T, dtype=np.int32)
+    cache.store(dev(x), T, dev(slots))
+    after = download(cache, pool)
+    values = after.values(1, slots)
+    assert values[7, :, 3].max() == 65532 and np.abs(values - x[:, 2:]).max() <= 516 / 2
+    for type_ in TYPES:
+        v = dev(np.zeros((T, 2, D), NP[type_]))
+        cache.load(dev(slots), T, None, v, type=type_)
+        with np.errstate(over="ignore"):
+            assert np.array_equal(v.to_array(NP[type_], (T, 2, D)), values.astype(NP[type_]))
+    table = np.arange(4, dtype=np.int32)[None]
+    for type_ in TYPES:
+        for m in (1, 6, 40):
+            q = (0.1 * rng.standard_normal((m, 4, D))).astype(NP[type_])
+            got = run_attention(after, q, (m,), (T,), table, type_, cache=cache)
+            of_sequences(after, q, (m,), (T,), table, got, type_=type_)
