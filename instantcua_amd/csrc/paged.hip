@@ -754,10 +754,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 constexpr int CH_ROWS = 128, CH_HALF = 64;
 constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
 constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
-// q8: a half's scales [K, V][group][slot] and the largest of V, [group][16-slot tile].
-constexpr int CH_SCALES = 8 * CH_HALF * 2 + 16 * 4;
+constexpr int CH_SCALES = 8 * CH_HALF * 2;      // q8: a half's scales [K, V][group][slot]
 // And for the eight tiles of two stages whether V has values that are no numbers, whether the page exists, and
-// the power of two that V's scales are below.
+// (q8, fp16 queries) the power of two that V's scales are below.
 constexpr int CH_FLAGS = 2 * CH_STAGE + 4 * CH_SCALES, CH_LDS = CH_FLAGS + 192;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -883,7 +882,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     auto half_at = [&](int kv, int st, int hb) { return (uint32_t)((kv * 2 + st) * 2 + hb) * CH_MAT; };
     auto scales_at = [&](int st, int hb) { return (f16*)(lds + 2 * CH_STAGE + (st * 2 + hb) * CH_SCALES); };
-    auto tops_at = [&](int st, int hb) { return (float*)(scales_at(st, hb) + 8 * CH_HALF); };
     // fp16: this wave's tile of iteration it, pool row r, from memory to LDS; slots that are not there become
     // zeros.  Row l / 16 (+ 4 j) of the tile, place l % 16.
     int src_off[4];
@@ -945,7 +943,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             *(u32x4*)(dst + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
         }
         scales_at(it & 1, par)[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = sc;
-        if (kv) {  // the largest scale of each group: over the lanes with the same l % 4
+        if (kv && !HL) {  // the largest scale
             int top = scale[1] & 0x7FFF;  // fp16 bits rise with the value
             top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x124, 0xF, 0xF, true));  // row_ror:4, 8: within 16 lanes
             top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x128, 0xF, 0xF, true));
@@ -953,13 +951,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             top = max((int)r16[0], (int)r16[1]);
             auto r32 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
             top = max((int)r32[0], (int)r32[1]);
-            if constexpr (HL) {
-                if (lane < 4) tops_at(it & 1, par)[4 * lane + wi] = h2f((uint16_t)top);
-            } else {
-                top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR1, 0xF, 0xF, true));
-                top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR2, 0xF, 0xF, true));
-                if (lane == 0) tile_top[(it & 1) * 8 + wave] = (top >> 10) - 14;
-            }
+            top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR1, 0xF, 0xF, true));
+            top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR2, 0xF, 0xF, true));
+            if (lane == 0) tile_top[(it & 1) * 8 + wave] = (top >> 10) - 14;
         }
     };
 
@@ -1196,13 +1190,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         l += sum[0] + sum[1];
     };
-    // fp32 queries: a block's dims 32 dt .. + 31 are one group, whose scales, by the power of two that brings
-    // the half's largest below 1, go to the probabilities, and the power to the sum.
+    // fp32 queries: a block's dims 32 dt .. + 31 are one group, whose scales go to the probabilities.  A row's
+    // products of the two, by the power of two that puts the largest in [2^14, 2^15), are split into fp16 hi + lo
+    // parts, and the power goes to the sum: values that the row does not see, or gives little weight, take nothing
+    // from its accuracy, however large.  (By the power of the largest scale instead, a value of 65504 at a later
+    // token left 1.2e-4 of error to rows of small values.)
     auto exact_values = [&](int it, int kt, const f32x16& S) __attribute__((always_inline)) {
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
         const uint32_t Vs = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
-        const f16* scales = scales_at(it & 1, par);
-        const float* all_tops = tops_at(it & 1, par);
+        const f16* scales = scales_at(it & 1, par) + 4 * CH_HALF + 32 * kt + 4 * h;
         float p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1211,25 +1207,30 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) {
-            const f32x4 tops = *(const f32x4*)(all_tops + 4 * dt);
-            const int e2 = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+            float x[16], top = 0.f;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const v4h sc = *(const v4h*)(scales + dt * CH_HALF + 8 * b);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[4 * b + e] = p[4 * b + e] * (float)sc[e];
+                    top = fmaxf(top, fabsf(x[4 * b + e]));
+                }
+            }
+            const int e2 = max(__builtin_amdgcn_frexp_expf(max_x2(top)), -100) - 15;
             const float down = ldexpf(1.f, -e2), up = ldexpf(1.f, e2);
             f32x16 y = {};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 v8h ph, pl;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const v4h sc = *(const v4h*)(scales + 4 * CH_HALF + dt * CH_HALF + 32 * kt + 16 * c + 8 * k + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = p[8 * c + 4 * k + e] * ((float)sc[e] * down);
-                        // One value for both parts: else the compiler rounds the product itself to fp16 for one
-                        // of them, which next to a tie is not its fp32 value rounded.
-                        asm("" : "+v"(x));
-                        ph[4 * k + e] = (f16)x;
-                        pl[4 * k + e] = (f16)(x - (float)ph[4 * k + e]);
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    float z = x[8 * c + e] * down;
+                    // One value for both parts: else the compiler rounds the product itself to fp16 for one
+                    // of them, which next to a tie is not its fp32 value rounded.
+                    asm("" : "+v"(z));
+                    ph[e] = (f16)z;
+                    pl[e] = (f16)(z - (float)ph[e]);
                 }
                 const v8h v = v_operand(Vs, c, dt);
                 y = mfma32(v, ph, y);

@@ -127,3 +127,28 @@ def test_a_stored_value_of_65504_is_read_alike():
             q = (0.1 * rng.standard_normal((m, 4, D))).astype(NP[type_])
             got = run_attention(after, q, (m,), (T,), table, type_, cache=cache)
             of_sequences(after, q, (m,), (T,), table, got, type_=type_)
+
+
+@pytest.mark.parametrize("size", [516.0, -516.0, 3000.0, 65504.0])
+def test_q8_values_beyond_fp16_in_chunks_of_fp32_queries(size):
+    q8_values_beyond_fp16(paged.F32, 40, size)
+
+
+@pytest.mark.parametrize("where", ["later", "light"])
+@pytest.mark.parametrize("m", [5, 60])
+def test_large_values_leave_rows_exact_that_do_not_see_them(m, where):
+    """fp32 queries over small q8 values: a value of 65504 at a later token, or a large one at a slot of next to no
+    weight, takes nothing from the accuracy of a row."""
+    rng = np.random.default_rng(57)
+    kv = 126
+    pool, table = filled(WeightFormat.Q8, 2, 16, (kv,), rng)
+    pool.scales[0][:] = np.where(np.isnan(pool.scales[0]), np.nan, 1e-3)
+    pool.scales[1][:] = np.where(np.isnan(pool.scales[1]), np.nan, 1e-4 * rng.uniform(0.6, 1, pool.scales[1].shape))
+    if where == "later":
+        pool.scales[1][table[0, (kv - 1) // 16], :, (kv - 1) % 16] = 516
+    else:
+        at = table[0, 4], slice(None), 3  # slot 67, a score of -60 log 2
+        pool.data[0][at], pool.scales[0][at], pool.scales[1][at] = -127, 60 * np.log(2) / (4 * 127 * D ** 0.5), 500
+    q = (4 + 0.1 * rng.standard_normal((m, 4, D))).astype(np.float32)
+    got = run_attention(pool, q, (m,), (kv,), table, paged.F32)
+    of_sequences(pool, q, (m,), (kv,), table, got)
