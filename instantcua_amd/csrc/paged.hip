@@ -928,7 +928,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const bool odd = kv && __ballot(!(fabsf(h2f(scale[1])) <= 65504.f));
         if (kv && lane == 0) tile_odd[(it & 1) * 8 + wave] = odd;
         if (kv && !(fabsf(h2f(scale[1])) <= 65504.f)) scale[1] = 0;
-        const f16 sc = __builtin_bit_cast(f16, scale[kv]);
+        f16 sc = __builtin_bit_cast(f16, scale[kv]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const u32x4 w = codes[kv][k / 2];
@@ -942,8 +942,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
             *(u32x4*)(dst + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
         }
-        scales_at(it & 1, par)[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = sc;
-        if (kv && !HL) {  // the largest scale
+        if (kv && !HL) {  // the power of two that the largest scale is below; where less than 1, scales are raised by it
             int top = scale[1] & 0x7FFF;  // fp16 bits rise with the value
             top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x124, 0xF, 0xF, true));  // row_ror:4, 8: within 16 lanes
             top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x128, 0xF, 0xF, true));
@@ -953,8 +952,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             top = max((int)r32[0], (int)r32[1]);
             top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR1, 0xF, 0xF, true));
             top = max(top, __builtin_amdgcn_update_dpp(0, top, DPP_XOR2, 0xF, 0xF, true));
-            if (lane == 0) tile_top[(it & 1) * 8 + wave] = (top >> 10) - 14;
+            top = (top >> 10) - 14;
+            if (lane == 0) tile_top[(it & 1) * 8 + wave] = top;
+            sc *= __builtin_bit_cast(f16, (uint16_t)((15 - min(top, 0)) << 10));
         }
+        scales_at(it & 1, par)[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = sc;
     };
 
     auto stage = [&](int it) __attribute__((always_inline)) {
@@ -1061,10 +1063,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 16; ++i) mb = fmaxf(mb, S[i]);
         return mb;
     };
-    // The maximum that is subtracted follows the true one when that is more than 2^P_SLACK ahead.
-    auto follow_max = [&](float mb, float up) __attribute__((always_inline)) {
-        mb = max_x2(mb) * qc + up;
-        if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK)) {
+    // The maximum that is subtracted follows the true one when that is more than 2^P_SLACK ahead.  q8 with fp16
+    // queries: the values' sums have a maximum of their own, of scores plus the power of two e that V's scales of
+    // their half are below, and both are whole numbers.
+    constexpr bool WEIGHED = CODES && !HL;
+    float mv = NEG_INF;
+    auto follow_max = [&](float mb, float e) __attribute__((always_inline)) {
+        mb = max_x2(mb) * qc;
+        if constexpr (WEIGHED) {
+            if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK || mb + e > mv + P_SLACK)) {
+                asm volatile("");
+                const float top = __builtin_ceilf(mb), m_new = fmaxf(m, top), mv_new = fmaxf(mv, top + e);
+                const float corr = mv_new == mv ? 1.f : __builtin_amdgcn_exp2f(mv - mv_new);
+                l *= m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                mv = mv_new;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) O[dt] *= corr;
+            }
+        } else if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK)) {
             asm volatile("");
             const float m_new = fmaxf(m, mb);
             const float corr = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
@@ -1156,9 +1173,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
         scale_scores(it, 1, NG - 1, y[1], S[1]);
     };
-    // Values, fp16 queries: the maximum that was subtracted was raised by the power of two that brings the
-    // half's largest scale to 1, so probabilities times scales stay in fp16's range.
-    auto codes_values = [&](int it, const f32x16 S[2]) __attribute__((always_inline)) {
+    // Values, fp16 queries.  A probability p, of 2^P_SHIFT at a score of m, becomes p 2^(m - mv + e) for the sums,
+    // e <= 0 the power of two that its 16 slots' scales were raised by: so p and its products with scales are both
+    // rounded where they have all of fp16's bits, whatever the size of V's values (up to 2^14 apart among 64
+    // slots), and the products end below 2^15.
+    auto codes_values = [&](int it, const f32x16 S[2], const int4& tops) __attribute__((always_inline)) {
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
         const uint32_t st = (it & 1) * 2 * CH_MAT;
         const f16* scales = scales_at(it & 1, par) + 4 * CH_HALF + 4 * h;
@@ -1170,9 +1189,20 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int e = 0; e < 8; ++e)
                 p[c % 2][e / 2][e % 2] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(S[c / 2][8 * (c % 2) + e], qc, -sub_m));
         };
+        // 2^(m - mv + e): at most 2^14, as mv follows wherever m does.
+        const float lead = m == NEG_INF ? 0.f : m - mv;
+        auto factor = [&](int c) __attribute__((always_inline)) {
+            const int e = c == 0 ? tops.x : c == 1 ? tops.y : c == 2 ? tops.z : tops.w;
+            const f16 y = (f16)__builtin_amdgcn_exp2f(lead + (float)min(e, 0));
+            return f16x2{y, y};
+        };
         exponentials(0);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            const f16x2 g = factor(c);
+            f16x2 pg[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pg[k] = p[c % 2][k] * g;
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) {
                 u32x4 ph;
@@ -1180,7 +1210,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int k = 0; k < 2; ++k) {
                     const u32x2 sc = *(const u32x2*)(scales + dt * CH_HALF + 16 * c + 8 * k);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) ph[2 * k + e] = h2_bits(p[c % 2][2 * k + e] * as_h2(sc[e]));
+                    for (int e = 0; e < 2; ++e) ph[2 * k + e] = h2_bits(pg[2 * k + e] * as_h2(sc[e]));
                 }
                 O[dt] = mfma32(v_operand(st, c, dt), __builtin_bit_cast(v8h, ph), O[dt]);
                 sum[dt % 2] = dot2(p[c % 2][dt], ones, sum[dt % 2]);
@@ -1295,22 +1325,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 codes_scores(it, S);
                 mask(it, 0, S[0]);
                 mask(it, 1, S[1]);
-                int up = 0;
-                if constexpr (!HL) {
-                    const int4 tops = *(const int4*)(tile_top + (it & 1) * 8 + 4 * par);
-                    up = max(max(max(tops.x, tops.y), max(tops.z, tops.w)), 0);
-                }
-                follow_max(fmaxf(block_max(S[0]), block_max(S[1])), (float)up);
+                int4 tops = {0, 0, 0, 0};
+                if constexpr (!HL) tops = *(const int4*)(tile_top + (it & 1) * 8 + 4 * par);
+                follow_max(fmaxf(block_max(S[0]), block_max(S[1])), (float)max(max(tops.x, tops.y), max(tops.z, tops.w)));
                 if constexpr (HL) {
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt) exact_values(it, kt, S[kt]);
                 } else {
-                    codes_values(it, S);
+                    codes_values(it, S, tops);
                 }
             }
             add_odd_values(it);
         }
         if (it + 1 < it1) staged(it + 1);
+    }
+
+    if constexpr (WEIGHED) {  // the sums relative to m again
+        const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(mv - m);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) O[dt] *= f;
     }
 
     // The halves' states join: waves 4 .. 7 hand theirs to waves 0 .. 3.

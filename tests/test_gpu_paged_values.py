@@ -152,3 +152,54 @@ def test_large_values_leave_rows_exact_that_do_not_see_them(m, where):
     q = (4 + 0.1 * rng.standard_normal((m, 4, D))).astype(np.float32)
     got = run_attention(pool, q, (m,), (kv,), table, paged.F32)
     of_sequences(pool, q, (m,), (kv,), table, got)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m", [1, 40])
+@pytest.mark.parametrize("size,weight", [(1e-2, 12), (1e-4, 17), (1e-4, 20), (3e-5, 17), (3e-5, 20)])
+def test_small_values_behind_a_slot_that_takes_the_weight(fmt, type_, m, size, weight):
+    """A first slot of value zero has nearly all of every softmax; what the 2^-12 to 2^-20 weights of the others
+    give has its own size's accuracy, also where V is small."""
+    rng = np.random.default_rng(54)
+    kv, page = 2000, 64
+    pool, table = filled(fmt, 2, page, (kv,), rng)
+    first = table[0, 0], slice(None), 0
+    if pool.q8:
+        pool.scales[0][:] = np.where(np.isnan(pool.scales[0]), np.nan, 1e-3)
+        pool.scales[1][:] = np.where(np.isnan(pool.scales[1]), np.nan, size * rng.uniform(0.6, 1, pool.scales[1].shape))
+        pool.data[0][first], pool.scales[0][first], pool.scales[1][first] = 127, weight * np.log(2) / (4 * 127 * D ** 0.5), 0
+    else:
+        pool.data[0][:] = pool.data[0] * np.float16(0.1)
+        pool.data[1][:] = pool.data[1] * np.float16(size * 60)
+        pool.data[0][first], pool.data[1][first] = weight * np.log(2) / (4 * D ** 0.5), 0
+    q = (4 + 0.1 * rng.standard_normal((m, 4, D))).astype(NP[type_])
+    got = run_attention(pool, q, (m,), (kv,), table, type_)
+    # fp16 outputs below 2^-14 step by 2^-24: half a step, spread evenly.
+    of_sequences(pool, q, (m,), (kv,), table, got, floor=2.0 ** -25 if type_ == paged.F16 else 0.0, type_=type_)
+
+
+@pytest.mark.parametrize("size", [516.0, -516.0, 3000.0, 65504.0])
+def test_q8_values_beyond_fp16_in_chunks_of_fp16_queries(size):
+    q8_values_beyond_fp16(paged.F16, 40, size)
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_values_of_all_sizes_along_a_sequence(order):
+    """fp16 queries, a prompt over q8 values whose size changes by factors of up to 2^13 from 64 slots to the next,
+    and among the 16-slot tiles of one: rows are as exact as their outputs' size asks."""
+    rng = np.random.default_rng(58)
+    kv, m = 640, 600
+    pool, table = filled(WeightFormat.Q8, 1, 64, (kv,), rng)
+    p = np.arange(kv)
+    size = {"rising": 2.0 ** (p // 64 * 1.4 - 13), "falling": 2.0 ** (1 - p // 64 * 1.4), "mixed": 2.0 ** -(p // 16 * 5 % 12)}[order]
+    w = pool.where(pool_slots(pool, table[0], kv))
+    pool.scales[1][w] = (size[:, None, None] * rng.uniform(0.6, 1, (kv, 1, 4))).astype(np.float16)
+    q = (0.5 * rng.standard_normal((m, 2, D))).astype(np.float16)
+    got = run_attention(pool, q, (m,), (kv,), table, paged.F16)
+    of_sequences(pool, q, (m,), (kv,), table, got, floor=2.0 ** -25, type_=paged.F16)
+
+
+def pool_slots(pool, row, n):
+    p = np.arange(n)
+    return row[p // pool.page].astype(np.int64) * pool.page + p % pool.page
