@@ -250,7 +250,8 @@ typedef struct {
  * (k_qk_norm_rope, Shaders.swift:871-923): y = x / sqrt(mean(x^2) + eps) * norm for each query and key
  * head (norm NULL: y = x), then the rotation of the first rot_dim values by the table row of the
  * token's position, pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`.  Queries go to q,
- * keys and values to the pool: rounded to fp16, or quantised with the bytes that icua_quantize gives.
+ * keys and values to the pool: rounded to fp16, or quantised with the bytes that icua_quantize gives (a group
+ * of 32 with an infinity or NaN: a scale that is no number, and nothing else of the row).
  * Arithmetic is fp32.  In an f16 pool keys and values are at most 65504 in magnitude, the largest fp16 (larger
  * ones become infinities).  A q8 pool holds groups of up to 127 * 65504; code times scale may be half a step
  * above the value (65532 for 65504), which fp32 outputs hold and fp16 ones round to an infinity.

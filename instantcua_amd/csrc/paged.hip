@@ -40,14 +40,17 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
 }
 
 // q8 code and scale of four values of a group held by 8 consecutive lanes, with the float32 steps of
-// the converter's quantiser (Convert.swift:215-241), so a stored row has the bytes that quantising
-// the float32 row as a matrix gives.
+// the converter's quantiser (Convert.swift:215-241), so a stored row of numbers has the bytes that
+// quantising the float32 row as a matrix gives.  The maximum is taken of magnitudes as integers, in which
+// NaN is the largest: a group with one gets a scale that is none (as floats the maximum passes it over, and
+// its code would stand for the group's largest value).
 __device__ __forceinline__ uint32_t q8_codes(f32x4 v, uint16_t& scale) {
 #pragma clang fp contract(off)
-    float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    amax = fmaxf(amax, dpp<DPP_XOR1>(amax));
-    amax = fmaxf(amax, dpp<DPP_XOR2>(amax));
-    amax = fmaxf(amax, dpp<DPP_HALF_MIRROR>(amax));
+    auto larger = [](float a, float b) { return as_f32(max(as_u32(a), as_u32(b))); };  // of magnitudes
+    float amax = larger(larger(fabsf(v[0]), fabsf(v[1])), larger(fabsf(v[2]), fabsf(v[3])));
+    amax = larger(amax, dpp<DPP_XOR1>(amax));
+    amax = larger(amax, dpp<DPP_XOR2>(amax));
+    amax = larger(amax, dpp<DPP_HALF_MIRROR>(amax));
     uint16_t sh = f2h(amax / 127.0f);
     if (h2f(sh) * 127.0f < amax) sh = (uint16_t)(sh + 1u);
     scale = sh;

@@ -200,6 +200,30 @@ def test_values_of_all_sizes_along_a_sequence(order):
     of_sequences(pool, q, (m,), (kv,), table, got, floor=2.0 ** -25, type_=paged.F16)
 
 
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_stored_rows_that_are_no_numbers_stay_so(fmt, what):
+    """A key or value that is no number is none in the pool either: the value itself (f16), its group (q8)."""
+    rng = np.random.default_rng(55)
+    pool = ref.Pool(fmt, 2, 16, 1)
+    cache = upload(pool)
+    x = rng.standard_normal((5, 4, D)).astype(np.float32)
+    x[1, 0, 40], x[3, 3, 127] = what, what
+    slots = np.arange(5, dtype=np.int32)
+    cache.store(dev(x), 5, dev(slots))
+    k, v = (dev(np.zeros((5, 2, D), np.float32)) for _ in range(2))
+    cache.load(dev(slots), 5, k, v)
+    got = np.concatenate([b.to_array(np.float32, (5, 2, D)) for b in (k, v)], 1)  # [token][k heads, v heads]
+    width = 32 if pool.q8 else 1
+    spoiled = np.zeros(got.shape, bool)
+    spoiled[1, 0, 40 // width * width:40 // width * width + width] = True
+    spoiled[3, 3, 127 // width * width:128] = True
+    assert not np.isfinite(got[spoiled]).any()
+    off = np.abs(np.where(spoiled, 0, got) - np.where(spoiled, 0, x))
+    assert np.abs(x[~spoiled]).max() < 4.5  # q8: half a step of a scale that is one fp16 step above 4.5 / 127 at most
+    assert (off <= np.where(spoiled, 0, np.abs(x)) * 2.0 ** -11 + (4.5 / 254 * (1 + 2.0 ** -9) if pool.q8 else 0))[~spoiled].all()
+
+
 def pool_slots(pool, row, n):
     p = np.arange(n)
     return row[p // pool.page].astype(np.int64) * pool.page + p % pool.page
