@@ -284,9 +284,10 @@ int icua_paged_store(const icua_pages_t* pages, const icua_paged_store_t* args, 
  * fp32 queries are computed to fp32 accuracy (fp16 hi + lo operands), fp16 ones with fp16 operands;
  * scores, softmax and sums are fp32.  max_q and max_kv bound the sequences' new tokens and slots (0:
  * n_tokens, table_width * page_slots) and decide the launch with n_seqs and n_tokens; slots past
- * max_kv are not read, and a sequence of more than max_q tokens has no defined output.  At most 2^21
- * (sequence, KV head) pairs, 2^26 (token, head) rows and n_seqs * max_kv of 2^36.  Slots of a page number outside
- * the pool take no part.  `work` holds icua_paged_attention_work() bytes, written and read within the
+ * max_kv are not read, and a sequence of more than max_q tokens has no defined output.  At most 2^14
+ * sequences (every workgroup looks through them, so that a larger batch is faster in parts), 2^21 (sequence, KV
+ * head) pairs, 2^26 (token, head) rows and n_seqs * max_kv of 2^36.  Slots of a page number outside the pool
+ * take no part.  `work` holds icua_paged_attention_work() bytes, written and read within the
  * call: calls that may run at the same time (other streams, captured graphs) each have their own. */
 typedef struct {
     int32_t type;            /* ICUA_TYPE_* of q and out */

@@ -1804,6 +1804,9 @@ static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention
     a.max_kv = args->max_kv ? std::min(args->max_kv, slots) : slots;
     if ((int64_t)a.n_seqs * ((a.max_kv + 127) / 128) > (1 << 29))
         return fail("paged_attention: more than 2^36 slots in all");
+    // Workgroups look through the sequences before theirs: 49 ms at this many of 9 tokens and 8 KV heads, and with
+    // their square from there.
+    if (a.n_seqs > 1 << 14) return fail("paged_attention: more than 2^14 sequences in a call");
     const int max_q = args->max_q ? std::min(args->max_q, args->n_tokens) : args->n_tokens;
     plan = paged_plan(pages->fmt, a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv);
     return 0;

@@ -1,4 +1,4 @@
-"""GPU tests of the operators on paged K/V caches where the values are unusual.  Definitions in paged_ref.py."""
+"""GPU tests of the operators on paged K/V caches where values or batches are unusual.  Definitions in paged_ref.py."""
 import os
 import sys
 
@@ -222,6 +222,19 @@ def test_stored_rows_that_are_no_numbers_stay_so(fmt, what):
     off = np.abs(np.where(spoiled, 0, got) - np.where(spoiled, 0, x))
     assert np.abs(x[~spoiled]).max() < 4.5  # q8: half a step of a scale that is one fp16 step above 4.5 / 127 at most
     assert (off <= np.where(spoiled, 0, np.abs(x)) * 2.0 ** -11 + (4.5 / 254 * (1 + 2.0 ** -9) if pool.q8 else 0))[~spoiled].all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_chunks_among_hundreds_of_sequences(fmt):
+    """Chunks are found behind runs of more than 64 sequences that have none, many of them of one length."""
+    rng = np.random.default_rng(38)
+    q_lens = [1] * 70 + [20] * 90 + [2] * 130 + [0] * 20 + [30, 1, 80]
+    kv_lens = [int(x) for x in rng.integers(1, 40, 70)] + [33] * 90 + [int(x) for x in rng.integers(2, 50, 150)] + [30, 200, 100]
+    pool, table = filled(fmt, 2, 16, kv_lens, rng)
+    q = rng.standard_normal((sum(q_lens), 2, D)).astype(np.float32)
+    got = run_attention(pool, q, q_lens, kv_lens, table, paged.F32)
+    want, reach, vmax = ref.attention(pool, q, q_lens, kv_lens, table)
+    assert np.abs(got - want).max() <= ref.attention_tol(False, pool.q8, reach, vmax)
 
 
 def pool_slots(pool, row, n):
