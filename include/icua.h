@@ -311,7 +311,8 @@ int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attent
 
 /* Reads rows of the pool back: for row r, KV head g the 128 values at pool slot slots[r], as fp32 (the
  * exact scale * code of q8) or fp16 (rounded), to k and v (either NULL) + r * token_stride + g *
- * head_stride (both 0: [n_rows][n_kv][128]).  Rows whose slot is outside the pool keep their outputs. */
+ * head_stride (both 0: [n_rows][n_kv][128]; else a token's heads lie within token_stride or a head's rows
+ * within head_stride).  Rows whose slot is outside the pool keep their outputs. */
 typedef struct {
     int32_t type;            /* ICUA_TYPE_* of k and v */
     int32_t n_rows;

@@ -1877,6 +1877,8 @@ int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, vo
     }
     if (a.token_stride < HD || a.head_stride < HD || a.token_stride % 8 || a.head_stride % 8)
         return fail("paged_load: strides must be at least 128 and multiples of 8 values");
+    if (a.token_stride < (__int128)(a.map.n_kv - 1) * a.head_stride + HD && a.head_stride < (__int128)(args->n_rows - 1) * a.token_stride + HD)
+        return fail("paged_load: strides let rows overlap: a token's heads must lie within token_stride, or a head's rows within head_stride");
     if (args->n_rows == 0 || (!args->k && !args->v)) return 0;
     if ((args->k && !buffer_ok(args->k)) || (args->v && !buffer_ok(args->v)))
         return fail("paged_load: k and v must be aligned to 16 bytes");
