@@ -98,7 +98,9 @@ class PagedCache:
 
     def attention_work(self, n_heads: int, n_seqs: int, n_tokens: int, table_width: Optional[int] = None,
                        max_q: int = 0, max_kv: int = 0) -> int:
-        """Bytes of workspace for an attention call of these sizes."""
+        """Bytes of workspace for an attention call of exactly these sizes; without ``table_width`` the table is
+        taken to be as wide as ``max_kv`` slots need, or one page if that is 0 too (a call without a bound on
+        slots over wider tables has to say their width here)."""
         if table_width is None:
             table_width = max(1, -(-max_kv // self.page_slots))
         a = _Attention(0, n_heads, n_seqs, n_tokens, max_q, max_kv, 0.0, table_width=table_width)
