@@ -237,6 +237,35 @@ def test_chunks_among_hundreds_of_sequences(fmt):
     assert np.abs(got - want).max() <= ref.attention_tol(False, pool.q8, reach, vmax)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m", [1, 7, 40, 130])
+@pytest.mark.parametrize("spread", [0.05, 1.0, 4.0])
+def test_attention_error_in_root_mean_square(fmt, type_, m, spread):
+    """Scores of this rms; single tokens, drafts and chunks, every row by itself and all together."""
+    rng = np.random.default_rng(56)
+    q_lens, kv_lens = (m, 1, m), (601, 333, 200)
+    pool, table = filled(fmt, 2, 16, kv_lens, rng)
+    q = rng.standard_normal((2 * m + 1, 4, D))
+    size = np.sqrt(np.mean([np.mean(pool.values(0, pool_slots(pool, t, n)) ** 2) for t, n in zip(table, kv_lens)]))
+    q = (q * spread / size).astype(NP[type_])
+    got = run_attention(pool, q, q_lens, kv_lens, table, type_)
+    of_sequences(pool, q, q_lens, kv_lens, table, got, type_=type_)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m", [1, 20])
+def test_attention_error_over_a_long_sequence(fmt, type_, m):
+    """The same where many workgroups share the slots and their partials are joined."""
+    rng = np.random.default_rng(59)
+    kv = 9001
+    pool, table = filled(fmt, 1, 64, (kv,), rng)
+    q = (rng.standard_normal((m, 2, D)) / np.sqrt(np.mean(pool.values(0, pool_slots(pool, table[0], kv)) ** 2))).astype(NP[type_])
+    got = run_attention(pool, q, (m,), (kv,), table, type_)
+    of_sequences(pool, q, (m,), (kv,), table, got, type_=type_)
+
+
 def pool_slots(pool, row, n):
     p = np.arange(n)
     return row[p // pool.page].astype(np.int64) * pool.page + p % pool.page
