@@ -83,7 +83,7 @@ __device__ __forceinline__ f32x4 rotate4(f32x4 x, f32x4 o, int d, int rot, bool 
 
 // 16 lanes a (token, head) vector, 16 vectors a workgroup.  Bound by memory: a token's row is read once
 // and its queries, keys and values written once.  4096 tokens of 16 + 8 + 8 heads, fp32 in, fp16 out: 101 MB in
-// 23.4 us, 4.3 TB/s, four fifths of what a copy reaches; eight tokens: 3.5 us, a launch.
+// 24 us, 4.2 TB/s, four fifths of what a copy reaches; eight tokens: 3.4 us, a launch.
 template <int TYPE, int QTYPE, int FMT>
 __global__ __launch_bounds__(256) void paged_store_kernel(PagedStoreArgs a) {
     const int nvec = a.n_heads + 2 * a.map.n_kv;
@@ -203,7 +203,8 @@ __global__ __launch_bounds__(256) void paged_load_kernel(PagedLoadArgs a) {
 //
 // fp32 queries and probabilities are split into fp16 hi + lo parts, two products each; queries are
 // first scaled by a power of two that puts the row's largest value in [2^9, 2^10), so that neither
-// part leaves fp16's range.
+// part leaves fp16's range.  The parts of a probability have 22 bits from 2^-12 of the row's largest on, and
+// 2^-34 of the largest below that.
 
 constexpr float P_SHIFT = 9.0f, P_SLACK = 6.0f;
 
@@ -472,8 +473,9 @@ __device__ __forceinline__ int few_per(const PagedAttnArgs& a, int total) {
 // with a step in flight each; three or four without one are no faster, and a step ahead with three does not fit
 // the registers.  A step's latency is 2.4 us from memory, the queries' and tables' before it some 2 us, so a
 // single token over 4096 slots is bound by latency: 9 us, and 4 to join.  Long caches are bound by memory: eight
-// tokens over up to 32768 fp16 slots 115 us, 5.4 TB/s; 64 tokens over up to 8192 q8 slots 111 us, 4.5 TB/s (a q8
-// step is some 450 instructions, 2.7 us of a wave).
+// tokens over up to 32768 fp16 slots 115 us, 5.4 TB/s; 64 tokens over up to 8192 q8 slots 105 us, 4.7 TB/s (a q8
+// step is some 450 instructions, 2.7 us of a wave), 113 with fp32 queries.  Those spill 15 registers (fp16 slots)
+// and 5 (q8), fp16 queries none.
 template <int TYPE, int FMT, int NW>
 __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uint8_t* lds) {
     // fp32 probabilities in two parts.  With fp16 queries and q8, two parts of V cost as much as two of the
@@ -697,33 +699,33 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
         const int at = threadIdx.x * DIMS, d0 = at % HD, orow = at / HD;
         const RowOf out = row_of(sp, orow, group, g);
         if (out.t >= 0 && (whole || orow < a.few.rows)) {
-        float mt = NEG_INF, lt = 0.f;
-        float2 ml[NW];
+            float mt = NEG_INF, lt = 0.f;
+            float2 ml[NW];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            ml[w] = sml[w * 16 + orow];
-            mt = fmaxf(mt, ml[w].x);
-        }
-        float x[DIMS] = {};
-        const float* src = (const float*)so + (d0 % 8) * ROWS_PITCH * 4 + (d0 / 32) * 80 + orow * 4 + d0 / 8 % 4;
+            for (int w = 0; w < NW; ++w) {
+                ml[w] = sml[w * 16 + orow];
+                mt = fmaxf(mt, ml[w].x);
+            }
+            float x[DIMS] = {};
+            const float* src = (const float*)so + (d0 % 8) * ROWS_PITCH * 4 + (d0 / 32) * 80 + orow * 4 + d0 / 8 % 4;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = ml[w].x == mt ? 1.f : __builtin_amdgcn_exp2f(ml[w].x - mt);
-            lt += ml[w].y * f;
+            for (int w = 0; w < NW; ++w) {
+                const float f = ml[w].x == mt ? 1.f : __builtin_amdgcn_exp2f(ml[w].x - mt);
+                lt += ml[w].y * f;
 #pragma unroll
-            for (int k = 0; k < DIMS; ++k) x[k] += src[(w * 8 + k) * ROWS_PITCH * 4] * f;
-        }
-        const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
-        const int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
+                for (int k = 0; k < DIMS; ++k) x[k] += src[(w * 8 + k) * ROWS_PITCH * 4] * f;
+            }
+            const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+            const int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
 #pragma unroll
-        for (int k = 0; k < DIMS; k += 4) {
-            const f32x4 y = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]} * inv;
-            if (!whole)
-                *(f32x4*)(a.few_part + part * HD + d0 + k) = y;
-            else
-                store4<TYPE>(a.out, (int64_t)out.t * a.out_stride + out.head * HD + d0 + k, y);
-        }
-        if (!whole && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
+            for (int k = 0; k < DIMS; k += 4) {
+                const f32x4 y = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]} * inv;
+                if (!whole)
+                    *(f32x4*)(a.few_part + part * HD + d0 + k) = y;
+                else
+                    store4<TYPE>(a.out, (int64_t)out.t * a.out_stride + out.head * HD + d0 + k, y);
+            }
+            if (!whole && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
         }
     }
 }
@@ -743,7 +745,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // K and V are staged in LDS, two stages of 128 slots, by copies that run under the products: fp16 from memory
 // to LDS directly; q8 through registers, as the exact codes in fp16, whose scales go to the groups' sums in fp32
 // and to the probabilities.  (Dequantised K, rounded to fp16, doubles the error of a batch of prompts, 4.8e-4
-// for 2.9e-4; it takes 107 us where this takes 138.)
+// for 2.9e-4; it took 107 us where this took 138, both in their first calls.)
 //
 // A staged row is 16 chunks of 16 bytes, chunk c at place c ^ swizzle(row): the operand reads of K (16 rows
 // at one chunk) and of V (4 rows at four chunks) then spread over all banks.  With only the low three bits
@@ -753,7 +755,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // exponentials, 64 products of 32 cycles), 200 scalar ones and 100 of LDS, in some 4300 cycles; products fill 38 %
 // of them, vector instructions 41 %, LDS 20 %.  Wave priorities and a start of half the waves apart change nothing.
 // A workgroup's first K and V are there 5 us after it starts, and 3 us join and write its rows.  A prompt of 4096
-// tokens, 16 heads: 95 us, 0.73 PFLOP/s of the causal half.
+// tokens, 16 heads, fp16 queries: 87 us, 0.79 PFLOP/s of the causal half; q8 142 us.  With fp32 queries, twice the
+// products (f16 pool) and also a split of each group's products (q8): 138 and 303 us; they spill 17 and 15 registers.
+//
+// q8, 12 sessions of chunks and single tokens, 126 us: vector instructions fill 51 % of the SIMDs' cycles, LDS 49 %
+// of the CUs' (a third of that conflicts: the staged codes of four rows share a quarter of the places), products 18 %.
 constexpr int CH_ROWS = 128, CH_HALF = 64;
 constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
 constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
@@ -1073,18 +1079,22 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         return mb;
     };
     // The maximum that is subtracted follows the true one when that is more than 2^P_SLACK ahead.  q8 with fp16
-    // queries: the values' sums have a maximum of their own, of scores plus the power of two e that V's scales of
-    // their half are below, and both are whole numbers.
+    // queries: the values' sums have a maximum of their own, m + mv, of scores plus the power of two e that V's
+    // scales of their half are below.  mv is a whole number; m is not, so that the probability of the largest
+    // score is a power of two and its products with scales are exact (2.9e-4 of error, 3.3e-4 with a whole m).
     constexpr bool WEIGHED = CODES && !HL;
-    float mv = NEG_INF;
+    float mv = 0.f;
     auto follow_max = [&](float mb, float e) __attribute__((always_inline)) {
         mb = max_x2(mb) * qc;
         if constexpr (WEIGHED) {
-            if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK || mb + e > mv + P_SLACK)) {
+            if (__builtin_amdgcn_ballot_w64(mb > m + P_SLACK || mb + e > m + mv + P_SLACK)) {
                 asm volatile("");
-                const float top = __builtin_ceilf(mb), m_new = fmaxf(m, top), mv_new = fmaxf(mv, top + e);
-                const float corr = mv_new == mv ? 1.f : __builtin_amdgcn_exp2f(mv - mv_new);
-                l *= m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+                const float m_new = fmaxf(m, mb);
+                // (2^-7: what rounding adds to a whole number does not make it the next.)
+                const float mv_new = m_new == NEG_INF ? 0.f : __builtin_ceilf(fmaxf(m + mv, mb + e) - m_new - 0.0078125f);
+                const float down = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+                const float corr = m == NEG_INF ? 0.f : down * __builtin_amdgcn_exp2f(mv - mv_new);
+                l *= down;
                 m = m_new;
                 mv = mv_new;
 #pragma unroll
@@ -1182,7 +1192,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
         scale_scores(it, 1, NG - 1, y[1], S[1]);
     };
-    // Values, fp16 queries.  A probability p, of 2^P_SHIFT at a score of m, becomes p 2^(m - mv + e) for the sums,
+    // Values, fp16 queries.  A probability p, of 2^P_SHIFT at a score of m, becomes p 2^(e - mv) for the sums,
     // e <= 0 the power of two that its 16 slots' scales were raised by: so p and its products with scales are both
     // rounded where they have all of fp16's bits, whatever the size of V's values (up to 2^14 apart among 64
     // slots), and the products end below 2^15.
@@ -1198,11 +1208,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int e = 0; e < 8; ++e)
                 p[c % 2][e / 2][e % 2] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(S[c / 2][8 * (c % 2) + e], qc, -sub_m));
         };
-        // 2^(m - mv + e): at most 2^14, as mv follows wherever m does.
-        const float lead = m == NEG_INF ? 0.f : m - mv;
+        // 2^(e - mv): at most 2^14, as mv is -14 or more.
         auto factor = [&](int c) __attribute__((always_inline)) {
             const int e = c == 0 ? tops.x : c == 1 ? tops.y : c == 2 ? tops.z : tops.w;
-            const f16 y = (f16)__builtin_amdgcn_exp2f(lead + (float)min(e, 0));
+            const f16 y = (f16)__builtin_amdgcn_exp2f((float)min(e, 0) - mv);
             return f16x2{y, y};
         };
         exponentials(0);
@@ -1233,7 +1242,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // products of the two, by the power of two that puts the largest in [2^14, 2^15), are split into fp16 hi + lo
     // parts, and the power goes to the sum: values that the row does not see, or gives little weight, take nothing
     // from its accuracy, however large.  (By the power of the largest scale instead, a value of 65504 at a later
-    // token left 1.2e-4 of error to rows of small values.)
+    // token left 4e-4 of error to rows of small values.)
     auto exact_values = [&](int it, int kt, const f32x16& S) __attribute__((always_inline)) {
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
         const uint32_t Vs = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
@@ -1350,7 +1359,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     if constexpr (WEIGHED) {  // the sums relative to m again
-        const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(mv - m);
+        const float f = __builtin_amdgcn_exp2f(mv);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) O[dt] *= f;
     }
@@ -1516,9 +1525,9 @@ static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv) {
 
 // Units of few-row sequences among `want` workgroups: no sequence in more than PAGED_MAX_SPLITS of them.
 //
-// 512 workgroups are what the registers let run at once.  fp16 steps are twice a q8 step's bytes, and half as
-// many workgroups read long caches faster: eight sequences of up to 32768 slots 115 us, 124 with 512; 64 q8
-// ones of up to 8192 108 us with 512, 141 with 256, 116 with 1024.
+// 512 workgroups are what the registers let run at once: 64 q8 sequences of up to 8192 slots take 110 us with 512,
+// 143 with 256, 127 with 768 and 116 with 1024.  fp16 steps are twice a q8 step's bytes, and half as many workgroups
+// read long caches faster: eight sequences of up to 32768 slots 121 us, 128 without the doubled shares.
 static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, int rows, int max_kv) {
     const int most = std::max(1, (max_kv + unit - 1) / unit);
     const int n = (int)std::min(std::max<int64_t>(1, want / n_kv), (int64_t)n_seqs * most);
