@@ -1419,8 +1419,9 @@ __device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int hea
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int i = i0 + 2 * k + (lane >> 5);
-            const float w = __shfl(f, i);  // 0 past the last; by all lanes, as an inactive one hands nothing over
-            if (w != 0.f) o += x[k] * w;
+            // 0 past the last; by all lanes, as an inactive one hands nothing over.  A partial without weight is added
+            // too: one that is no number (of a slot of V that the row sees) makes the output none.
+            o += x[k] * __shfl(f, i);
         }
     }
 #pragma unroll

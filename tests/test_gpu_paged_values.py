@@ -269,3 +269,29 @@ def test_attention_error_over_a_long_sequence(fmt, type_, m):
 def pool_slots(pool, row, n):
     p = np.arange(n)
     return row[p // pool.page].astype(np.int64) * pool.page + p % pool.page
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m", [1, 20])
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_values_that_are_no_numbers_where_workgroups_join(fmt, type_, m, what):
+    """A slot whose weight, e^-200, is nothing in fp32, in another workgroup's share than the slot that has it all:
+    the rows that see it give no number, as they do where one workgroup has both."""
+    rng = np.random.default_rng(60)
+    kv = 3000
+    pool, table = filled(fmt, 1, 64, (kv,), rng)
+    first, far = (table[0, 0], slice(None), 0), (table[0, 2500 // 64], slice(None), 2500 % 64)
+    if pool.q8:
+        pool.scales[0][:] = np.where(np.isnan(pool.scales[0]), np.nan, 1e-3)
+        pool.data[0][first], pool.scales[0][first] = 127, 200 / (4 * 127 * D ** 0.5)
+        pool.scales[1][far][..., 1] = what
+    else:
+        pool.data[0][:] = pool.data[0] * np.float16(0.1)
+        pool.data[0][first] = 200 / (4 * D ** 0.5)
+        pool.data[1][far][..., 37] = what
+    q = (4 + 0.1 * rng.standard_normal((m, 2, D))).astype(NP[type_])
+    got = run_attention(pool, q, (m,), (kv,), table, type_)
+    spoiled = np.zeros(D, bool)
+    spoiled[slice(32, 64) if pool.q8 else 37] = True
+    assert not np.isfinite(got[..., spoiled]).any() and np.isfinite(got[..., ~spoiled]).all()
