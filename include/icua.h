@@ -282,12 +282,14 @@ int icua_paged_store(const icua_pages_t* pages, const icua_paged_store_t* args, 
  * sees slots 0 .. kv_len - m + i, and a token that sees none gets zeros.  Query head h reads KV head
  * h * n_kv / n_heads.  Rows of q behind the last sequence's keep their outputs as they are.
  * fp32 queries are computed to fp32 accuracy (fp16 hi + lo operands; probabilities to 22 bits, or 2^-34 of
- * the row's largest), fp16 ones with fp16 operands; scores, softmax and sums are fp32.  max_q and max_kv bound the sequences' new tokens and slots (0:
- * n_tokens, table_width * page_slots) and decide the launch with n_seqs and n_tokens; slots past
- * max_kv are not read, and a sequence of more than max_q tokens has no defined output.  At most 2^14
- * sequences (every workgroup looks through them, so that a larger batch is faster in parts), 2^21 (sequence, KV
- * head) pairs, 2^26 (token, head) rows and n_seqs * max_kv of 2^36.  Slots of a page number outside the pool
- * take no part.  `work` holds icua_paged_attention_work() bytes, written and read within the
+ * the row's largest), fp16 ones with fp16 operands (over q8 V's scales should not differ by more than 2^14
+ * among 64 slots of a prompt: smaller values lose accuracy there); scores, softmax and sums are fp32.  max_q
+ * and max_kv bound the sequences' new tokens and slots (0: n_tokens, table_width * page_slots) and decide
+ * the launch with n_seqs and n_tokens; slots past max_kv are not read, and a sequence of more than max_q
+ * tokens has no defined output.  At most 2^14 sequences (every workgroup looks through them, so that a
+ * larger batch is faster in parts), 2^21 (sequence, KV head) pairs, 2^26 (token, head) rows and n_seqs *
+ * max_kv of 2^36.  Slots of a page number outside the pool take no part.  `work` holds
+ * icua_paged_attention_work() bytes, written and read within the
  * call: calls that may run at the same time (other streams, captured graphs) each have their own. */
 typedef struct {
     int32_t type;            /* ICUA_TYPE_* of q and out */
