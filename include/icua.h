@@ -219,6 +219,63 @@ int icua_quantize_noalloc(int fmt, const float* d_m, int rows, int cols, void* d
 int icua_quantize_bench(int fmt, const float* d_m, int rows, int cols, void* d_codes, void* d_sb, int iters,
                         double* avg_us);
 
+enum { ICUA_TYPE_F32 = 0, ICUA_TYPE_F16 = 1 };
+
+/* ---- products on 8-bit integers with a scale for each token and each output channel ----
+ * The matrix products of a batch of tokens (icua_gemv: up to 8 rows, scales for groups of weights): tokens are
+ * quantised to 8 bits as they come, matrices once (each output channel is a row of icua_i8_quantize, without a norm).
+ * The calls enqueue on `stream` (a hipStream_t; NULL: the null stream) and return without waiting; they allocate
+ * nothing, keep nothing and can be captured into a graph.  Buffers and stream belong to the current device.
+ * Arguments are checked before anything is enqueued.  Row strides are in values (0: dense); the buffers of one call
+ * do not overlap but where it is said. */
+
+/* Codes and scales of rows: y = x / sqrt(mean(x^2) + eps) * norm (norm NULL: y = x, eps is not used),
+ *   scale = max |y| / 127,  code = 127 y / max |y|, rounded to the nearest, ties to even:
+ * -127 .. 127, and exactly those of the definition (the arithmetic is 64-bit).  A row of zeros has codes and scale
+ * zero; a row with an infinity or NaN (in y) has codes zero and a scale that is no number.
+ * Scales beyond fp32's range become 0 or infinite. */
+typedef struct {
+    int32_t type;            /* ICUA_TYPE_* of x */
+    int32_t n_rows;          /* 0: nothing to do */
+    int32_t n_cols;          /* a positive multiple of 16, at most 2^17 */
+    const void* x;           /* [n_rows] rows, aligned to 16 bytes; x_stride a multiple of 8 */
+    int64_t x_stride;
+    const float* norm;       /* [n_cols] or NULL, aligned to 16 bytes */
+    float eps;
+    int8_t* codes;           /* [n_rows] rows, aligned to 16 bytes; codes_stride a multiple of 16 */
+    int64_t codes_stride;
+    float* scales;           /* [n_rows] */
+} icua_i8_quantize_t;
+int icua_i8_quantize(const icua_i8_quantize_t* args, void* stream);
+
+/* y[m][n] = x_scales[m] * w_scales[n] * sum_k x[m][k] w[n][k]  (+ add[m][n]),  or with `gated`, w's rows being n_out
+ * gates and then n_out ups (the fused gate|up rows of a feed-forward block), y = g / (1 + exp(-g)) * u of the two
+ * products g and u.  Sums are exact; scales, gate and addition are fp32, rounded once to y's type (beyond fp16's range:
+ * an infinity).  A row whose scale is no number becomes NaN.  `add` may be y itself, if that is fp32 with the same
+ * stride (a residual that is updated in place).  `work` holds icua_i8_matmul_work() bytes, written and read within the
+ * call: calls that may run at the same time (other streams, captured graphs) each have their own. */
+typedef struct {
+    int32_t type;            /* ICUA_TYPE_* of y */
+    int32_t gated;           /* 0 or 1; not together with add */
+    int32_t n_rows, n_out;   /* tokens and output channels (0: nothing to do), n_rows * n_out <= 2^36 */
+    int32_t n_in;            /* a positive multiple of 16, at most 2^17 */
+    const int8_t* x;         /* [n_rows] rows of codes, -127 .. 127, aligned to 16 bytes; x_stride a multiple of 16 */
+    int64_t x_stride;
+    const float* x_scales;   /* [n_rows] */
+    const int8_t* w;         /* [n_out] rows ([2 n_out]), as x */
+    int64_t w_stride;
+    const float* w_scales;   /* [n_out] ([2 n_out]) */
+    const float* add;        /* [n_rows] rows of n_out, or NULL */
+    int64_t add_stride;
+    void* y;                 /* [n_rows] rows of n_out, of any stride */
+    int64_t y_stride;
+    void* work;
+    size_t work_bytes;
+} icua_i8_matmul_t;
+int icua_i8_matmul(const icua_i8_matmul_t* args, void* stream);
+/* Bytes of `work` for a call with exactly these sizes (the pointers in args are not looked at). */
+int icua_i8_matmul_work(const icua_i8_matmul_t* args, size_t* bytes);
+
 /* ---- paged K/V caches: several sequences in one pool of pages, on device buffers ----
  * The reference has one contiguous cache of one session (kc/vc, Engine.swift:110-112); these operators
  * serve batches of sequences of any lengths, which may share pages (a common prompt prefix).
@@ -235,8 +292,6 @@ int icua_quantize_bench(int fmt, const float* d_m, int rows, int cols, void* d_c
  * be checked by the host: numbers that point outside the pool or the tables are never followed (what
  * happens to their rows is said at each call).  Row strides are in values and multiples of 8; value
  * buffers are aligned to 16 bytes. */
-enum { ICUA_TYPE_F32 = 0, ICUA_TYPE_F16 = 1 };
-
 typedef struct {
     int32_t fmt;             /* ICUA_FMT_F16 or ICUA_FMT_Q8 */
     int32_t n_kv;            /* KV heads, 1..1024 */

@@ -1727,12 +1727,12 @@ static int stride_check(const char* what, int64_t& stride, int64_t width) {
 static bool type_ok(int t) { return t == TYPE_F32 || t == TYPE_F16; }
 
 // Work goes to the current device: a stream of another one is refused.
-static int stream_check(void* stream) {
+static int stream_check(void* stream, const char* what = "paged") {
     int dev = 0, sdev = 0;
     if (!stream) return 0;
     HIPCK(hipGetDevice(&dev));
     HIPCK(hipStreamGetDevice((hipStream_t)stream, &sdev));
-    if (dev != sdev) return fail("paged: the stream belongs to another device than the current one");
+    if (dev != sdev) return fail(std::string(what) + ": the stream belongs to another device than the current one");
     return 0;
 }
 
@@ -1893,6 +1893,112 @@ int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, vo
     a.k_out = args->k;
     a.v_out = args->v;
     HIPCK(launch_paged_load(pages->fmt, args->type, a, (hipStream_t)stream));
+    return 0;
+}
+
+// ---- products on 8-bit integers
+
+constexpr int I8_MAX_IN = 1 << 17;  // sums of products of codes stay below 2^31
+
+// A row stride of `width` values (0: dense) in multiples of `of`.
+static int i8_stride(const std::string& what, int64_t& stride, int64_t width, int of) {
+    if (stride == 0) stride = width;
+    if (stride < width || stride % of) return fail(what + " must be at least a row" + (of > 1 ? " and a multiple of " + std::to_string(of) + " values" : ""));
+    return 0;
+}
+// Whether [p, p + bytes) and [q, q + more) overlap.
+static bool overlap(const void* p, __int128 bytes, const void* q, __int128 more) {
+    return p && q && bytes > 0 && more > 0 && (__int128)(uintptr_t)p < (__int128)(uintptr_t)q + more && (__int128)(uintptr_t)q < (__int128)(uintptr_t)p + bytes;
+}
+// Bytes from the first value of `rows` rows to behind their last.
+static __int128 span(int64_t rows, int64_t stride, int64_t width, int size) { return rows > 0 ? ((__int128)(rows - 1) * stride + width) * size : 0; }
+
+int icua_i8_quantize(const icua_i8_quantize_t* args, void* stream) {
+    if (!args) return fail("i8_quantize: null argument");
+    if (!type_ok(args->type)) return fail("i8_quantize: bad type");
+    if (args->n_rows < 0) return fail("i8_quantize: negative n_rows");
+    if (args->n_cols < 16 || args->n_cols % 16 || args->n_cols > I8_MAX_IN) return fail("i8_quantize: n_cols must be a positive multiple of 16, at most 2^17");
+    I8QuantArgs a{};
+    a.n_rows = args->n_rows;
+    a.n_cols = args->n_cols;
+    a.x_stride = args->x_stride;
+    a.codes_stride = args->codes_stride;
+    if (i8_stride("i8_quantize: x_stride", a.x_stride, a.n_cols, 8) || i8_stride("i8_quantize: codes_stride", a.codes_stride, a.n_cols, 16)) return -1;
+    if (args->norm && !(args->eps >= 0.f)) return fail("i8_quantize: eps must not be negative");
+    if (args->n_rows == 0) return 0;
+    if (!buffer_ok(args->x) || !buffer_ok(args->codes)) return fail("i8_quantize: x and codes must be set and aligned to 16 bytes");
+    if (args->norm && !buffer_ok(args->norm)) return fail("i8_quantize: norm must be aligned to 16 bytes");
+    if (!args->scales || (uintptr_t)args->scales % 4) return fail("i8_quantize: scales must be set and aligned to 4 bytes");
+    const __int128 codes = span(a.n_rows, a.codes_stride, a.n_cols, 1), scales = span(1, 0, a.n_rows, 4);
+    const __int128 x = span(a.n_rows, a.x_stride, a.n_cols, args->type == TYPE_F32 ? 4 : 2), norm = span(1, 0, a.n_cols, 4);
+    if (overlap(args->codes, codes, args->scales, scales) || overlap(args->codes, codes, args->x, x) || overlap(args->scales, scales, args->x, x) ||
+        overlap(args->codes, codes, args->norm, norm) || overlap(args->scales, scales, args->norm, norm))
+        return fail("i8_quantize: codes and scales must not overlap each other or the inputs");
+    if (stream_check(stream, "i8_quantize")) return -1;
+    a.x = args->x;
+    a.norm = args->norm;
+    a.eps = args->eps;
+    a.codes = args->codes;
+    a.scales = args->scales;
+    HIPCK(launch_i8_quantize(args->type, a, (hipStream_t)stream));
+    return 0;
+}
+
+// Sizes of a product: checked.
+static int i8_matmul_sizes(const icua_i8_matmul_t* args, I8MatmulArgs& a) {
+    if (!args) return fail("i8_matmul: null argument");
+    if (!type_ok(args->type)) return fail("i8_matmul: bad type");
+    if (args->gated != 0 && args->gated != 1) return fail("i8_matmul: gated must be 0 or 1");
+    if (args->n_rows < 0 || args->n_out < 0) return fail("i8_matmul: negative size");
+    if (args->n_out > (1 << 30) || (int64_t)args->n_rows * args->n_out > ((int64_t)1 << 36)) return fail("i8_matmul: more than 2^30 channels or 2^36 outputs");
+    if (args->n_in < 16 || args->n_in % 16 || args->n_in > I8_MAX_IN) return fail("i8_matmul: n_in must be a positive multiple of 16, at most 2^17");
+    a.n_rows = args->n_rows;
+    a.n_out = args->n_out;
+    a.n_in = args->n_in;
+    return 0;
+}
+
+int icua_i8_matmul_work(const icua_i8_matmul_t* args, size_t* bytes) {
+    I8MatmulArgs a{};
+    if (!bytes) return fail("i8_matmul_work: null argument");
+    if (i8_matmul_sizes(args, a)) return -1;
+    *bytes = 0;
+    return 0;
+}
+
+int icua_i8_matmul(const icua_i8_matmul_t* args, void* stream) {
+    I8MatmulArgs a{};
+    if (i8_matmul_sizes(args, a)) return -1;
+    a.x_stride = args->x_stride;
+    a.w_stride = args->w_stride;
+    a.add_stride = args->add_stride;
+    a.y_stride = args->y_stride;
+    if (i8_stride("i8_matmul: x_stride", a.x_stride, a.n_in, 16) || i8_stride("i8_matmul: w_stride", a.w_stride, a.n_in, 16) ||
+        i8_stride("i8_matmul: add_stride", a.add_stride, a.n_out, 1) || i8_stride("i8_matmul: y_stride", a.y_stride, a.n_out, 1))
+        return -1;
+    if (args->gated && args->add) return fail("i8_matmul: add is for products that are not gated");
+    if (a.n_rows == 0 || a.n_out == 0) return 0;
+    if (!buffer_ok(args->x) || !buffer_ok(args->w)) return fail("i8_matmul: x and w must be set and aligned to 16 bytes");
+    if (!args->x_scales || !args->w_scales || (uintptr_t)args->x_scales % 4 || (uintptr_t)args->w_scales % 4)
+        return fail("i8_matmul: x_scales and w_scales must be set and aligned to 4 bytes");
+    const int size = args->type == TYPE_F32 ? 4 : 2;
+    if (!args->y || (uintptr_t)args->y % size) return fail("i8_matmul: y must be set and aligned to its type");
+    if ((uintptr_t)args->add % 4) return fail("i8_matmul: add must be aligned to 4 bytes");
+    const __int128 y = span(a.n_rows, a.y_stride, a.n_out, size);
+    const int64_t channels = args->gated ? 2 * (int64_t)a.n_out : a.n_out;
+    const bool in_place = args->add == args->y && size == 4 && a.add_stride == a.y_stride;
+    if ((!in_place && overlap(args->y, y, args->add, span(a.n_rows, a.add_stride, a.n_out, 4))) || overlap(args->y, y, args->x, span(a.n_rows, a.x_stride, a.n_in, 1)) ||
+        overlap(args->y, y, args->w, span(channels, a.w_stride, a.n_in, 1)) || overlap(args->y, y, args->x_scales, span(1, 0, a.n_rows, 4)) ||
+        overlap(args->y, y, args->w_scales, span(1, 0, channels, 4)))
+        return fail("i8_matmul: y must not overlap an input, but for an fp32 y that is add, with its stride");
+    if (stream_check(stream, "i8_matmul")) return -1;
+    a.x = args->x;
+    a.x_scales = args->x_scales;
+    a.w = args->w;
+    a.w_scales = args->w_scales;
+    a.add = args->add;
+    a.y = args->y;
+    HIPCK(launch_i8_matmul(args->type, args->gated != 0, a, (hipStream_t)stream));
     return 0;
 }
 

@@ -113,6 +113,31 @@ __device__ __forceinline__ float sum_x4(float v) {
     return swap32_add(s, s);
 }
 
+// ------------------------------------------------------------------------------------------
+// Copies from memory to LDS that run under the products.
+
+// Each lane's 16 bytes from memory to LDS, lane l's to dst + 16 l (dst the same in all lanes).  As assembly
+// (it has no outputs): after the builtin the compiler waits for the copy before the next transposing read,
+// whatever stage that reads.
+__device__ __forceinline__ void copy_to_lds(const uint8_t* p, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(p) : "memory", "m0");
+}
+// The same from base + offset, base the same in all lanes.
+__device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory", "m0");
+}
+
+// This wave's LDS writes are done and of its copies and loads at most the last `pending` in flight (63: no
+// matter), then all waves meet.  The empty statements keep memory accesses on their side of the barrier.
+template <int pending>
+__device__ __forceinline__ void staged_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((pending & 15) | (7 << 4) | (0 << 8) | ((pending >> 4) << 14));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// ------------------------------------------------------------------------------------------
 // Per-head RMSNorm(128) + RoPE of one 128-vector by one wave: lane i owns the rotation pair
 // (i, i + 64).
 __device__ __forceinline__ void norm_rope_pair(float& a, float& b, const float* w, const float* cs, int lane) {

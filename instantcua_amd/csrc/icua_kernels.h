@@ -216,6 +216,34 @@ constexpr int64_t QUANT_SCRATCH_GROUPS = (int64_t)8 << 20;
 constexpr int QUANT_MAX_DEVICES = 64;
 hipError_t quant_scratch(uint8_t** out);
 
+// ---- Products on 8-bit integers (int8.hip); the arguments have been checked by the caller.
+struct I8QuantArgs {
+    int n_rows, n_cols;
+    const void* x;
+    int64_t x_stride;
+    const float* norm;              // [n_cols] or null
+    float eps;
+    int8_t* codes;
+    int64_t codes_stride;
+    float* scales;                  // [n_rows]
+};
+hipError_t launch_i8_quantize(int type, const I8QuantArgs& a, hipStream_t s);
+
+struct I8MatmulArgs {
+    int n_rows, n_out, n_in;
+    const int8_t* x;                // [n_rows] rows of n_in codes
+    int64_t x_stride;
+    const float* x_scales;          // [n_rows]
+    const int8_t* w;                // [n_out] rows of n_in codes (gated: [2 n_out], gate rows first)
+    int64_t w_stride;
+    const float* w_scales;
+    const float* add;               // [n_rows] rows of n_out, or null
+    int64_t add_stride;
+    void* y;
+    int64_t y_stride;
+};
+hipError_t launch_i8_matmul(int type, bool gated, const I8MatmulArgs& a, hipStream_t s);
+
 // ---- Operators on paged K/V caches (paged.hip); the arguments have been checked by the caller.
 struct PagedStoreArgs {
     PageMap map;

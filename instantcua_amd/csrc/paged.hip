@@ -776,27 +776,6 @@ __device__ __constant__ const u32x4 g_zeros = {0, 0, 0, 0};  // what slots that 
 __device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
 __device__ __forceinline__ f32x16 mfma32(v8h a, v8h b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// Each lane's 16 bytes from memory to LDS, lane l's to dst + 16 l (dst the same in all lanes).  As assembly
-// (it has no outputs): after the builtin the compiler waits for the copy before the next transposing read,
-// whatever stage that reads.
-__device__ __forceinline__ void copy_to_lds(const uint8_t* p, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(p) : "memory", "m0");
-}
-// The same from base + offset, base the same in all lanes.
-__device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory", "m0");
-}
-
-// This wave's LDS writes are done and of its copies and loads at most the last `pending` in flight (63: no
-// matter), then all waves meet.  The empty statements keep memory accesses on their side of the barrier.
-template <int pending>
-__device__ __forceinline__ void staged_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((pending & 15) | (7 << 4) | (0 << 8) | ((pending >> 4) << 14));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // The sequence and tile (of `rows` query rows a KV head) that number `index` stands for, over the
 // sequences with more than ROWS_TILE rows; false past the last one.  A wave looks at 64 sequences at a time,
 // and takes those with the most slots first, so that the last workgroups to run are short.  Every workgroup
