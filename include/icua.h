@@ -366,6 +366,32 @@ int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t
 /* Bytes of `work` for a call with exactly these sizes (the pointers in args are not looked at). */
 int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, size_t* bytes);
 
+/* The same for a window: a token at slot p of its sequence (kv_len - m + i for token i of m) sees slot j <= p if p - j <
+ * window or j < sinks: its own and the window - 1 slots before it, and the sequence's first ones.  The slots between are
+ * not read, whatever they hold, and their pages may be given back (table entries of any value; a page that is gone takes
+ * part in nothing).  A window of max_kv or more is icua_paged_attention. */
+typedef struct {
+    int32_t window;          /* at least 1 */
+    int32_t sinks;           /* at least 0 */
+} icua_paged_window_t;
+int icua_paged_attention_window(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_window_t* window, void* stream);
+int icua_paged_attention_window_work(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_window_t* window, size_t* bytes);
+
+/* The same as icua_paged_attention for sequences that share their first slots: sequences group_start[g] ..
+ * group_start[g + 1] - 1 have the same K/V in slots 0 .. prefix_len[g] - 1 (the same pages, as a rule), which are read
+ * once for all of the group's tokens, through the table of its first sequence; kv_len and tables still count and hold
+ * the shared slots of every sequence.  Sequences before the first group and behind the last one share nothing.  What a
+ * token sees does not change: one that does not see all of the prefix (a sequence shorter than it, say) sees its part.
+ * Slots are shared 128 at a time: up to 127 at the prefix's end are read by each sequence. */
+typedef struct {
+    int32_t n_groups;        /* 0..64 */
+    int32_t max_prefix;      /* bound of prefix_len (0: max_kv); of a longer one max_prefix slots are shared */
+    const int32_t* group_start; /* [n_groups + 1] sequence numbers, rising */
+    const int32_t* prefix_len;  /* [n_groups] */
+} icua_paged_prefix_t;
+int icua_paged_attention_prefix(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_prefix_t* prefix, void* stream);
+int icua_paged_attention_prefix_work(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_prefix_t* prefix, size_t* bytes);
+
 /* Reads rows of the pool back: for row r, KV head g the 128 values at pool slot slots[r], as fp32 (the
  * exact scale * code of q8) or fp16 (rounded), to k and v (either NULL) + r * token_stride + g *
  * head_stride (both 0: [n_rows][n_kv][128]; else a token's heads lie within token_stride or a head's rows

@@ -1783,7 +1783,7 @@ int icua_paged_store(const icua_pages_t* pages, const icua_paged_store_t* args, 
 }
 
 // Sizes of an attention call: checked, with the defaults filled in.
-static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention_t* args, bool buffers, PagedAttnArgs& a,
+static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention_t* args, bool buffers, PagedFormSizes f, PagedAttnArgs& a,
                            PagedPlan& plan) {
     if (!args) return fail("paged_attention: null argument");
     if (pages_check(pages, a.map, buffers)) return -1;
@@ -1808,24 +1808,36 @@ static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention
     // their square from there.
     if (a.n_seqs > 1 << 14) return fail("paged_attention: more than 2^14 sequences in a call");
     const int max_q = args->max_q ? std::min(args->max_q, args->n_tokens) : args->n_tokens;
-    plan = paged_plan(pages->fmt, a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv);
+    if (f.form == PAGED_WINDOW) {
+        if (f.window < 1 || f.sinks < 0) return fail("paged_attention: a window is at least 1 slot, its first slots at least 0");
+        f.window = std::min(f.window, std::max(1, a.max_kv));  // as much as there is
+        f.sinks = std::min(f.sinks, a.max_kv);
+    }
+    if (f.form == PAGED_PREFIX) {
+        if (f.n_groups < 0 || f.n_groups > PREFIX_GROUPS) return fail("paged_attention: n_groups must be in 0..64");
+        if (f.max_prefix < 0) return fail("paged_attention: negative size");
+        f.max_prefix = f.max_prefix ? std::min(f.max_prefix, a.max_kv) : a.max_kv;
+        if (f.n_groups == 0 || f.max_prefix < PREFIX_STEP) f.form = PAGED_ALL;  // nothing is shared
+    }
+    a.f = f;
+    plan = paged_plan(pages->fmt, a.n_heads, a.map.n_kv, a.n_seqs, a.n_tokens, max_q, a.max_kv, f);
     return 0;
 }
-static size_t plan_bytes(const PagedPlan& p) { return (p.few_rows + p.part_rows) * (HD + 2) * sizeof(float); }
+static size_t plan_bytes(const PagedPlan& p) { return (p.few_rows + p.part_rows + p.pre_rows) * (HD + 2) * sizeof(float); }
 
-int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, size_t* bytes) {
+static int attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, const PagedFormSizes& f, size_t* bytes) {
     PagedAttnArgs a{};
     PagedPlan plan{};
     if (!bytes) return fail("paged_attention_work: null argument");
-    if (attention_sizes(pages, args, false, a, plan)) return -1;
+    if (attention_sizes(pages, args, false, f, a, plan)) return -1;
     *bytes = plan_bytes(plan);
     return 0;
 }
 
-int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t* args, void* stream) {
+static int attention_call(const icua_pages_t* pages, const icua_paged_attention_t* args, const PagedFormSizes& f, const icua_paged_prefix_t* prefix, void* stream) {
     PagedAttnArgs a{};
     PagedPlan plan{};
-    if (attention_sizes(pages, args, true, a, plan)) return -1;
+    if (attention_sizes(pages, args, true, f, a, plan)) return -1;
     a.q_stride = args->q_stride;
     a.out_stride = args->out_stride;
     if (stride_check("q_stride", a.q_stride, (int64_t)a.n_heads * HD)) return -1;
@@ -1834,6 +1846,7 @@ int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t
     if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
     if (!buffer_ok(args->q) || !buffer_ok(args->out)) return fail("paged_attention: q and out must be set and aligned to 16 bytes");
     if (!args->q_start || !args->kv_len || !args->tables) return fail("paged_attention: q_start, kv_len and tables must be set");
+    if (f.n_groups && (!prefix->group_start || !prefix->prefix_len)) return fail("paged_attention: group_start and prefix_len must be set");
     const size_t need = plan_bytes(plan);
     if (need && (!buffer_ok(args->work) || args->work_bytes < need))
         return fail("paged_attention: work must hold " + std::to_string(need) + " bytes, aligned to 16");
@@ -1851,15 +1864,48 @@ int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t
     a.few = plan.few;
     a.big = plan.big;
     a.tiles = plan.tiles;
+    a.pre = plan.pre;
+    a.pre_tiles = plan.pre_tiles;
+    a.part_at = (int64_t)plan.few_rows;
+    a.pre_at = (int64_t)(plan.few_rows + plan.part_rows);
     float* const few_part = (float*)args->work;
     float* const part = few_part + plan.few_rows * HD;
-    float2* const ml = (float2*)(part + plan.part_rows * HD);
-    a.few_part = plan.few_rows ? few_part : nullptr;
+    float2* const ml = (float2*)(part + (plan.part_rows + plan.pre_rows) * HD);
+    a.few_part = plan.few_rows || a.f.form == PAGED_PREFIX ? few_part : nullptr;
     a.few_ml = ml;
     a.part = plan.part_rows ? part : nullptr;
     a.part_ml = ml + plan.few_rows;
+    if (prefix) {
+        a.group_start = prefix->group_start;
+        a.prefix_len = prefix->prefix_len;
+    }
     HIPCK(launch_paged_attention(pages->fmt, args->type, a, (hipStream_t)stream));
     return 0;
+}
+
+int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attention_t* args, size_t* bytes) {
+    return attention_work(pages, args, {PAGED_ALL, 0, 0, 0, 0}, bytes);
+}
+int icua_paged_attention(const icua_pages_t* pages, const icua_paged_attention_t* args, void* stream) {
+    return attention_call(pages, args, {PAGED_ALL, 0, 0, 0, 0}, nullptr, stream);
+}
+
+int icua_paged_attention_window_work(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_window_t* window, size_t* bytes) {
+    if (!window) return fail("paged_attention: null argument");
+    return attention_work(pages, args, {PAGED_WINDOW, window->window, window->sinks, 0, 0}, bytes);
+}
+int icua_paged_attention_window(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_window_t* window, void* stream) {
+    if (!window) return fail("paged_attention: null argument");
+    return attention_call(pages, args, {PAGED_WINDOW, window->window, window->sinks, 0, 0}, nullptr, stream);
+}
+
+int icua_paged_attention_prefix_work(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_prefix_t* prefix, size_t* bytes) {
+    if (!prefix) return fail("paged_attention: null argument");
+    return attention_work(pages, args, {PAGED_PREFIX, 0, 0, prefix->n_groups, prefix->max_prefix}, bytes);
+}
+int icua_paged_attention_prefix(const icua_pages_t* pages, const icua_paged_attention_t* args, const icua_paged_prefix_t* prefix, void* stream) {
+    if (!prefix) return fail("paged_attention: null argument");
+    return attention_call(pages, args, {PAGED_PREFIX, 0, 0, prefix->n_groups, prefix->max_prefix}, prefix, stream);
 }
 
 int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, void* stream) {

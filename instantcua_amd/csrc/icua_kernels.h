@@ -285,9 +285,16 @@ struct PagedPlan {
     PagedSplit big;                 // those of more
     int tiles;                      // upper bound of the 128-row tiles of the latter (0: none)
     size_t few_rows, part_rows;     // partial rows of the two (0: none is split)
+    PagedSplit pre;                 // shared prefixes of groups with more rows
+    int pre_tiles;                  // and their tiles
+    size_t pre_rows;                // partial rows of prefixes
 };
 constexpr int PAGED_MAX_SPLITS = 64;
-PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv);
+// The form's sizes: a window and first slots (PAGED_WINDOW); groups and their longest prefix (PAGED_PREFIX).
+struct PagedFormSizes {
+    int form, window, sinks, n_groups, max_prefix;
+};
+PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv, const PagedFormSizes& f);
 struct PagedAttnArgs {
     PageMap map;
     const void *k, *v, *k_sb, *v_sb;
@@ -307,6 +314,12 @@ struct PagedAttnArgs {
     float2* few_ml;                 // (maximum, denominator) of each
     float* part;                    // [n_tokens][n_heads][big.n][128], null: none
     float2* part_ml;
+    PagedFormSizes f;
+    const int32_t *group_start;     // PAGED_PREFIX: [n_groups + 1] first sequence of every group
+    const int32_t *prefix_len;      // [n_groups] slots
+    PagedSplit pre;
+    int pre_tiles;
+    int64_t part_at, pre_at;        // partial rows of `part` and of prefixes ([n_tokens][n_heads][pre.n]) behind few_part
 };
 hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s);
 

@@ -430,6 +430,70 @@ __device__ __forceinline__ float row_value(const void* v, const void* v_sb, int6
     return h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d];
 }
 
+// What the kernels deal out are spans: rows of query tokens and the slots that they go through.  Every sequence is
+// one.  With a window it leaves out the slots between the first ones and those of its first row's window.  With
+// prefixes the groups' are spans too, in front of the sequences': the rows of all the group's tokens over the shared
+// slots, read once for all of them; the sequences then begin behind those, and a row's two parts are joined.
+template <int FORM>
+__device__ __forceinline__ int n_spans(const PagedAttnArgs& a) { return a.n_seqs + (FORM == PAGED_PREFIX ? a.f.n_groups : 0); }
+
+// Lane g: group g.
+template <int FORM>
+__device__ __forceinline__ PrefixGroup load_groups(const PagedAttnArgs& a) {
+    PrefixGroup y = {0, 0, 0};
+    if constexpr (FORM == PAGED_PREFIX) {
+        const int g = threadIdx.x & 63;
+        if (g < a.f.n_groups) y = prefix_group(a.group_start, a.prefix_len, g, a.n_seqs, a.f.max_prefix);
+    }
+    return y;
+}
+struct Span {
+    SeqSpan sp;   // n_kv: of a prefix its slots
+    SlotGap gap;  // (a 128-row tile of a window has its own)
+    __device__ __forceinline__ int slots() const { return max(0, sp.n_kv - gap.skip); }
+};
+// Lane i's span s0 + i, up to `end`.  (s0 is 0 where there are groups among them: group g is lane g's.)
+template <int FORM>
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, const PrefixGroup& gr, int s0, int end) {
+    const int i = s0 + (threadIdx.x & 63);
+    Span y = {{0, 0, 0}, {0, 0}};
+    if constexpr (FORM != PAGED_PREFIX) {
+        if (i < end) y.sp = seq_span(a.q_start, a.kv_len, i, a.n_tokens, a.max_kv);
+        if constexpr (FORM == PAGED_WINDOW) y.gap = window_gap(y.sp.n_kv - y.sp.n_q, y.sp.n_kv, a.f.window, a.f.sinks, 32);
+    } else {
+        const bool pre = i < a.f.n_groups, there = i < end;
+        const int s = i - a.f.n_groups;
+        if (there && !pre) y.sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
+        for (int g = 0; g < a.f.n_groups; ++g) {
+            const int n = __builtin_amdgcn_readlane(gr.n, g), first = __builtin_amdgcn_readlane(gr.s0, g), last = __builtin_amdgcn_readlane(gr.s1, g);
+            if (n && !pre && s >= first && s < last) y.gap.skip = n;
+        }
+        if (there && pre && gr.n) {
+            const int t0 = min(max(a.q_start[gr.s0], 0), a.n_tokens), t1 = min(max(a.q_start[gr.s1], t0), a.n_tokens);
+            y.sp = {t0, t1 - t0, gr.n};
+        }
+    }
+    return y;
+}
+// The last slot of a prefix of n slots that this lane's token t sees; true if all tokens of the group's sequences
+// see all of it.
+__device__ __forceinline__ bool prefix_last(const PagedAttnArgs& a, int s0, int s1, int n, int t, int& last) {
+    bool all = true;
+    last = n - 1;
+    for (int b = s0; b < s1; b += WAVE) {
+        SeqSpan x = {0, 0, 0};
+        if (b + (int)(threadIdx.x & 63) < s1) x = seq_span(a.q_start, a.kv_len, b + (threadIdx.x & 63), a.n_tokens, a.max_kv);
+        uint64_t few = __ballot(x.n_q > 0 && x.n_kv - x.n_q < n - 1);
+        for (; few; few &= few - 1) {
+            all = false;
+            const int j = __ffsll((unsigned long long)few) - 1;
+            const int t0 = __builtin_amdgcn_readlane(x.t0, j), m = __builtin_amdgcn_readlane(x.n_q, j), kv = __builtin_amdgcn_readlane(x.n_kv, j);
+            if (t >= t0 && t < t0 + m) last = min(last, kv - m + t - t0);
+        }
+    }
+    return all;
+}
+
 // Sequences with at most 16 query rows a KV head (single tokens, drafts).  Their slots, in units of a step
 // of all waves of a workgroup, are dealt out evenly: workgroup w of a KV head's `few.n` has units w * per ..
 // of all sequences in a row, whatever the sequences' lengths.  A sequence that lies in one workgroup is
@@ -443,23 +507,23 @@ constexpr int ROWS_PITCH = 80;  // 16-byte places of a wave's results of one dt
 template <int NW>
 constexpr size_t rows_lds() { return NW * (8 * ROWS_PITCH * 16 + 16 * 8); }
 
-// Lane i: sequence s0 + i, its units (0: the chunk kernel's, or none) and those up to its end since s0; `sum`:
+// Lane i: span s0 + i, its units (0: the chunk kernel's, or none) and those up to its end since s0; `sum`:
 // of all 64.
 struct FewUnits {
-    SeqSpan sp;
+    Span x;
     int n, end, sum;
 };
-__device__ __forceinline__ FewUnits few_units(const PagedAttnArgs& a, int group, int s0) {
-    const int lane = threadIdx.x & 63;
-    FewUnits u = {{0, 0, 0}, 0, 0, 0};
-    if (s0 + lane < a.n_seqs) u.sp = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
-    if (u.sp.n_q > 0 && u.sp.n_q * group <= ROWS_TILE) u.n = max(1, (u.sp.n_kv + a.few.unit - 1) / a.few.unit);
+template <int FORM>
+__device__ __forceinline__ FewUnits few_units(const PagedAttnArgs& a, const PrefixGroup& gr, int group, int s0) {
+    const int lane = threadIdx.x & 63, spans = n_spans<FORM>(a);
+    FewUnits u = {span_of<FORM>(a, gr, s0, spans), 0, 0, 0};
+    if (u.x.sp.n_q > 0 && u.x.sp.n_q * group <= ROWS_TILE) u.n = max(1, (u.x.slots() + a.few.unit - 1) / a.few.unit);
     u.end = u.n;
-    for (int o = 1; o < min(WAVE, a.n_seqs); o <<= 1) {
+    for (int o = 1; o < min(WAVE, spans); o <<= 1) {
         const int y = __shfl_up(u.end, o);
         if (lane >= o) u.end += y;
     }
-    u.sum = __builtin_amdgcn_readlane(u.end, min(WAVE, a.n_seqs) - 1);
+    u.sum = __builtin_amdgcn_readlane(u.end, min(WAVE, spans) - 1);
     return u;
 }
 // Units a workgroup takes, of this many.
@@ -476,7 +540,7 @@ __device__ __forceinline__ int few_per(const PagedAttnArgs& a, int total) {
 // tokens over up to 32768 fp16 slots 115 us, 5.4 TB/s; 64 tokens over up to 8192 q8 slots 105 us, 4.7 TB/s (a q8
 // step is some 450 instructions, 2.7 us of a wave), 113 with fp32 queries.  Those spill 15 registers (fp16 slots)
 // and 5 (q8), fp16 queries none.
-template <int TYPE, int FMT, int NW>
+template <int FORM, int TYPE, int FMT, int NW>
 __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uint8_t* lds) {
     // fp32 probabilities in two parts.  With fp16 queries and q8, two parts of V cost as much as two of the
     // probabilities and leave the smaller error (2.5e-4 for 2.9e-4 of the outputs' rms, 2.1e-4 the output's own).
@@ -485,9 +549,11 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
     float2* const sml = (float2*)(lds + NW * 8 * ROWS_PITCH * 16);  // [NW][16]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
     const int g = index % a.map.n_kv, w = index / a.map.n_kv, group = a.n_heads / a.map.n_kv;
-    FewUnits u = few_units(a, group, 0);
+    const PrefixGroup gr = load_groups<FORM>(a);
+    const int spans = n_spans<FORM>(a);
+    FewUnits u = few_units<FORM>(a, gr, group, 0);
     int total = u.sum;
-    for (int s0 = WAVE; s0 < a.n_seqs; s0 += WAVE) total += few_units(a, group, s0).sum;
+    for (int s0 = WAVE; s0 < spans; s0 += WAVE) total += few_units<FORM>(a, gr, group, s0).sum;
     const int per = few_per(a, total), end = min(total, (w + 1) * per);
     int pos = w * per, s0 = 0, before = 0;
     while (pos < end) {
@@ -496,25 +562,52 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
         if (!past) {
             before += u.sum;
             s0 += WAVE;
-            if (s0 >= a.n_seqs) return;
-            u = few_units(a, group, s0);
+            if (s0 >= spans) return;
+            u = few_units<FORM>(a, gr, group, s0);
             continue;
         }
         const int at_lane = __ffsll((unsigned long long)past) - 1, seq_end = before + __builtin_amdgcn_readlane(u.end, at_lane);
         const int seq_units = __builtin_amdgcn_readlane(u.n, at_lane), first = pos - (seq_end - seq_units), count = min(end, seq_end) - pos;
-        const SeqSpan sp = {__builtin_amdgcn_readlane(u.sp.t0, at_lane), __builtin_amdgcn_readlane(u.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.sp.n_kv, at_lane)};
+        const SeqSpan sp = {__builtin_amdgcn_readlane(u.x.sp.t0, at_lane), __builtin_amdgcn_readlane(u.x.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.x.sp.n_kv, at_lane)};
         const bool whole = count == seq_units;
         pos += count;
-        const RowOf row = row_of(sp, r16, group, g);
-        // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.
+        RowOf row = row_of(sp, r16, group, g);
+        // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.  (Of a window: and those of its own.)
         const int start = first * a.few.unit;
-        const int lim = sp.n_kv, all = sp.n_kv - sp.n_q, c1 = min(lim, start + count * a.few.unit);
-        const int32_t* table = a.tables + (int64_t)(s0 + at_lane) * a.table_width;
+        const int lim = sp.n_kv;
+        int all = sp.n_kv - sp.n_q;
+        SlotGap gap = {0, 0};
+        int seq = s0 + at_lane;
+        bool pre = false, joined = false;
+        if constexpr (FORM != PAGED_ALL) gap = {__builtin_amdgcn_readlane(u.x.gap.from, at_lane), __builtin_amdgcn_readlane(u.x.gap.skip, at_lane)};
+        if constexpr (FORM == PAGED_PREFIX) {
+            pre = seq < a.f.n_groups;
+            joined = pre || gap.skip > 0;
+            if (pre) {
+                const int g0 = __builtin_amdgcn_readlane(gr.s0, seq), g1 = __builtin_amdgcn_readlane(gr.s1, seq);
+                all = prefix_last(a, g0, g1, lim, row.t, row.last) ? lim - 1 : -1;
+                seq = g0;
+            } else {
+                seq -= a.f.n_groups;
+            }
+        }
+        const int c1 = min(FORM == PAGED_ALL ? lim : max(0, lim - gap.skip), start + count * a.few.unit);  // of numbers without the gap
+        // Whether this lane's row sees a slot, and whether no row does.  (Without short cuts: selects, no branches.
+        // With them the compiler, ROCm 7.2's, left out the select of -inf for slots before the window.)
+        auto sees = [&](int slot) __attribute__((always_inline)) -> bool {
+            if constexpr (FORM != PAGED_WINDOW) return slot <= row.last;
+            return (slot <= row.last) & ((slot < a.f.sinks) | (slot > row.last - a.f.window));
+        };
+        auto unseen = [&](int slot) __attribute__((always_inline)) -> bool {
+            if constexpr (FORM != PAGED_WINDOW) return false;
+            return (slot >= a.f.sinks) & (slot <= all - a.f.window);
+        };
+        const int32_t* table = a.tables + (int64_t)seq * a.table_width;
         // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).
         auto step_slot = [&](int sub, int i) { return sub + ROWS_STEP * (wave + NW * i); };
         auto lookup = [&](int sub) {
             const int slot = step_slot(sub, lane / 2) + PAGED_TILE * (lane % 2);
-            return slot < c1 ? seq_slot_row(a.map, table, a.table_width, slot) : -1;
+            return slot < c1 ? seq_slot_row(a.map, table, a.table_width, gap_slot(gap, slot)) : -1;
         };
         constexpr int SUB = NW * ROWS_STEP * (WAVE / 2);
         int rows = lookup(start);
@@ -542,7 +635,7 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
         if (n > 0) fetch(0, A);
         const Query<TYPE> y = query_of<TYPE>(qrow, a.scale);
         auto step = [&](int i, Tile<FMT>* t) __attribute__((always_inline)) {
-            const int at = step_slot(sub, i);
+            const int at = gap_slot(gap, step_slot(sub, i));
             const int ok[2] = {__builtin_amdgcn_readlane(rows, 2 * i) < 0 ? 0 : lim, __builtin_amdgcn_readlane(rows, 2 * i + 1) < 0 ? 0 : lim};
             float p[8];
 #pragma unroll
@@ -552,7 +645,8 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                 for (int e = 0; e < 4; ++e) p[4 * k + e] = sc[e] * y.c;
             }
             uint32_t odd = 0;
-            const bool masked = at + ROWS_STEP - 1 > all || ok[0] == 0 || ok[1] == 0;
+            bool masked = at + ROWS_STEP - 1 > all || ok[0] == 0 || ok[1] == 0;
+            if constexpr (FORM == PAGED_WINDOW) masked |= at + ROWS_STEP > a.f.sinks && at <= lim - 1 - a.f.window;
             if (masked) {
                 asm volatile("");
 #pragma unroll
@@ -560,9 +654,9 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int slot = at + 16 * k + 4 * q + e;
-                        if (slot > row.last || slot >= ok[k]) p[4 * k + e] = NEG_INF;
+                        if (!sees(slot) | (slot >= ok[k])) p[4 * k + e] = NEG_INF;
                         // Values of slots that no row sees may be anything: they take no part.
-                        if (slot >= ok[k]) {
+                        if ((slot >= ok[k]) | unseen(slot)) {
                             t[k].v[e] = 0;
                             if constexpr (FMT == FMT_Q8) t[k].vs[e] = 0;
                         }
@@ -646,14 +740,14 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                     if constexpr (PLO) pj += of_slot(pl);
                     const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
                     const uint16_t scale = ((const uint16_t*)a.v_sb)[vrow * NG + q];  // dims 32 q .. + 31 are group q
-                    const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+                    const uint32_t seen = sees(at + j) ? 0xFFFFFFFFu : 0;
                     if (!beyond_fp16(scale)) continue;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int dt = 0; dt < 8; ++dt) {
                             const float x = row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * e + dt);
-                            O[dt][e] += no_number(as_u32(x)) ? as_f32(as_u32(x) & sees) : pj * x;
+                            O[dt][e] += no_number(as_u32(x)) ? as_f32(as_u32(x) & seen) : pj * x;
                         }
                 }
             if (__ballot(odd != 0))
@@ -661,13 +755,13 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
                     const int r = __builtin_amdgcn_readlane(rows, 2 * i + j / PAGED_TILE);
                     if (r < 0 || at + j >= lim) continue;
                     const int64_t vrow = (int64_t)r + g * a.map.page_slots + j % PAGED_TILE;
-                    const uint32_t sees = at + j <= row.last ? 0xFFFFFFFFu : 0;
+                    const uint32_t seen = sees(at + j) ? 0xFFFFFFFFu : 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int dt = 0; dt < 8; ++dt) {
                             const uint32_t x = as_u32(row_value<FMT>(a.v, a.v_sb, vrow, 32 * q + 8 * e + dt));
-                            O[dt][e] += as_f32(x & sees & no_number(x));
+                            O[dt][e] += as_f32(x & seen & no_number(x));
                         }
                 }
         };
@@ -715,25 +809,30 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
 #pragma unroll
                 for (int k = 0; k < DIMS; ++k) x[k] += src[(w * 8 + k) * ROWS_PITCH * 4] * f;
             }
-            const float inv = !whole ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
-            const int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
+            const bool partial = !whole || joined;
+            const float inv = partial ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+            int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
+            if (joined && whole) {
+                const int64_t out_row = (int64_t)out.t * a.n_heads + out.head;
+                part = pre ? a.pre_at + out_row * a.pre.n : a.part_at + out_row * a.big.n;
+            }
 #pragma unroll
             for (int k = 0; k < DIMS; k += 4) {
                 const f32x4 y = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]} * inv;
-                if (!whole)
+                if (partial)
                     *(f32x4*)(a.few_part + part * HD + d0 + k) = y;
                 else
                     store4<TYPE>(a.out, (int64_t)out.t * a.out_stride + out.head * HD + d0 + k, y);
             }
-            if (!whole && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
+            if (partial && d0 == 0) a.few_ml[part] = make_float2(mt, lt);
         }
     }
 }
 
-template <int TYPE, int FMT>
+template <int FORM, int TYPE, int FMT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows_kernel(PagedAttnArgs a) {
     __shared__ __align__(16) uint8_t lds[rows_lds<4>()];
-    rows_work<TYPE, FMT, 4>(a, blockIdx.x, lds);
+    rows_work<FORM, TYPE, FMT, 4>(a, blockIdx.x, lds);
 }
 
 // Sequences with more query rows: 128 rows of a (sequence, KV head) a workgroup, eight waves.  Wave w has
@@ -781,13 +880,15 @@ __device__ __forceinline__ f32x16 mfma32(v8h a, v8h b, f32x16 c) { return __buil
 // and takes those with the most slots first, so that the last workgroups to run are short.  Every workgroup
 // looks through the sequences before its own, so a batch's time has a part that grows with their square:
 // 9 tokens over 200 slots of each of 1024 sequences 0.65 ms, of 16384 (the most in a call) 49 ms.
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int group, int rows, int index, int& s, int& tile, int& tiles, SeqSpan& sp) {
+//
+// Of the spans first .. end - 1.
+template <int FORM>
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, const PrefixGroup& gr, int first, int end, int group, int rows, int index, int& s, int& tile, int& tiles, Span& span) {
     const int lane = threadIdx.x & 63;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
-        const int count = min(WAVE, a.n_seqs - s0);
-        SeqSpan x = {0, 0, 0};
-        if (lane < count) x = seq_span(a.q_start, a.kv_len, s0 + lane, a.n_tokens, a.max_kv);
-        const int n = x.n_q * group > ROWS_TILE ? (x.n_q * group + rows - 1) / rows : 0;
+    for (int s0 = first; s0 < end; s0 += WAVE) {
+        const int count = min(WAVE, end - s0);
+        const Span x = span_of<FORM>(a, gr, s0, end);
+        const int n = x.sp.n_q * group > ROWS_TILE ? (x.sp.n_q * group + rows - 1) / rows : 0, slots = FORM == PAGED_PREFIX ? x.slots() : x.sp.n_kv;
         int sum = n;
 #pragma unroll
         for (int o = 1; o < WAVE; o <<= 1) sum += __shfl_xor(sum, o);
@@ -796,23 +897,24 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, int group, int
             index -= sum;
             continue;
         }
-        int begin = 0;  // tiles of the sequences that come before lane's
+        int begin = 0;  // tiles of the spans that come before lane's
         for (int j = 0; j < count; ++j) {
-            const int kv = __builtin_amdgcn_readlane(x.n_kv, j), add = __builtin_amdgcn_readlane(n, j);
-            if (kv > x.n_kv || (kv == x.n_kv && j < lane)) begin += add;
+            const int kv = __builtin_amdgcn_readlane(slots, j), add = __builtin_amdgcn_readlane(n, j);
+            if (kv > slots || (kv == slots && j < lane)) begin += add;
         }
         const uint64_t mine = __ballot(index >= begin && index < begin + n);
         const int i = __ffsll((unsigned long long)mine) - 1;
         tile = index - __builtin_amdgcn_readlane(begin, i);
         tiles = __builtin_amdgcn_readlane(n, i);
-        sp = {__builtin_amdgcn_readlane(x.t0, i), __builtin_amdgcn_readlane(x.n_q, i), __builtin_amdgcn_readlane(x.n_kv, i)};
+        span.sp = {__builtin_amdgcn_readlane(x.sp.t0, i), __builtin_amdgcn_readlane(x.sp.n_q, i), __builtin_amdgcn_readlane(x.sp.n_kv, i)};
+        span.gap = {__builtin_amdgcn_readlane(x.gap.from, i), __builtin_amdgcn_readlane(x.gap.skip, i)};
         s = s0 + i;
         return true;
     }
     return false;
 }
 
-template <int TYPE, int FMT>
+template <int FORM, int TYPE, int FMT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
     constexpr bool HL = TYPE == TYPE_F32, CODES = FMT == FMT_Q8;
     extern __shared__ __align__(1024) uint8_t lds[];
@@ -820,25 +922,65 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int *const tile_there = tile_odd + 16, *const tile_top = tile_odd + 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
-    // The last workgroups have the sequences of few rows: they are short, and bound by memory.
-    const int index = blockIdx.x, few = index - a.tiles * a.map.n_kv * a.big.n;
-    if (few >= 0) {
-        rows_work<TYPE, FMT, 8>(a, few, lds);
+    // The first workgroups have the shared prefixes, the last ones the spans of few rows: they are short, and bound
+    // by memory.
+    int index = blockIdx.x;
+    bool pre = false;
+    PagedSplit parts = a.big;
+    if constexpr (FORM == PAGED_PREFIX) {
+        pre = index < a.pre_tiles * a.map.n_kv * a.pre.n;
+        if (pre)
+            parts = a.pre;
+        else
+            index -= a.pre_tiles * a.map.n_kv * a.pre.n;
+    }
+    const int few = index - a.tiles * a.map.n_kv * a.big.n;
+    if (!pre && few >= 0) {
+        rows_work<FORM, TYPE, FMT, 8>(a, few, lds);
         return;
     }
-    const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % a.big.n;
+    const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % parts.n;
+    const PrefixGroup gr = load_groups<FORM>(a);
+    const int first_span = FORM != PAGED_PREFIX || pre ? 0 : a.f.n_groups, end_span = pre ? a.f.n_groups : n_spans<FORM>(a);
     int s, tile, tiles;
-    SeqSpan sp;
-    if (!find_tile(a, group, CH_ROWS, at / a.big.n, s, tile, tiles, sp)) return;
+    Span span;
+    if (!find_tile<FORM>(a, gr, first_span, end_span, group, CH_ROWS, at / parts.n, s, tile, tiles, span)) return;
     tile = tiles - 1 - tile;  // those that see the most slots first
+    const SeqSpan sp = span.sp;
     const int before = sp.n_kv - sp.n_q;  // token i sees slots up to before + i
     const int r0 = tile * CH_ROWS + 32 * wi;
     const bool active = r0 < sp.n_q * group;
-    const int w_first = before + r0 / group, w_last = before + min(sp.n_q - 1, (r0 + 31) / group);
-    const int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
-    const RowOf row = row_of(sp, r0 + c32, group, g);
-    const int c0 = min(lim, split * a.big.chunk), c1 = min(lim, c0 + a.big.chunk);
+    int w_first = before + r0 / group, w_last = before + min(sp.n_q - 1, (r0 + 31) / group);
+    int all_seen = before + tile * CH_ROWS / group;  // slots up to this one all rows of the workgroup see
+    int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
+    RowOf row = row_of(sp, r0 + c32, group, g);
+    // Iterations are of 128 slots, numbered without those that are skipped.
+    int it_from = 0, it_skip = 0, group_s1 = 0;
+    bool joined = false;
+    if constexpr (FORM == PAGED_WINDOW) {
+        const SlotGap gap = window_gap(all_seen, lim, a.f.window, a.f.sinks, 128);
+        it_from = gap.from / 128;
+        it_skip = gap.skip / 128;
+    }
+    if constexpr (FORM == PAGED_PREFIX) {
+        it_skip = span.gap.skip / 128;
+        joined = pre || it_skip > 0;
+        if (pre) {
+            group_s1 = __builtin_amdgcn_readlane(gr.s1, s);
+            s = __builtin_amdgcn_readlane(gr.s0, s);
+            lim = sp.n_kv;
+            w_first = w_last = all_seen = lim - 1;
+            row.last = lim - 1;
+        } else {
+            s -= a.f.n_groups;
+        }
+    }
+    auto first_slot = [&](int it) __attribute__((always_inline)) { return (FORM == PAGED_ALL || it < it_from ? it : it + it_skip) * 128; };
+    const int left = FORM == PAGED_ALL ? lim : max(0, lim - 128 * it_skip);
+    const int c0 = min(left, split * parts.chunk), c1 = min(left, c0 + parts.chunk);
     const int it0 = c0 / 128, it1 = c1 > c0 ? (c1 + 127) / 128 : it0;
+    // A window's rows see slots from first_own on, those of this wave from w_low .. w_high, and the first ones.
+    const int first_own = row.last - a.f.window + 1, w_low = w_first - a.f.window + 1, w_high = w_last - a.f.window + 1;
 
     // Query operands: dims 16 ks + 8 h .. + 7 of the column's row.  Loaded first, then the first K and V are
     // asked for, and what both take is waited for once.
@@ -866,8 +1008,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             auto b = arguments();
             const PageMap map = {b->map.n_pages, b->map.n_kv, b->map.page_slots};
             sub = it;
-            const int slot = (sub + lane) * 128 + 16 * wave;
-            rows = slot < c1 ? seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, slot) : -1;
+            const int slot = first_slot(sub + lane) + 16 * wave;
+            rows = slot < (FORM == PAGED_ALL ? c1 : lim) ? seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, slot) : -1;
         }
         return __builtin_amdgcn_readlane(rows, it - sub);
     };
@@ -882,7 +1024,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int j = 0; j < 4; ++j) src_off[j] = (4 * j + lane / 16) * (HD * 2) + (((lane & 15) ^ swizzle(4 * j + lane / 16)) << 4);
     auto copy = [&](int kv, int it, int r) __attribute__((always_inline)) {
-        const int n = r < 0 ? 0 : lim - (it * 128 + 16 * wave);
+        const int n = r < 0 ? 0 : lim - (first_slot(it) + 16 * wave);
         const uint32_t dst = lds0 + half_at(kv, it & 1, par) + wi * 16 * HD * 2;
         const uint8_t* src = (kv ? v_base : k_base) + (int64_t)(max(r, 0) + head_row) * (HD * 2);
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
@@ -903,7 +1045,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     u32x4 codes[2][2];
     uint16_t scale[2] = {0, 0};
     auto fetch = [&](int kv, int it, int r) __attribute__((always_inline)) {
-        const int n = r < 0 ? 0 : lim - (it * 128 + 16 * wave);
+        const int n = r < 0 ? 0 : lim - (first_slot(it) + 16 * wave);
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
         codes[kv][0] = codes[kv][1] = u32x4{0, 0, 0, 0};
         scale[kv] = 0;
@@ -1001,19 +1143,27 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // Whether the table has pages outside the pool.
     bool bad_pages = false;
-    {
+    auto look_at_pages = [&](int c0, int c1) {
         const int32_t* table = a.tables + (int64_t)s * a.table_width;
         const int last_page = c1 > c0 ? (c1 - 1) / a.map.page_slots : -1;
         for (int p = c0 / a.map.page_slots; p <= last_page; p += WAVE)
             if (__ballot(p + lane <= last_page && page_row(a.map, table[min(p + lane, last_page)], 0) < 0)) bad_pages = true;
+    };
+    if constexpr (FORM == PAGED_ALL) {
+        look_at_pages(c0, c1);
+    } else {
+        look_at_pages(c0, min(c1, 128 * it_from));
+        look_at_pages(max(c0, 128 * it_from) + 128 * it_skip, c1 + 128 * it_skip);
     }
+    if constexpr (FORM == PAGED_PREFIX)
+        if (pre && !prefix_last(a, s, group_s1, lim, row.t, row.last)) w_first = all_seen = -1;
     if (it0 < it1) staged(it0);
 
     f32x16 O[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
     float m = NEG_INF, l = 0.f;
-    auto base_of = [&](int it) { return it * 128 + CH_HALF * par; };
+    auto base_of = [&](int it) __attribute__((always_inline)) { return first_slot(it) + CH_HALF * par; };
     // LDS addresses of operands in stage 0.  K of block 0: slot c32, dims 16 ks + 8 h .. + 7, at k_at ^ (ks <<
     // 5).  V^T: dims 32 dt + c32 of slots 4 h + {0 .. 3} (k = 1: + 8, the operand's other half), at v_at[k] ^
     // (dt << 6).  (A row's place in a stage is a multiple of its 256 bytes.)
@@ -1038,12 +1188,19 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // Scores of a block are unscaled; element i: slot 8 (i / 4) + 4 h + i % 4.
     auto mask = [&](int it, int kt, f32x16& S) __attribute__((always_inline)) {
         const int base = base_of(it) + 32 * kt;
-        if (base + 31 <= w_first && !bad_pages) return;
+        const bool ends = FORM == PAGED_WINDOW && base + 31 >= a.f.sinks && base < w_high;  // before some row's window
+        if (base + 31 <= w_first && !bad_pages && !ends) return;
         asm volatile("");  // keeps the branch: the selects are not made where they are not needed
         const int seen = row.last - base - 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (8 * (i / 4) + i % 4 > seen) S[i] = NEG_INF;
+        if (ends) {
+            const int from = a.f.sinks - base - 4 * h, to = first_own - base - 4 * h;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((8 * (i / 4) + i % 4 >= from) & (8 * (i / 4) + i % 4 < to)) S[i] = NEG_INF;
+        }
         if (bad_pages) {
             const int2 there = *(const int2*)(tile_there + (it & 1) * 8 + 4 * par + 2 * kt);
 #pragma unroll
@@ -1270,7 +1427,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     // Whether some row of the workgroup does not see all of an iteration: of an f16 pool, all of its values are
     // made finite then, also for waves whose rows see them.
-    auto cleaned = [&](int it) __attribute__((always_inline)) { return it * 128 + 127 > before + tile * CH_ROWS / group; };
+    auto cleaned = [&](int it) __attribute__((always_inline)) {
+        const int at = first_slot(it);
+        return at + 127 > all_seen || (FORM == PAGED_WINDOW && at + 127 >= a.f.sinks && at <= lim - 1 - a.f.window);
+    };
     // Values that are no numbers were kept out of the products: they go to the rows that see them.
     auto add_odd_values = [&](int it) __attribute__((always_inline)) {
         const int base = base_of(it);
@@ -1282,7 +1442,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int j = 0; j < CH_HALF && base + j < lim; ++j) {
             const int r = seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, base + j);
             if (r < 0) continue;
-            const uint32_t sees = base + j <= row.last ? 0xFFFFFFFFu : 0;
+            const bool own = FORM != PAGED_WINDOW || (base + j < a.f.sinks) | (base + j >= first_own);
+            const uint32_t sees = (base + j <= row.last) & own ? 0xFFFFFFFFu : 0;
 #pragma unroll
             for (int k = 0; k < 16; ++k)
 #pragma unroll
@@ -1310,12 +1471,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         staged_barrier<63>();
     };
     // Iterations whose half some row of this wave sees.
-    const int my1 = active && base_of(it0) <= w_last ? min(it1, (w_last - CH_HALF * par) / 128 + 1) : it0;
+    int my1 = active && base_of(it0) <= w_last ? (w_last - CH_HALF * par) / 128 + 1 : it0;
+    if (FORM != PAGED_ALL && my1 > it_from) my1 = max(it_from, my1 - it_skip);
+    my1 = min(it1, my1);
     for (int it = it0; it < it1; ++it) {
         staged_barrier<0>();
         if (it + 1 < it1) stage(it + 1);
         if constexpr (FMT == FMT_F16) clean_values(it);
-        if (it < my1) {
+        if (it < my1 && (FORM != PAGED_WINDOW || base_of(it) < a.f.sinks || base_of(it) + CH_HALF > w_low)) {
             if constexpr (!CODES) {
                 half_step(it);
             } else {
@@ -1361,8 +1524,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const float mt = fmaxf(m, ml.x);
     const float f0 = m == mt ? 1.f : __builtin_amdgcn_exp2f(m - mt), f1 = ml.x == mt ? 1.f : __builtin_amdgcn_exp2f(ml.x - mt);
     const float lt = l * f0 + ml.y * f1;
-    const float inv = a.big.n > 1 ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
-    const int64_t out_row = (int64_t)row.t * a.n_heads + row.head;
+    const bool partial = parts.n > 1 || joined;
+    const float inv = partial ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
+    const int64_t out_row = ((int64_t)row.t * a.n_heads + row.head) * parts.n + split;
+    float* const part = FORM != PAGED_PREFIX ? a.part : a.few_part + (pre ? a.pre_at : a.part_at) * HD;
+    float2* const part_ml = FORM != PAGED_PREFIX ? a.part_ml : a.few_ml + (pre ? a.pre_at : a.part_at);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         const f32x4 o1 = mo[(wi * 16 + k) * 64 + lane];
@@ -1370,12 +1536,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = (O[k / 4][4 * (k % 4) + e] * f0 + o1[e] * f1) * inv;
         const int d = 32 * (k / 4) + 8 * (k % 4) + 4 * h;
-        if (a.big.n > 1)
-            *(f32x4*)(a.part + (out_row * a.big.n + split) * HD + d) = y;
+        if (partial)
+            *(f32x4*)(part + out_row * HD + d) = y;
         else
             store4<TYPE>(a.out, (int64_t)row.t * a.out_stride + row.head * HD + d, y);
     }
-    if (a.big.n > 1 && h == 0) a.part_ml[out_row * a.big.n + split] = make_float2(mt, lt);
+    if (partial && h == 0) part_ml[out_row] = make_float2(mt, lt);
 }
 
 // Joins the partials of a row, at part_at(0 .. n - 1): 32 lanes have a partial's 128 values, four each, so a
@@ -1410,40 +1576,87 @@ __device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int hea
     if (lane < 32) store4<TYPE>(a.out, (int64_t)t * a.out_stride + head * HD + d, o * inv);
 }
 
-// Row r of a few-row sequence s and KV head g, if workgroups share the sequence.
-template <int TYPE>
-__device__ __forceinline__ void merge_few(const PagedAttnArgs& a, int s, const SeqSpan& sp, int g, int r) {
+// The workgroups of a KV head that share few-row span s: `n` of them from w0 on.
+struct FewParts {
+    int w0, n;
+};
+template <int FORM>
+__device__ __forceinline__ FewParts few_parts(const PagedAttnArgs& a, const PrefixGroup& gr, int s) {
     const int group = a.n_heads / a.map.n_kv;
-    int total = 0, begin = 0, n = 0;  // units of all sequences, those before s, its own
-    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
-        const FewUnits u = few_units(a, group, s0);
+    int total = 0, begin = 0, n = 0;  // units of all spans, those before s, its own
+    for (int s0 = 0; s0 < n_spans<FORM>(a); s0 += WAVE) {
+        const FewUnits u = few_units<FORM>(a, gr, group, s0);
         if (s >= s0 && s < s0 + WAVE) {
             n = __builtin_amdgcn_readlane(u.n, s - s0);
             begin = total + __builtin_amdgcn_readlane(u.end, s - s0) - n;
         }
         total += u.sum;
     }
-    const int per = few_per(a, total), w0 = begin / per, parts = (begin + n - 1) / per - w0 + 1;
-    if (parts < 2 || r >= a.few.rows) return;
-    merge_row<TYPE>(a, sp.t0 + r / group, g * group + r % group, a.few_part, a.few_ml, parts, [&](int i) {
-        return (((int64_t)(w0 + i) * a.map.n_kv + g) * 2 + (i == 0)) * a.few.rows + r;
-    });
+    const int per = few_per(a, total), w0 = begin / per;
+    return {w0, (begin + n - 1) / per - w0 + 1};
+}
+// Partial i of its row r, KV head g.
+__device__ __forceinline__ int64_t few_at(const PagedAttnArgs& a, const FewParts& p, int g, int r, int i) {
+    return (((int64_t)(p.w0 + i) * a.map.n_kv + g) * 2 + (i == 0)) * a.few.rows + r;
+}
+
+// Row r of a few-row sequence s and KV head g, if workgroups share the sequence.
+template <int FORM, int TYPE>
+__device__ __forceinline__ void merge_few(const PagedAttnArgs& a, int s, const SeqSpan& sp, int g, int r) {
+    const int group = a.n_heads / a.map.n_kv;
+    const FewParts p = few_parts<FORM>(a, PrefixGroup{}, s);
+    if (p.n < 2 || r >= a.few.rows) return;
+    merge_row<TYPE>(a, sp.t0 + r / group, g * group + r % group, a.few_part, a.few_ml, p.n, [&](int i) { return few_at(a, p, g, r, i); });
 }
 
 // Where only sequences of few rows are split: a workgroup has four of the at most 16 rows of a (sequence, KV
 // head), a wave one.
-template <int TYPE>
+template <int FORM, int TYPE>
 __global__ __launch_bounds__(256) void paged_merge_rows_kernel(PagedAttnArgs a) {
     const int r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int s = blockIdx.x / a.map.n_kv, g = blockIdx.x % a.map.n_kv;
     const SeqSpan sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
     const int rows = sp.n_q * (a.n_heads / a.map.n_kv);
     if (rows > ROWS_TILE || r >= rows) return;
-    merge_few<TYPE>(a, s, sp, g, r);
+    merge_few<FORM, TYPE>(a, s, sp, g, r);
+}
+
+// Row (t, head) of sequence s with prefixes: the partials of its group's, then its own.  Those of a span that one
+// workgroup has done are in its place in `part`.
+template <int TYPE>
+__device__ __forceinline__ void merge_prefix(const PagedAttnArgs& a, int t, int head, int s, const SeqSpan& sp) {
+    const int lane = threadIdx.x & 63, group = a.n_heads / a.map.n_kv, g = head / group;
+    const int64_t row = (int64_t)t * a.n_heads + head;
+    const PrefixGroup gr = load_groups<PAGED_PREFIX>(a);
+    const uint64_t in = __ballot(lane < a.f.n_groups && gr.n > 0 && s >= gr.s0 && s < gr.s1);
+    FewParts pre = {0, 0}, own = {0, a.big.n};
+    bool pre_few = false;
+    const bool own_few = sp.n_q * group <= ROWS_TILE;
+    int pre_r = 0;
+    if (in) {
+        const int i = 63 - __clzll((long long)in);  // the last one that has it, as span_of takes it
+        const Span x = span_of<PAGED_PREFIX>(a, gr, 0, a.f.n_groups);
+        const int t0 = __builtin_amdgcn_readlane(x.sp.t0, i), n_q = __builtin_amdgcn_readlane(x.sp.n_q, i);
+        pre_few = n_q * group <= ROWS_TILE;
+        pre = {0, a.pre.n};
+        pre_r = min(max((t - t0) * group + head % group, 0), a.few.rows - 1);  // (of starts that rise: as it is)
+        if (pre_few) pre = few_parts<PAGED_PREFIX>(a, gr, i);
+    }
+    if (own_few)
+        own = few_parts<PAGED_PREFIX>(a, gr, a.f.n_groups + s);
+    else if (!a.tiles)
+        return;  // more tokens than max_q
+    if (!in && own.n < 2) return;  // written already
+    const int own_r = (t - sp.t0) * group + head % group;
+    merge_row<TYPE>(a, t, head, a.few_part, a.few_ml, pre.n + own.n, [&](int i) {
+        if (i < pre.n) return pre_few && pre.n > 1 ? few_at(a, pre, g, pre_r, i) : a.pre_at + row * a.pre.n + i;
+        i -= pre.n;
+        return own_few && own.n > 1 ? few_at(a, own, g, own_r, i) : a.part_at + row * a.big.n + i;
+    });
 }
 
 // Else a wave a row, over all tokens; rows of no sequence stay as they are.
-template <int TYPE>
+template <int FORM, int TYPE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int lane = threadIdx.x & 63, group = a.n_heads / a.map.n_kv;
@@ -1456,8 +1669,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
         if (!mine) continue;
         const int i = __ffsll((unsigned long long)mine) - 1;
         const SeqSpan sp = {__builtin_amdgcn_readlane(x.t0, i), __builtin_amdgcn_readlane(x.n_q, i), __builtin_amdgcn_readlane(x.n_kv, i)};
-        if (sp.n_q * group <= ROWS_TILE)
-            merge_few<TYPE>(a, s0 + i, sp, head / group, (t - sp.t0) * group + head % group);
+        if constexpr (FORM == PAGED_PREFIX)
+            merge_prefix<TYPE>(a, t, head, s0 + i, sp);
+        else if (sp.n_q * group <= ROWS_TILE)
+            merge_few<FORM, TYPE>(a, s0 + i, sp, head / group, (t - sp.t0) * group + head % group);
         else
             merge_row<TYPE>(a, t, head, a.part, a.part_ml, a.big.n, [&](int k) { return row * a.big.n + k; });
         return;
@@ -1497,63 +1712,83 @@ hipError_t launch_paged_load(int fmt, int type, const PagedLoadArgs& a, hipStrea
 
 // Splits of max_kv slots among `per` workgroups of each (sequence, rows, KV head) that make up to `want`
 // in all, each a multiple of 128 slots.
-static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv) {
+static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv, int max_splits) {
     const int64_t most = std::max(1, (max_kv + 127) / 128);
-    const int n = (int)std::min<int64_t>({std::max<int64_t>(1, want / std::max<int64_t>(1, groups)), most, PAGED_MAX_SPLITS});
+    const int n = (int)std::min<int64_t>({std::max<int64_t>(1, want / std::max<int64_t>(1, groups)), most, max_splits});
     const int chunk = std::max(128, ((max_kv + n - 1) / n + 127) / 128 * 128);
     return {std::max(1, (max_kv + chunk - 1) / chunk), chunk};
 }
 
-// Units of few-row sequences among `want` workgroups: no sequence in more than PAGED_MAX_SPLITS of them.
+// Units of few-row sequences among `want` workgroups: no sequence in more than max_splits of them.
 //
 // 512 workgroups are what the registers let run at once: 64 q8 sequences of up to 8192 slots take 110 us with 512,
 // 143 with 256, 127 with 768 and 116 with 1024.  fp16 steps are twice a q8 step's bytes, and half as many workgroups
 // read long caches faster: eight sequences of up to 32768 slots 121 us, 128 without the doubled shares.
-static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, int rows, int max_kv) {
+static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, int rows, int max_kv, int max_splits) {
     const int most = std::max(1, (max_kv + unit - 1) / unit);
     const int n = (int)std::min(std::max<int64_t>(1, want / n_kv), (int64_t)n_seqs * most);
-    return {n, unit, most < 2 ? 1 : (most - 2) / (PAGED_MAX_SPLITS - 1) + 1, twice, rows};
+    return {n, unit, most < 2 ? 1 : (most - 2) / (max_splits - 1) + 1, twice, rows};
 }
 
-PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv) {
+PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv, const PagedFormSizes& f) {
     PagedPlan p{};
-    const int group = n_heads / n_kv, few = (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
+    const bool prefix = f.form == PAGED_PREFIX;
+    const int group = n_heads / n_kv, spans = n_seqs + (prefix ? f.n_groups : 0);
+    const int few = prefix ? ROWS_TILE : (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
+    const int max_splits = prefix ? PAGED_MAX_SPLITS / 2 : PAGED_MAX_SPLITS;  // a row has partials of two spans
+    if (f.form == PAGED_WINDOW) max_kv = window_slots(max_kv, f.window, f.sinks);
     p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
-    if ((int64_t)max_q * group > ROWS_TILE) {
-        p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
-        p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv);
-        p.few = few_of(256, 8 * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv);
-    } else {
-        p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, n_seqs, few, max_kv);
+    p.pre = {1, std::max(128, (f.max_prefix + 127) / 128 * 128)};
+    const bool big = (int64_t)max_q * group > ROWS_TILE, pre = prefix && (int64_t)n_tokens * group > ROWS_TILE;
+    if (pre) {
+        p.pre_tiles = (int)(((int64_t)n_tokens * group + 127 * std::min<int64_t>(f.n_groups, (int64_t)n_tokens * group / (ROWS_TILE + 1))) / CH_ROWS);
+        p.pre = split_slots((int64_t)p.pre_tiles * n_kv, 256, f.max_prefix, max_splits);
     }
-    if (p.big.n > 1) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
+    if (big) {
+        p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
+        p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv, max_splits);
+    }
+    if (big || pre)
+        p.few = few_of(256, 8 * ROWS_STEP, INT32_MAX, n_kv, spans, few, max_kv, max_splits);
+    else
+        p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, spans, few, max_kv, max_splits);
+    if (p.big.n > 1 || prefix) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
+    if (prefix) p.pre_rows = (size_t)n_tokens * n_heads * p.pre.n;
     if (p.few.n > 1 && max_kv > p.few.unit) p.few_rows = (size_t)p.few.n * n_kv * 2 * few;
     return p;
 }
 
-template <int TYPE, int FMT>
+template <int FORM, int TYPE, int FMT>
 static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
     const unsigned few = (unsigned)a.few.n * a.map.n_kv;
     hipError_t e;
-    if (a.tiles) {
-        e = hipFuncSetAttribute((const void*)paged_chunk_kernel<TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, CH_LDS);
+    if (a.tiles || a.pre_tiles) {
+        e = hipFuncSetAttribute((const void*)paged_chunk_kernel<FORM, TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, CH_LDS);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_chunk_kernel<TYPE, FMT>), dim3(few + (unsigned)a.tiles * a.map.n_kv * a.big.n), dim3(512), CH_LDS, s, a);
+        const unsigned tiles = (unsigned)a.tiles * a.map.n_kv * a.big.n + (unsigned)a.pre_tiles * a.map.n_kv * a.pre.n;
+        hipLaunchKernelGGL((paged_chunk_kernel<FORM, TYPE, FMT>), dim3(few + tiles), dim3(512), CH_LDS, s, a);
     } else {
-        hipLaunchKernelGGL((paged_rows_kernel<TYPE, FMT>), dim3(few), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((paged_rows_kernel<FORM, TYPE, FMT>), dim3(few), dim3(256), 0, s, a);
     }
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.part)
-        hipLaunchKernelGGL(paged_merge_kernel<TYPE>, dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a);
+    if (a.part || FORM == PAGED_PREFIX)
+        hipLaunchKernelGGL((paged_merge_kernel<FORM, TYPE>), dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a);
     else if (a.few_part)
-        hipLaunchKernelGGL(paged_merge_rows_kernel<TYPE>, dim3((unsigned)a.n_seqs * a.map.n_kv, (unsigned)(a.few.rows + 3) / 4), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((paged_merge_rows_kernel<FORM, TYPE>), dim3((unsigned)a.n_seqs * a.map.n_kv, (unsigned)(a.few.rows + 3) / 4), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
+template <int FORM>
+static hipError_t attention_form(int fmt, int type, const PagedAttnArgs& a, hipStream_t s) {
+    if (fmt == FMT_Q8) return type == TYPE_F32 ? attention_of<FORM, TYPE_F32, FMT_Q8>(a, s) : attention_of<FORM, TYPE_F16, FMT_Q8>(a, s);
+    return type == TYPE_F32 ? attention_of<FORM, TYPE_F32, FMT_F16>(a, s) : attention_of<FORM, TYPE_F16, FMT_F16>(a, s);
+}
+
 hipError_t launch_paged_attention(int fmt, int type, const PagedAttnArgs& a, hipStream_t s) {
-    if (fmt == FMT_Q8) return type == TYPE_F32 ? attention_of<TYPE_F32, FMT_Q8>(a, s) : attention_of<TYPE_F16, FMT_Q8>(a, s);
-    return type == TYPE_F32 ? attention_of<TYPE_F32, FMT_F16>(a, s) : attention_of<TYPE_F16, FMT_F16>(a, s);
+    if (a.f.form == PAGED_WINDOW) return attention_form<PAGED_WINDOW>(fmt, type, a, s);
+    if (a.f.form == PAGED_PREFIX) return attention_form<PAGED_PREFIX>(fmt, type, a, s);
+    return attention_form<PAGED_ALL>(fmt, type, a, s);
 }
 
 }  // namespace icua

@@ -41,6 +41,8 @@ EXPORTS = [
     "icua_memcpy_d2h", "icua_device_sync", "icua_repack", "icua_gemv", "icua_gemv_bench", "icua_dequant",
     "icua_quantize", "icua_quantize_noalloc", "icua_quantize_bench", "icua_vision", "icua_generate_vision",
     "icua_paged_store", "icua_paged_attention", "icua_paged_attention_work", "icua_paged_load",
+    "icua_paged_attention_window", "icua_paged_attention_window_work", "icua_paged_attention_prefix",
+    "icua_paged_attention_prefix_work",
     "icua_i8_quantize", "icua_i8_matmul", "icua_i8_matmul_work",
     # include/icua_tok.h
     "icua_tok_last_error", "icua_tok_open", "icua_tok_close", "icua_tok_vocab_size", "icua_tok_special_id",
@@ -122,6 +124,9 @@ def lib() -> C.CDLL:
         L.icua_paged_attention.argtypes = [vp, vp, vp]
         L.icua_paged_attention_work.argtypes = [vp, vp, C.POINTER(sz)]
         L.icua_paged_load.argtypes = [vp, vp, vp]
+        for form in ("window", "prefix"):
+            getattr(L, f"icua_paged_attention_{form}").argtypes = [vp, vp, vp, vp]
+            getattr(L, f"icua_paged_attention_{form}_work").argtypes = [vp, vp, vp, C.POINTER(sz)]
         L.icua_i8_quantize.argtypes = [vp, vp]
         L.icua_i8_matmul.argtypes = [vp, vp]
         L.icua_i8_matmul_work.argtypes = [vp, C.POINTER(sz)]

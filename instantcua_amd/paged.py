@@ -2,7 +2,8 @@
 ``include/icua.h``).
 
 ``PagedCache`` is one layer's pool.  ``store`` normalises, rotates and writes new tokens, ``attention``
-runs every sequence's new tokens over its slots, ``load`` reads slots back.  Buffers are anything with
+runs every sequence's new tokens over its slots (``attention_window``: over a window of them and a few first
+ones; ``attention_prefix``: sequences that share their first slots), ``load`` reads slots back.  Buffers are anything with
 a device address ``ptr`` (``engine.DeviceBuffer``).  The calls enqueue on ``stream`` (a hipStream_t as
 an integer, 0: the null stream) and return without waiting; ``engine.lib().icua_device_sync`` or a copy
 to the host waits.  Errors raise ``EngineError``.
@@ -39,6 +40,14 @@ class _Attention(C.Structure):
                 ("q_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64), ("q_start", C.c_void_p),
                 ("kv_len", C.c_void_p), ("tables", C.c_void_p), ("table_width", C.c_int32), ("work", C.c_void_p),
                 ("work_bytes", C.c_size_t)]
+
+
+class _Window(C.Structure):
+    _fields_ = [("window", C.c_int32), ("sinks", C.c_int32)]
+
+
+class _Prefix(C.Structure):
+    _fields_ = [("n_groups", C.c_int32), ("max_prefix", C.c_int32), ("group_start", C.c_void_p), ("prefix_len", C.c_void_p)]
 
 
 class _Load(C.Structure):
@@ -101,21 +110,60 @@ class PagedCache:
         """Bytes of workspace for an attention call of exactly these sizes; without ``table_width`` the table is
         taken to be as wide as ``max_kv`` slots need, or one page if that is 0 too (a call without a bound on
         slots over wider tables has to say their width here)."""
+        return self._work("", None, n_heads, n_seqs, n_tokens, table_width, max_q, max_kv)
+
+    def _work(self, form, more, n_heads, n_seqs, n_tokens, table_width, max_q, max_kv):
         if table_width is None:
             table_width = max(1, -(-max_kv // self.page_slots))
         a = _Attention(0, n_heads, n_seqs, n_tokens, max_q, max_kv, 0.0, table_width=table_width)
         n = C.c_size_t()
-        _check(lib().icua_paged_attention_work(self._at, C.addressof(a), C.byref(n)))
+        extra = [] if more is None else [C.addressof(more)]
+        _check(getattr(lib(), f"icua_paged_attention{form}_work")(self._at, C.addressof(a), *extra, C.byref(n)))
         return n.value
 
     def attention(self, q, out, n_heads: int, q_start, kv_len, tables, n_seqs: int, n_tokens: int, table_width: int,
                   max_q: int = 0, max_kv: int = 0, scale: float = 0.0, type: int = F32, q_stride: int = 0,
                   out_stride: int = 0, work=None, stream: int = 0) -> None:
         """icua_paged_attention; ``work`` has ``attention_work`` bytes (None where that is 0)."""
-        a = _Attention(type, n_heads, n_seqs, n_tokens, max_q, max_kv, scale, _ptr(q), q_stride, _ptr(out),
-                       out_stride, _ptr(q_start), _ptr(kv_len), _ptr(tables), table_width, _ptr(work),
-                       0 if work is None else work.nbytes)
-        _check(lib().icua_paged_attention(self._at, C.addressof(a), stream))
+        self._attention("", None, stream, type, n_heads, n_seqs, n_tokens, max_q, max_kv, scale, _ptr(q), q_stride,
+                        _ptr(out), out_stride, _ptr(q_start), _ptr(kv_len), _ptr(tables), table_width, _ptr(work),
+                        0 if work is None else work.nbytes)
+
+    def _attention(self, form, more, stream, *fields):
+        a = _Attention(*fields)
+        extra = [] if more is None else [C.addressof(more)]
+        _check(getattr(lib(), f"icua_paged_attention{form}")(self._at, C.addressof(a), *extra, stream))
+
+    def attention_window_work(self, n_heads: int, n_seqs: int, n_tokens: int, window: int, sinks: int = 0,
+                              table_width: Optional[int] = None, max_q: int = 0, max_kv: int = 0) -> int:
+        """``attention_work`` of an ``attention_window`` call."""
+        return self._work("_window", _Window(window, sinks), n_heads, n_seqs, n_tokens, table_width, max_q, max_kv)
+
+    def attention_window(self, q, out, n_heads: int, q_start, kv_len, tables, n_seqs: int, n_tokens: int,
+                         table_width: int, window: int, sinks: int = 0, max_q: int = 0, max_kv: int = 0,
+                         scale: float = 0.0, type: int = F32, q_stride: int = 0, out_stride: int = 0, work=None,
+                         stream: int = 0) -> None:
+        """icua_paged_attention_window: a token sees its own and the ``window`` - 1 slots before it, and the first
+        ``sinks`` slots of its sequence; ``work`` has ``attention_window_work`` bytes (None where that is 0)."""
+        self._attention("_window", _Window(window, sinks), stream, type, n_heads, n_seqs, n_tokens, max_q, max_kv, scale,
+                        _ptr(q), q_stride, _ptr(out), out_stride, _ptr(q_start), _ptr(kv_len), _ptr(tables), table_width,
+                        _ptr(work), 0 if work is None else work.nbytes)
+
+    def attention_prefix_work(self, n_heads: int, n_seqs: int, n_tokens: int, n_groups: int, max_prefix: int = 0,
+                              table_width: Optional[int] = None, max_q: int = 0, max_kv: int = 0) -> int:
+        """``attention_work`` of an ``attention_prefix`` call."""
+        return self._work("_prefix", _Prefix(n_groups, max_prefix), n_heads, n_seqs, n_tokens, table_width, max_q, max_kv)
+
+    def attention_prefix(self, q, out, n_heads: int, q_start, kv_len, tables, n_seqs: int, n_tokens: int,
+                         table_width: int, group_start, prefix_len, n_groups: int, max_prefix: int = 0, max_q: int = 0,
+                         max_kv: int = 0, scale: float = 0.0, type: int = F32, q_stride: int = 0, out_stride: int = 0,
+                         work=None, stream: int = 0) -> None:
+        """icua_paged_attention_prefix: sequences ``group_start[g]`` .. ``group_start[g + 1]`` - 1 share their first
+        ``prefix_len[g]`` slots, which are read once; ``work`` has ``attention_prefix_work`` bytes (None where that is
+        0)."""
+        self._attention("_prefix", _Prefix(n_groups, max_prefix, _ptr(group_start), _ptr(prefix_len)), stream, type,
+                        n_heads, n_seqs, n_tokens, max_q, max_kv, scale, _ptr(q), q_stride, _ptr(out), out_stride,
+                        _ptr(q_start), _ptr(kv_len), _ptr(tables), table_width, _ptr(work), 0 if work is None else work.nbytes)
 
     def load(self, slots, n_rows: int, k=None, v=None, type: int = F32, token_stride: int = 0, head_stride: int = 0,
              stream: int = 0) -> None:
