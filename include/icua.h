@@ -226,8 +226,8 @@ enum { ICUA_TYPE_F32 = 0, ICUA_TYPE_F16 = 1 };
  * quantised to 8 bits as they come, matrices once (each output channel is a row of icua_i8_quantize, without a norm).
  * The calls enqueue on `stream` (a hipStream_t; NULL: the null stream) and return without waiting; they allocate
  * nothing, keep nothing and can be captured into a graph.  Buffers and stream belong to the current device.
- * Arguments are checked before anything is enqueued.  Row strides are in values (0: dense); the buffers of one call
- * do not overlap but where it is said. */
+ * Arguments are checked before anything is enqueued.  Row strides are in values (0: dense), at most 2^22; the buffers
+ * of one call do not overlap but where it is said. */
 
 /* Codes and scales of rows: y = x / sqrt(mean(x^2) + eps) * norm (norm NULL: y = x, eps is not used),
  *   scale = max |y| / 127,  code = 127 y / max |y|, rounded to the nearest, ties to even:
@@ -236,7 +236,7 @@ enum { ICUA_TYPE_F32 = 0, ICUA_TYPE_F16 = 1 };
  * Scales beyond fp32's range become 0 or infinite. */
 typedef struct {
     int32_t type;            /* ICUA_TYPE_* of x */
-    int32_t n_rows;          /* 0: nothing to do */
+    int32_t n_rows;          /* at most 2^24; 0: nothing to do */
     int32_t n_cols;          /* a positive multiple of 16, at most 2^17 */
     const void* x;           /* [n_rows] rows, aligned to 16 bytes; x_stride a multiple of 8 */
     int64_t x_stride;
@@ -257,7 +257,7 @@ int icua_i8_quantize(const icua_i8_quantize_t* args, void* stream);
 typedef struct {
     int32_t type;            /* ICUA_TYPE_* of y */
     int32_t gated;           /* 0 or 1; not together with add */
-    int32_t n_rows, n_out;   /* tokens and output channels (0: nothing to do), n_rows * n_out <= 2^36 */
+    int32_t n_rows, n_out;   /* tokens, at most 2^24, and output channels, at most 2^22 (0: nothing to do); n_rows * n_out <= 2^36 */
     int32_t n_in;            /* a positive multiple of 16, at most 2^17 */
     const int8_t* x;         /* [n_rows] rows of codes, -127 .. 127, aligned to 16 bytes; x_stride a multiple of 16 */
     int64_t x_stride;

@@ -1944,12 +1944,14 @@ int icua_paged_load(const icua_pages_t* pages, const icua_paged_load_t* args, vo
 
 // ---- products on 8-bit integers
 
-constexpr int I8_MAX_IN = 1 << 17;  // sums of products of codes stay below 2^31
+constexpr int I8_MAX_IN = 1 << 17;      // sums of products of codes stay below 2^31
+constexpr int I8_MAX_STRIDE = 1 << 22;  // a tile's 256 rows lie within 2^31 bytes
 
 // A row stride of `width` values (0: dense) in multiples of `of`.
 static int i8_stride(const std::string& what, int64_t& stride, int64_t width, int of) {
     if (stride == 0) stride = width;
-    if (stride < width || stride % of) return fail(what + " must be at least a row" + (of > 1 ? " and a multiple of " + std::to_string(of) + " values" : ""));
+    if (stride < width || stride % of || stride > I8_MAX_STRIDE)
+        return fail(what + " must be at least a row" + (of > 1 ? ", a multiple of " + std::to_string(of) + " values" : "") + " and at most 2^22");
     return 0;
 }
 // Whether [p, p + bytes) and [q, q + more) overlap.
@@ -1962,7 +1964,7 @@ static __int128 span(int64_t rows, int64_t stride, int64_t width, int size) { re
 int icua_i8_quantize(const icua_i8_quantize_t* args, void* stream) {
     if (!args) return fail("i8_quantize: null argument");
     if (!type_ok(args->type)) return fail("i8_quantize: bad type");
-    if (args->n_rows < 0) return fail("i8_quantize: negative n_rows");
+    if (args->n_rows < 0 || args->n_rows > (1 << 24)) return fail("i8_quantize: n_rows must be in 0..2^24");
     if (args->n_cols < 16 || args->n_cols % 16 || args->n_cols > I8_MAX_IN) return fail("i8_quantize: n_cols must be a positive multiple of 16, at most 2^17");
     I8QuantArgs a{};
     a.n_rows = args->n_rows;
@@ -1996,7 +1998,8 @@ static int i8_matmul_sizes(const icua_i8_matmul_t* args, I8MatmulArgs& a) {
     if (!type_ok(args->type)) return fail("i8_matmul: bad type");
     if (args->gated != 0 && args->gated != 1) return fail("i8_matmul: gated must be 0 or 1");
     if (args->n_rows < 0 || args->n_out < 0) return fail("i8_matmul: negative size");
-    if (args->n_out > (1 << 30) || (int64_t)args->n_rows * args->n_out > ((int64_t)1 << 36)) return fail("i8_matmul: more than 2^30 channels or 2^36 outputs");
+    if (args->n_rows > (1 << 24) || args->n_out > I8_MAX_STRIDE || (int64_t)args->n_rows * args->n_out > ((int64_t)1 << 36))
+        return fail("i8_matmul: more than 2^24 rows, 2^22 channels or 2^36 outputs");
     if (args->n_in < 16 || args->n_in % 16 || args->n_in > I8_MAX_IN) return fail("i8_matmul: n_in must be a positive multiple of 16, at most 2^17");
     a.n_rows = args->n_rows;
     a.n_out = args->n_out;

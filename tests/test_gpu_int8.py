@@ -168,6 +168,10 @@ SHAPES = [
     (64, 128, 6144, 0), (65, 63, 4096, 0), (100, 257, 112, 0), (127, 255, 384, 2), (128, 256, 2048, 0),
     (129, 513, 528, 0), (200, 2048, 2048, 0), (257, 300, 1024, 1), (400, 777, 240, 0), (1000, 96, 512, 0),
     (1111, 1300, 640, 0), (2048, 2050, 256, 0), (4, 3, 1 << 17, 0), (130, 2, 20000, 0),
+    # With those before, every tile of the products: whole ones, ragged ones, ends of 16 to 112 codes.
+    (36, 1478, 400, 1), (24, 2050, 1040, 0), (150, 17, 688, 0), (2, 9193, 1040, 1), (200, 2050, 2064, 0), (33, 8284, 1040, 0),
+    (250, 2050, 2064, 3), (3, 16659, 2480, 0), (66, 17549, 144, 1), (512, 4096, 272, 0), (1030, 6150, 400, 0), (131, 35815, 80, 0),
+    (1024, 6144, 256, 0), (67, 839, 144, 0), (130, 17037, 112, 1), (300, 6100, 336, 0),
 ]
 
 

@@ -29,7 +29,7 @@ def library():
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(type=2), "type"), (dict(type=-1), "type"), (dict(n_rows=-1), "negative"), (dict(n_cols=0), "n_cols"),
+    (dict(type=2), "type"), (dict(type=-1), "type"), (dict(n_rows=-1), "n_rows"), (dict(n_rows=(1 << 24) + 1), "n_rows"), (dict(n_cols=0), "n_cols"), (dict(x_stride=(1 << 22) + 8), "x_stride"),
     (dict(n_cols=24), "n_cols"), (dict(n_cols=-16), "n_cols"), (dict(n_cols=(1 << 17) + 16), "n_cols"),
     (dict(x_stride=2040), "x_stride"), (dict(x_stride=2052), "x_stride"), (dict(codes_stride=2032), "codes_stride"),
     (dict(codes_stride=2056), "codes_stride"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
@@ -47,7 +47,8 @@ def test_quantize_refuses(kw, match):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(type=2), "type"), (dict(gated=2), "gated"), (dict(n_rows=-1), "negative"), (dict(n_out=-1), "negative"),
-    (dict(n_out=(1 << 30) + 1), "2\\^30"), (dict(n_rows=1 << 20, n_out=(1 << 16) + 1), "2\\^36"), (dict(n_in=0), "n_in"),
+    (dict(n_out=(1 << 22) + 1), "2\\^22"), (dict(n_rows=1 << 20, n_out=(1 << 16) + 1), "2\\^36"),
+    (dict(n_rows=(1 << 24) + 1), "2\\^24"), (dict(x_stride=(1 << 22) + 16), "x_stride"), (dict(y_stride=(1 << 22) + 1), "y_stride"), (dict(n_in=0), "n_in"),
     (dict(n_in=2040), "n_in"), (dict(n_in=(1 << 17) + 16), "n_in"), (dict(x_stride=2032), "x_stride"),
     (dict(x_stride=2056), "x_stride"), (dict(w_stride=16), "w_stride"), (dict(w_stride=2050), "w_stride"),
     (dict(add_stride=99), "add_stride"), (dict(y_stride=99), "y_stride"), (dict(gated=True, add=At(7 * G)), "gated"),
