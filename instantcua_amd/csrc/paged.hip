@@ -430,49 +430,42 @@ __device__ __forceinline__ float row_value(const void* v, const void* v_sb, int6
     return h2f(((const uint16_t*)v_sb)[row * NG + d / QG]) * (float)((const int8_t*)v)[row * HD + d];
 }
 
-// What the kernels deal out are spans: rows of query tokens and the slots that they go through.  Every sequence is
-// one.  With a window it leaves out the slots between the first ones and those of its first row's window.  With
-// prefixes the groups' are spans too, in front of the sequences': the rows of all the group's tokens over the shared
-// slots, read once for all of them; the sequences then begin behind those, and a row's two parts are joined.
-template <int FORM>
-__device__ __forceinline__ int n_spans(const PagedAttnArgs& a) { return a.n_seqs + (FORM == PAGED_PREFIX ? a.f.n_groups : 0); }
+// The slots that a sequence goes through: with a window all but those between the first ones and its first row's
+// window; behind a shared prefix those after it.  The prefix itself is gone through once for the rows of all the
+// group's tokens (the chunk kernel's first workgroups), and a row's two parts are joined.
 
-// Lane g: group g.
+// Lane g: group g.  (Its loads, and those of span_of, are of places inside the arrays whether they count or not, so
+// that they are all under way together.)
 template <int FORM>
 __device__ __forceinline__ PrefixGroup load_groups(const PagedAttnArgs& a) {
-    PrefixGroup y = {0, 0, 0};
-    if constexpr (FORM == PAGED_PREFIX) {
-        const int g = threadIdx.x & 63;
-        if (g < a.f.n_groups) y = prefix_group(a.group_start, a.prefix_len, g, a.n_seqs, a.f.max_prefix);
-    }
+    if constexpr (FORM != PAGED_PREFIX) return {0, 0, 0};
+    const int g = threadIdx.x & 63;
+    PrefixGroup y = prefix_group(a.group_start, a.prefix_len, min(g, a.f.n_groups - 1), a.n_seqs, a.f.max_prefix);
+    if (g >= a.f.n_groups) y = {0, 0, 0};
     return y;
 }
 struct Span {
-    SeqSpan sp;   // n_kv: of a prefix its slots
+    SeqSpan sp;
     SlotGap gap;  // (a 128-row tile of a window has its own)
     __device__ __forceinline__ int slots() const { return max(0, sp.n_kv - gap.skip); }
 };
-// Lane i's span s0 + i, up to `end`.  (s0 is 0 where there are groups among them: group g is lane g's.)
+// Lane i: sequence s0 + i.
 template <int FORM>
-__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, const PrefixGroup& gr, int s0, int end) {
-    const int i = s0 + (threadIdx.x & 63);
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, const PrefixGroup& gr, int s0) {
+    const int s = s0 + (int)(threadIdx.x & 63);
     Span y = {{0, 0, 0}, {0, 0}};
-    if constexpr (FORM != PAGED_PREFIX) {
-        if (i < end) y.sp = seq_span(a.q_start, a.kv_len, i, a.n_tokens, a.max_kv);
-        if constexpr (FORM == PAGED_WINDOW) y.gap = window_gap(y.sp.n_kv - y.sp.n_q, y.sp.n_kv, a.f.window, a.f.sinks, 32);
-    } else {
-        const bool pre = i < a.f.n_groups, there = i < end;
-        const int s = i - a.f.n_groups;
-        if (there && !pre) y.sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
+    if constexpr (FORM == PAGED_ALL) {
+        if (s < a.n_seqs) y.sp = seq_span(a.q_start, a.kv_len, s, a.n_tokens, a.max_kv);
+        return y;
+    }
+    y.sp = seq_span(a.q_start, a.kv_len, min(s, a.n_seqs - 1), a.n_tokens, a.max_kv);
+    if (s >= a.n_seqs) y.sp = {0, 0, 0};
+    if constexpr (FORM == PAGED_WINDOW) y.gap = window_gap(y.sp.n_kv - y.sp.n_q, y.sp.n_kv, a.f.window, a.f.sinks, 32);
+    if constexpr (FORM == PAGED_PREFIX)
         for (int g = 0; g < a.f.n_groups; ++g) {
             const int n = __builtin_amdgcn_readlane(gr.n, g), first = __builtin_amdgcn_readlane(gr.s0, g), last = __builtin_amdgcn_readlane(gr.s1, g);
-            if (n && !pre && s >= first && s < last) y.gap.skip = n;
+            if (n && s >= first && s < last) y.gap.skip = n;
         }
-        if (there && pre && gr.n) {
-            const int t0 = min(max(a.q_start[gr.s0], 0), a.n_tokens), t1 = min(max(a.q_start[gr.s1], t0), a.n_tokens);
-            y.sp = {t0, t1 - t0, gr.n};
-        }
-    }
     return y;
 }
 // The last slot of a prefix of n slots that this lane's token t sees; true if all tokens of the group's sequences
@@ -504,10 +497,11 @@ __device__ __forceinline__ bool prefix_last(const PagedAttnArgs& a, int s0, int 
 // half again as long for lengths that differ by factors of up to 8.
 constexpr int ROWS_TILE = 16, ROWS_STEP = 32;
 constexpr int ROWS_PITCH = 80;  // 16-byte places of a wave's results of one dt
+// Of the forms with a gap each wave keeps its 64 sequences in LDS, not in registers: places of `kept` and `more`.
 template <int NW>
-constexpr size_t rows_lds() { return NW * (8 * ROWS_PITCH * 16 + 16 * 8); }
+constexpr size_t rows_lds(int form) { return NW * (8 * ROWS_PITCH * 16 + 16 * 8 + (form == PAGED_ALL ? 0 : WAVE * 32)); }
 
-// Lane i: span s0 + i, its units (0: the chunk kernel's, or none) and those up to its end since s0; `sum`:
+// Lane i: sequence s0 + i, its units (0: the chunk kernel's, or none) and those up to its end since s0; `sum`:
 // of all 64.
 struct FewUnits {
     Span x;
@@ -515,15 +509,15 @@ struct FewUnits {
 };
 template <int FORM>
 __device__ __forceinline__ FewUnits few_units(const PagedAttnArgs& a, const PrefixGroup& gr, int group, int s0) {
-    const int lane = threadIdx.x & 63, spans = n_spans<FORM>(a);
-    FewUnits u = {span_of<FORM>(a, gr, s0, spans), 0, 0, 0};
+    const int lane = threadIdx.x & 63;
+    FewUnits u = {span_of<FORM>(a, gr, s0), 0, 0, 0};
     if (u.x.sp.n_q > 0 && u.x.sp.n_q * group <= ROWS_TILE) u.n = max(1, (u.x.slots() + a.few.unit - 1) / a.few.unit);
     u.end = u.n;
-    for (int o = 1; o < min(WAVE, spans); o <<= 1) {
+    for (int o = 1; o < min(WAVE, a.n_seqs); o <<= 1) {
         const int y = __shfl_up(u.end, o);
         if (lane >= o) u.end += y;
     }
-    u.sum = __builtin_amdgcn_readlane(u.end, min(WAVE, spans) - 1);
+    u.sum = __builtin_amdgcn_readlane(u.end, min(WAVE, a.n_seqs) - 1);
     return u;
 }
 // Units a workgroup takes, of this many.
@@ -549,48 +543,57 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
     float2* const sml = (float2*)(lds + NW * 8 * ROWS_PITCH * 16);  // [NW][16]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
     const int g = index % a.map.n_kv, w = index / a.map.n_kv, group = a.n_heads / a.map.n_kv;
-    const PrefixGroup gr = load_groups<FORM>(a);
-    const int spans = n_spans<FORM>(a);
-    FewUnits u = few_units<FORM>(a, gr, group, 0);
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    i32x4* const kept = (i32x4*)(lds + NW * (8 * ROWS_PITCH * 16 + 16 * 8)) + wave * 2 * WAVE;  // (t0, n_q, n_kv, units)
+    i32x4* const more = kept + WAVE;                                                           // (units up to its end, gap)
+    FewUnits u;
+    PrefixGroup gr = load_groups<FORM>(a);
+    auto keep = [&]() __attribute__((always_inline)) {
+        if constexpr (FORM != PAGED_ALL) {
+            kept[lane] = i32x4{u.x.sp.t0, u.x.sp.n_q, u.x.sp.n_kv, u.n};
+            more[lane] = i32x4{u.end, u.x.gap.from, u.x.gap.skip, 0};
+        }
+    };
+    u = few_units<FORM>(a, gr, group, 0);
     int total = u.sum;
-    for (int s0 = WAVE; s0 < spans; s0 += WAVE) total += few_units<FORM>(a, gr, group, s0).sum;
+    for (int s0 = WAVE; s0 < a.n_seqs; s0 += WAVE) total += few_units<FORM>(a, gr, group, s0).sum;
     const int per = few_per(a, total), end = min(total, (w + 1) * per);
+    keep();
     int pos = w * per, s0 = 0, before = 0;
     while (pos < end) {
         // The sequence that has unit pos, and where its units begin.
-        const uint64_t past = __ballot(before + u.end > pos);
+        const uint64_t past = __ballot(before + (FORM == PAGED_ALL ? u.end : more[lane][0]) > pos);
         if (!past) {
             before += u.sum;
             s0 += WAVE;
-            if (s0 >= spans) return;
+            if (s0 >= a.n_seqs) return;
+            gr = load_groups<FORM>(a);
             u = few_units<FORM>(a, gr, group, s0);
+            keep();
             continue;
         }
-        const int at_lane = __ffsll((unsigned long long)past) - 1, seq_end = before + __builtin_amdgcn_readlane(u.end, at_lane);
-        const int seq_units = __builtin_amdgcn_readlane(u.n, at_lane), first = pos - (seq_end - seq_units), count = min(end, seq_end) - pos;
-        const SeqSpan sp = {__builtin_amdgcn_readlane(u.x.sp.t0, at_lane), __builtin_amdgcn_readlane(u.x.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.x.sp.n_kv, at_lane)};
-        const bool whole = count == seq_units;
-        pos += count;
-        RowOf row = row_of(sp, r16, group, g);
-        // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.  (Of a window: and those of its own.)
-        const int start = first * a.few.unit;
-        const int lim = sp.n_kv;
-        int all = sp.n_kv - sp.n_q;
-        SlotGap gap = {0, 0};
-        int seq = s0 + at_lane;
-        bool pre = false, joined = false;
-        if constexpr (FORM != PAGED_ALL) gap = {__builtin_amdgcn_readlane(u.x.gap.from, at_lane), __builtin_amdgcn_readlane(u.x.gap.skip, at_lane)};
-        if constexpr (FORM == PAGED_PREFIX) {
-            pre = seq < a.f.n_groups;
-            joined = pre || gap.skip > 0;
-            if (pre) {
-                const int g0 = __builtin_amdgcn_readlane(gr.s0, seq), g1 = __builtin_amdgcn_readlane(gr.s1, seq);
-                all = prefix_last(a, g0, g1, lim, row.t, row.last) ? lim - 1 : -1;
-                seq = g0;
-            } else {
-                seq -= a.f.n_groups;
+        const int at_lane = __ffsll((unsigned long long)past) - 1;
+        i32x4 k = {}, x = {};
+        if constexpr (FORM == PAGED_ALL) {
+            k = i32x4{__builtin_amdgcn_readlane(u.x.sp.t0, at_lane), __builtin_amdgcn_readlane(u.x.sp.n_q, at_lane), __builtin_amdgcn_readlane(u.x.sp.n_kv, at_lane), __builtin_amdgcn_readlane(u.n, at_lane)};
+            x[0] = __builtin_amdgcn_readlane(u.end, at_lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                k[i] = __builtin_amdgcn_readfirstlane(kept[at_lane][i]);
+                x[i] = __builtin_amdgcn_readfirstlane(more[at_lane][i]);
             }
         }
+        const int seq_end = before + x[0], seq_units = k[3], first = pos - (seq_end - seq_units), count = min(end, seq_end) - pos;
+        const SeqSpan sp = {k[0], k[1], k[2]};
+        const bool whole = count == seq_units;
+        pos += count;
+        const RowOf row = row_of(sp, r16, group, g);
+        // Slots that some row sees: 0 .. lim - 1; all of them see those up to `all`.  (Of a window: and those of its own.)
+        const int start = first * a.few.unit;
+        const int lim = sp.n_kv, all = sp.n_kv - sp.n_q;
+        const SlotGap gap = {FORM == PAGED_WINDOW ? x[1] : 0, x[2]};
+        const bool joined = FORM == PAGED_PREFIX && gap.skip > 0;  // to its prefix's part
         const int c1 = min(FORM == PAGED_ALL ? lim : max(0, lim - gap.skip), start + count * a.few.unit);  // of numbers without the gap
         // Whether this lane's row sees a slot, and whether no row does.  (Without short cuts: selects, no branches.
         // With them the compiler, ROCm 7.2's, left out the select of -inf for slots before the window.)
@@ -602,7 +605,7 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
             if constexpr (FORM != PAGED_WINDOW) return false;
             return (slot >= a.f.sinks) & (slot <= all - a.f.window);
         };
-        const int32_t* table = a.tables + (int64_t)seq * a.table_width;
+        const int32_t* table = a.tables + (int64_t)(s0 + at_lane) * a.table_width;
         // Lane i: the pool row of tile i % 2 of this wave's step i / 2 from `sub` on (-1: no such page).
         auto step_slot = [&](int sub, int i) { return sub + ROWS_STEP * (wave + NW * i); };
         auto lookup = [&](int sub) {
@@ -813,8 +816,7 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
             const float inv = partial ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
             int64_t part = ((int64_t)index * 2 + (first == 0)) * a.few.rows + orow;
             if (joined && whole) {
-                const int64_t out_row = (int64_t)out.t * a.n_heads + out.head;
-                part = pre ? a.pre_at + out_row * a.pre.n : a.part_at + out_row * a.big.n;
+                part = a.part_at + ((int64_t)out.t * a.n_heads + out.head) * a.big.n;
             }
 #pragma unroll
             for (int k = 0; k < DIMS; k += 4) {
@@ -831,7 +833,7 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
 
 template <int FORM, int TYPE, int FMT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows_kernel(PagedAttnArgs a) {
-    __shared__ __align__(16) uint8_t lds[rows_lds<4>()];
+    __shared__ __align__(16) uint8_t lds[rows_lds<4>(FORM)];
     rows_work<FORM, TYPE, FMT, 4>(a, blockIdx.x, lds);
 }
 
@@ -880,14 +882,12 @@ __device__ __forceinline__ f32x16 mfma32(v8h a, v8h b, f32x16 c) { return __buil
 // and takes those with the most slots first, so that the last workgroups to run are short.  Every workgroup
 // looks through the sequences before its own, so a batch's time has a part that grows with their square:
 // 9 tokens over 200 slots of each of 1024 sequences 0.65 ms, of 16384 (the most in a call) 49 ms.
-//
-// Of the spans first .. end - 1.
 template <int FORM>
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, const PrefixGroup& gr, int first, int end, int group, int rows, int index, int& s, int& tile, int& tiles, Span& span) {
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, const PrefixGroup& gr, int group, int rows, int index, int& s, int& tile, int& tiles, Span& span) {
     const int lane = threadIdx.x & 63;
-    for (int s0 = first; s0 < end; s0 += WAVE) {
-        const int count = min(WAVE, end - s0);
-        const Span x = span_of<FORM>(a, gr, s0, end);
+    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
+        const int count = min(WAVE, a.n_seqs - s0);
+        const Span x = span_of<FORM>(a, gr, s0);
         const int n = x.sp.n_q * group > ROWS_TILE ? (x.sp.n_q * group + rows - 1) / rows : 0, slots = FORM == PAGED_PREFIX ? x.slots() : x.sp.n_kv;
         int sum = n;
 #pragma unroll
@@ -897,7 +897,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, const PrefixGr
             index -= sum;
             continue;
         }
-        int begin = 0;  // tiles of the spans that come before lane's
+        int begin = 0;  // tiles of the sequences that come before lane's
         for (int j = 0; j < count; ++j) {
             const int kv = __builtin_amdgcn_readlane(slots, j), add = __builtin_amdgcn_readlane(n, j);
             if (kv > slots || (kv == slots && j < lane)) begin += add;
@@ -914,6 +914,28 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, const PrefixGr
     return false;
 }
 
+// The same for the groups' tokens over their prefixes: the group's first sequence and the one behind its last.
+__device__ __forceinline__ bool find_prefix_tile(const PagedAttnArgs& a, const PrefixGroup& gr, int group, int index, int& s0, int& s1, int& tile, int& tiles, Span& span) {
+    int t0 = 0, t1 = 0;
+    if (gr.n) {
+        t0 = min(max(a.q_start[gr.s0], 0), a.n_tokens);
+        t1 = min(max(a.q_start[gr.s1], t0), a.n_tokens);
+    }
+    const int n = ((t1 - t0) * group + CH_ROWS - 1) / CH_ROWS;
+    for (int g = 0; g < a.f.n_groups; ++g) {
+        tiles = __builtin_amdgcn_readlane(n, g);
+        if (index < tiles) {
+            s0 = __builtin_amdgcn_readlane(gr.s0, g);
+            s1 = __builtin_amdgcn_readlane(gr.s1, g);
+            tile = index;
+            span = {{__builtin_amdgcn_readlane(t0, g), __builtin_amdgcn_readlane(t1, g) - __builtin_amdgcn_readlane(t0, g), __builtin_amdgcn_readlane(gr.n, g)}, {0, 0}};
+            return true;
+        }
+        index -= tiles;
+    }
+    return false;
+}
+
 template <int FORM, int TYPE, int FMT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
     constexpr bool HL = TYPE == TYPE_F32, CODES = FMT == FMT_Q8;
@@ -922,8 +944,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int *const tile_there = tile_odd + 16, *const tile_top = tile_odd + 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
-    // The first workgroups have the shared prefixes, the last ones the spans of few rows: they are short, and bound
-    // by memory.
+    // The first workgroups have the shared prefixes, the last ones the sequences of few rows: they are short, and
+    // bound by memory.
     int index = blockIdx.x;
     bool pre = false;
     PagedSplit parts = a.big;
@@ -941,10 +963,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % parts.n;
     const PrefixGroup gr = load_groups<FORM>(a);
-    const int first_span = FORM != PAGED_PREFIX || pre ? 0 : a.f.n_groups, end_span = pre ? a.f.n_groups : n_spans<FORM>(a);
-    int s, tile, tiles;
+    int s, tile, tiles, group_s1 = 0;
     Span span;
-    if (!find_tile<FORM>(a, gr, first_span, end_span, group, CH_ROWS, at / parts.n, s, tile, tiles, span)) return;
+    if (!(pre ? find_prefix_tile(a, gr, group, at / parts.n, s, group_s1, tile, tiles, span) : find_tile<FORM>(a, gr, group, CH_ROWS, at / parts.n, s, tile, tiles, span))) return;
     tile = tiles - 1 - tile;  // those that see the most slots first
     const SeqSpan sp = span.sp;
     const int before = sp.n_kv - sp.n_q;  // token i sees slots up to before + i
@@ -955,7 +976,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
     RowOf row = row_of(sp, r0 + c32, group, g);
     // Iterations are of 128 slots, numbered without those that are skipped.
-    int it_from = 0, it_skip = 0, group_s1 = 0;
+    int it_from = 0, it_skip = 0;
     bool joined = false;
     if constexpr (FORM == PAGED_WINDOW) {
         const SlotGap gap = window_gap(all_seen, lim, a.f.window, a.f.sinks, 128);
@@ -966,13 +987,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         it_skip = span.gap.skip / 128;
         joined = pre || it_skip > 0;
         if (pre) {
-            group_s1 = __builtin_amdgcn_readlane(gr.s1, s);
-            s = __builtin_amdgcn_readlane(gr.s0, s);
             lim = sp.n_kv;
             w_first = w_last = all_seen = lim - 1;
             row.last = lim - 1;
-        } else {
-            s -= a.f.n_groups;
         }
     }
     auto first_slot = [&](int it) __attribute__((always_inline)) { return (FORM == PAGED_ALL || it < it_from ? it : it + it_skip) * 128; };
@@ -1156,7 +1173,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         look_at_pages(max(c0, 128 * it_from) + 128 * it_skip, c1 + 128 * it_skip);
     }
     if constexpr (FORM == PAGED_PREFIX)
-        if (pre && !prefix_last(a, s, group_s1, lim, row.t, row.last)) w_first = all_seen = -1;
+        if (pre && !prefix_last(a, s, group_s1, lim, row.t, row.last)) w_first = all_seen = __builtin_amdgcn_readfirstlane(-1);
     if (it0 < it1) staged(it0);
 
     f32x16 O[4];
@@ -1576,15 +1593,15 @@ __device__ __forceinline__ void merge_row(const PagedAttnArgs& a, int t, int hea
     if (lane < 32) store4<TYPE>(a.out, (int64_t)t * a.out_stride + head * HD + d, o * inv);
 }
 
-// The workgroups of a KV head that share few-row span s: `n` of them from w0 on.
+// The workgroups of a KV head that share few-row sequence s: `n` of them from w0 on.
 struct FewParts {
     int w0, n;
 };
 template <int FORM>
 __device__ __forceinline__ FewParts few_parts(const PagedAttnArgs& a, const PrefixGroup& gr, int s) {
     const int group = a.n_heads / a.map.n_kv;
-    int total = 0, begin = 0, n = 0;  // units of all spans, those before s, its own
-    for (int s0 = 0; s0 < n_spans<FORM>(a); s0 += WAVE) {
+    int total = 0, begin = 0, n = 0;  // units of all sequences, those before s, its own
+    for (int s0 = 0; s0 < a.n_seqs; s0 += WAVE) {
         const FewUnits u = few_units<FORM>(a, gr, group, s0);
         if (s >= s0 && s < s0 + WAVE) {
             n = __builtin_amdgcn_readlane(u.n, s - s0);
@@ -1621,37 +1638,25 @@ __global__ __launch_bounds__(256) void paged_merge_rows_kernel(PagedAttnArgs a) 
     merge_few<FORM, TYPE>(a, s, sp, g, r);
 }
 
-// Row (t, head) of sequence s with prefixes: the partials of its group's, then its own.  Those of a span that one
-// workgroup has done are in its place in `part`.
+// Row (t, head) of sequence s with prefixes: the partials of its group's, then its own.  Those of a few-row sequence
+// that one workgroup has done are in its place in `part`.
 template <int TYPE>
 __device__ __forceinline__ void merge_prefix(const PagedAttnArgs& a, int t, int head, int s, const SeqSpan& sp) {
-    const int lane = threadIdx.x & 63, group = a.n_heads / a.map.n_kv, g = head / group;
+    const int lane = threadIdx.x & 63, group = a.n_heads / a.map.n_kv;
     const int64_t row = (int64_t)t * a.n_heads + head;
     const PrefixGroup gr = load_groups<PAGED_PREFIX>(a);
-    const uint64_t in = __ballot(lane < a.f.n_groups && gr.n > 0 && s >= gr.s0 && s < gr.s1);
-    FewParts pre = {0, 0}, own = {0, a.big.n};
-    bool pre_few = false;
-    const bool own_few = sp.n_q * group <= ROWS_TILE;
-    int pre_r = 0;
-    if (in) {
-        const int i = 63 - __clzll((long long)in);  // the last one that has it, as span_of takes it
-        const Span x = span_of<PAGED_PREFIX>(a, gr, 0, a.f.n_groups);
-        const int t0 = __builtin_amdgcn_readlane(x.sp.t0, i), n_q = __builtin_amdgcn_readlane(x.sp.n_q, i);
-        pre_few = n_q * group <= ROWS_TILE;
-        pre = {0, a.pre.n};
-        pre_r = min(max((t - t0) * group + head % group, 0), a.few.rows - 1);  // (of starts that rise: as it is)
-        if (pre_few) pre = few_parts<PAGED_PREFIX>(a, gr, i);
-    }
-    if (own_few)
-        own = few_parts<PAGED_PREFIX>(a, gr, a.f.n_groups + s);
+    const bool few = sp.n_q * group <= ROWS_TILE;
+    const int pre = __ballot(gr.n > 0 && s >= gr.s0 && s < gr.s1) ? a.pre.n : 0;
+    FewParts own = {0, a.big.n};
+    if (few)
+        own = few_parts<PAGED_PREFIX>(a, gr, s);
     else if (!a.tiles)
         return;  // more tokens than max_q
-    if (!in && own.n < 2) return;  // written already
-    const int own_r = (t - sp.t0) * group + head % group;
-    merge_row<TYPE>(a, t, head, a.few_part, a.few_ml, pre.n + own.n, [&](int i) {
-        if (i < pre.n) return pre_few && pre.n > 1 ? few_at(a, pre, g, pre_r, i) : a.pre_at + row * a.pre.n + i;
-        i -= pre.n;
-        return own_few && own.n > 1 ? few_at(a, own, g, own_r, i) : a.part_at + row * a.big.n + i;
+    if (!pre && own.n < 2) return;  // written already
+    merge_row<TYPE>(a, t, head, a.few_part, a.few_ml, pre + own.n, [&](int i) {
+        if (i < pre) return a.pre_at + row * a.pre.n + i;
+        i -= pre;
+        return few && own.n > 1 ? few_at(a, own, head / group, (t - sp.t0) * group + head % group, i) : a.part_at + row * a.big.n + i;
     });
 }
 
@@ -1733,25 +1738,34 @@ static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, 
 PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv, const PagedFormSizes& f) {
     PagedPlan p{};
     const bool prefix = f.form == PAGED_PREFIX;
-    const int group = n_heads / n_kv, spans = n_seqs + (prefix ? f.n_groups : 0);
-    const int few = prefix ? ROWS_TILE : (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
+    const int group = n_heads / n_kv, few = (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
     const int max_splits = prefix ? PAGED_MAX_SPLITS / 2 : PAGED_MAX_SPLITS;  // a row has partials of two spans
     if (f.form == PAGED_WINDOW) max_kv = window_slots(max_kv, f.window, f.sinks);
     p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
     p.pre = {1, std::max(128, (f.max_prefix + 127) / 128 * 128)};
-    const bool big = (int64_t)max_q * group > ROWS_TILE, pre = prefix && (int64_t)n_tokens * group > ROWS_TILE;
-    if (pre) {
-        p.pre_tiles = (int)(((int64_t)n_tokens * group + 127 * std::min<int64_t>(f.n_groups, (int64_t)n_tokens * group / (ROWS_TILE + 1))) / CH_ROWS);
-        p.pre = split_slots((int64_t)p.pre_tiles * n_kv, 256, f.max_prefix, max_splits);
+    const bool big = (int64_t)max_q * group > ROWS_TILE;
+    if (prefix && n_tokens) {
+        // As many tiles as there may be; about half of a group's last one is in use.
+        const int64_t rows = (int64_t)n_tokens * group, groups = std::min<int64_t>(f.n_groups, rows);
+        const int64_t tiles = std::max<int64_t>(1, (rows + 63 * groups) / CH_ROWS), steps = (f.max_prefix + 127) / 128;
+        p.pre_tiles = (int)((rows + 127 * groups) / CH_ROWS);
+        // Beside few-row sequences a prefix's workgroups should end with them: of the CUs' time, at 2 us for 128 slots
+        // (q8 4) of a tile and 3 us for 256 slots of a sequence, half of the bound's, and 6 us to begin with, each
+        // takes its share less 8 us.  (64 tokens behind 7680 slots: 33 us with 8 or 10 ranges of slots, 36 with 6, 46
+        // with 30; over q8 60 with 8, 45 with 12 and 53 with 30.)
+        const double step = fmt == FMT_F16 ? 2. : 4., own = 6. + 1.5 * std::max(0, max_kv - f.max_prefix) / 256;
+        const double us = std::max(16., n_kv * (tiles * steps * step + n_seqs * own) / 256);
+        const int64_t ranges = big ? 256 / std::max<int64_t>(1, tiles * n_kv) : (int64_t)(steps * step / (us - 8.) + 0.999);
+        p.pre = split_slots(1, ranges, f.max_prefix, max_splits);
     }
     if (big) {
         p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
         p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv, max_splits);
     }
-    if (big || pre)
-        p.few = few_of(256, 8 * ROWS_STEP, INT32_MAX, n_kv, spans, few, max_kv, max_splits);
+    if (big || p.pre_tiles)  // (behind prefixes 384: 33 us where 256 take 37)
+        p.few = few_of(big ? 256 : 384, 8 * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     else
-        p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, spans, few, max_kv, max_splits);
+        p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     if (p.big.n > 1 || prefix) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
     if (prefix) p.pre_rows = (size_t)n_tokens * n_heads * p.pre.n;
     if (p.few.n > 1 && max_kv > p.few.unit) p.few_rows = (size_t)p.few.n * n_kv * 2 * few;
