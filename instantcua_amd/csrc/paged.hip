@@ -975,25 +975,22 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int all_seen = before + tile * CH_ROWS / group;  // slots up to this one all rows of the workgroup see
     int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
     RowOf row = row_of(sp, r0 + c32, group, g);
-    // Iterations are of 128 slots, numbered without those that are skipped.
-    int it_from = 0, it_skip = 0;
+    // Iterations are of 128 slots, numbered without those that are skipped, 64 or a multiple of it: a half of an
+    // iteration is a run of slots.  (Skipped 128 at a time, 16 first slots cost a window of 512 one iteration of 6.)
+    SlotGap gap = {0, 0};
     bool joined = false;
-    if constexpr (FORM == PAGED_WINDOW) {
-        const SlotGap gap = window_gap(all_seen, lim, a.f.window, a.f.sinks, 128);
-        it_from = gap.from / 128;
-        it_skip = gap.skip / 128;
-    }
+    if constexpr (FORM == PAGED_WINDOW) gap = window_gap(all_seen, lim, a.f.window, a.f.sinks, CH_HALF);
     if constexpr (FORM == PAGED_PREFIX) {
-        it_skip = span.gap.skip / 128;
-        joined = pre || it_skip > 0;
+        gap.skip = span.gap.skip;
+        joined = pre || gap.skip > 0;
         if (pre) {
             lim = sp.n_kv;
             w_first = w_last = all_seen = lim - 1;
             row.last = lim - 1;
         }
     }
-    auto first_slot = [&](int it) __attribute__((always_inline)) { return (FORM == PAGED_ALL || it < it_from ? it : it + it_skip) * 128; };
-    const int left = FORM == PAGED_ALL ? lim : max(0, lim - 128 * it_skip);
+    auto slot_of = [&](int v) __attribute__((always_inline)) { return FORM == PAGED_ALL ? v : FORM == PAGED_PREFIX ? v + gap.skip : gap_slot(gap, v); };
+    const int left = FORM == PAGED_ALL ? lim : max(0, lim - gap.skip);
     const int c0 = min(left, split * parts.chunk), c1 = min(left, c0 + parts.chunk);
     const int it0 = c0 / 128, it1 = c1 > c0 ? (c1 + 127) / 128 : it0;
     // A window's rows see slots from first_own on, those of this wave from w_low .. w_high, and the first ones.
@@ -1025,7 +1022,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             auto b = arguments();
             const PageMap map = {b->map.n_pages, b->map.n_kv, b->map.page_slots};
             sub = it;
-            const int slot = first_slot(sub + lane) + 16 * wave;
+            const int slot = slot_of((sub + lane) * 128 + 16 * wave);
             rows = slot < (FORM == PAGED_ALL ? c1 : lim) ? seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, slot) : -1;
         }
         return __builtin_amdgcn_readlane(rows, it - sub);
@@ -1041,7 +1038,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int j = 0; j < 4; ++j) src_off[j] = (4 * j + lane / 16) * (HD * 2) + (((lane & 15) ^ swizzle(4 * j + lane / 16)) << 4);
     auto copy = [&](int kv, int it, int r) __attribute__((always_inline)) {
-        const int n = r < 0 ? 0 : lim - (first_slot(it) + 16 * wave);
+        const int n = r < 0 ? 0 : lim - slot_of(it * 128 + 16 * wave);
         const uint32_t dst = lds0 + half_at(kv, it & 1, par) + wi * 16 * HD * 2;
         const uint8_t* src = (kv ? v_base : k_base) + (int64_t)(max(r, 0) + head_row) * (HD * 2);
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
@@ -1062,7 +1059,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     u32x4 codes[2][2];
     uint16_t scale[2] = {0, 0};
     auto fetch = [&](int kv, int it, int r) __attribute__((always_inline)) {
-        const int n = r < 0 ? 0 : lim - (first_slot(it) + 16 * wave);
+        const int n = r < 0 ? 0 : lim - slot_of(it * 128 + 16 * wave);
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
         codes[kv][0] = codes[kv][1] = u32x4{0, 0, 0, 0};
         scale[kv] = 0;
@@ -1169,8 +1166,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (FORM == PAGED_ALL) {
         look_at_pages(c0, c1);
     } else {
-        look_at_pages(c0, min(c1, 128 * it_from));
-        look_at_pages(max(c0, 128 * it_from) + 128 * it_skip, c1 + 128 * it_skip);
+        look_at_pages(c0, min(c1, gap.from));
+        look_at_pages(max(c0, gap.from) + gap.skip, c1 + gap.skip);
     }
     if constexpr (FORM == PAGED_PREFIX)
         if (pre && !prefix_last(a, s, group_s1, lim, row.t, row.last)) w_first = all_seen = __builtin_amdgcn_readfirstlane(-1);
@@ -1180,7 +1177,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
     float m = NEG_INF, l = 0.f;
-    auto base_of = [&](int it) __attribute__((always_inline)) { return first_slot(it) + CH_HALF * par; };
+    auto base_of = [&](int it) __attribute__((always_inline)) { return slot_of(it * 128 + CH_HALF * par); };
     // LDS addresses of operands in stage 0.  K of block 0: slot c32, dims 16 ks + 8 h .. + 7, at k_at ^ (ks <<
     // 5).  V^T: dims 32 dt + c32 of slots 4 h + {0 .. 3} (k = 1: + 8, the operand's other half), at v_at[k] ^
     // (dt << 6).  (A row's place in a stage is a multiple of its 256 bytes.)
@@ -1445,8 +1442,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // Whether some row of the workgroup does not see all of an iteration: of an f16 pool, all of its values are
     // made finite then, also for waves whose rows see them.
     auto cleaned = [&](int it) __attribute__((always_inline)) {
-        const int at = first_slot(it);
-        return at + 127 > all_seen || (FORM == PAGED_WINDOW && at + 127 >= a.f.sinks && at <= lim - 1 - a.f.window);
+        if constexpr (FORM != PAGED_WINDOW) return slot_of(it * 128) + 127 > all_seen;
+        bool some = false;
+        for (int half = 0; half < 2; ++half) {
+            const int at = slot_of(it * 128 + CH_HALF * half);
+            some |= (at + CH_HALF - 1 > all_seen) | ((at + CH_HALF > a.f.sinks) & (at <= lim - 1 - a.f.window));
+        }
+        return some;
     };
     // Values that are no numbers were kept out of the products: they go to the rows that see them.
     auto add_odd_values = [&](int it) __attribute__((always_inline)) {
@@ -1488,9 +1490,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         staged_barrier<63>();
     };
     // Iterations whose half some row of this wave sees.
-    int my1 = active && base_of(it0) <= w_last ? (w_last - CH_HALF * par) / 128 + 1 : it0;
-    if (FORM != PAGED_ALL && my1 > it_from) my1 = max(it_from, my1 - it_skip);
-    my1 = min(it1, my1);
+    const int v_last = FORM == PAGED_ALL || w_last < gap.from ? w_last : max(gap.from - 1, w_last - gap.skip);  // w_last's number
+    const int my1 = active && base_of(it0) <= w_last ? min(it1, (v_last - CH_HALF * par) / 128 + 1) : it0;
     for (int it = it0; it < it1; ++it) {
         staged_barrier<0>();
         if (it + 1 < it1) stage(it + 1);
@@ -1781,12 +1782,12 @@ static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
         if (e != hipSuccess) return e;
         const unsigned tiles = (unsigned)a.tiles * a.map.n_kv * a.big.n + (unsigned)a.pre_tiles * a.map.n_kv * a.pre.n;
         hipLaunchKernelGGL((paged_chunk_kernel<FORM, TYPE, FMT>), dim3(few + tiles), dim3(512), CH_LDS, s, a);
-    } else {
+    } else if constexpr (FORM != PAGED_PREFIX) {  // (prefixes have tiles)
         hipLaunchKernelGGL((paged_rows_kernel<FORM, TYPE, FMT>), dim3(few), dim3(256), 0, s, a);
     }
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.part || FORM == PAGED_PREFIX)
+    if (a.part)
         hipLaunchKernelGGL((paged_merge_kernel<FORM, TYPE>), dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a);
     else if (a.few_part)
         hipLaunchKernelGGL((paged_merge_rows_kernel<FORM, TYPE>), dim3((unsigned)a.n_seqs * a.map.n_kv, (unsigned)(a.few.rows + 3) / 4), dim3(256), 0, s, a);
