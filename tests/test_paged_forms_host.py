@@ -96,7 +96,7 @@ def test_what_a_window_goes_through(tmp_path):
 using namespace icua;
 int main() {
     const int lens[] = {0, 1, 2, 31, 32, 33, 127, 128, 129, 200, 256, 300, 511, 640, 1000};
-    for (int step : {32, 128})
+    for (int step : {32, 64, 128})
         for (int n : lens)
             for (int m : {1, 2, 16, 100, 128})
                 for (int window : {1, 2, 31, 32, 33, 64, 100, 128, 129, 255, 600, 1 << 30})
