@@ -279,6 +279,7 @@ struct PagedFew {
     int n, unit, least, twice;      // n workgroups a KV head, each with a share of `least` or more units of slots,
                                     // shares above `twice` doubled
     int rows;                       // upper bound of a sequence's query rows a KV head
+    int waves;                      // of a workgroup, where these sequences have a kernel of their own: 4 or 8
 };
 struct PagedPlan {
     PagedFew few;                   // sequences of at most 16 query rows a KV head

@@ -836,6 +836,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ __align__(16) uint8_t lds[rows_lds<4>(FORM)];
     rows_work<FORM, TYPE, FMT, 4>(a, blockIdx.x, lds);
 }
+// Eight waves a workgroup, for whole sequences.
+template <int FORM, int TYPE, int FMT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_rows8_kernel(PagedAttnArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    rows_work<FORM, TYPE, FMT, 8>(a, blockIdx.x, lds);
+}
 
 // Sequences with more query rows: 128 rows of a (sequence, KV head) a workgroup, eight waves.  Wave w has
 // rows 32 (w & 3) .. + 31 and of each 128 slots the half w >> 2; the two halves keep softmax states of their
@@ -1733,7 +1739,7 @@ static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv, int max_
 static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, int rows, int max_kv, int max_splits) {
     const int most = std::max(1, (max_kv + unit - 1) / unit);
     const int n = (int)std::min(std::max<int64_t>(1, want / n_kv), (int64_t)n_seqs * most);
-    return {n, unit, most < 2 ? 1 : (most - 2) / (max_splits - 1) + 1, twice, rows};
+    return {n, unit, most < 2 ? 1 : (most - 2) / (max_splits - 1) + 1, twice, rows, 4};
 }
 
 PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv, const PagedFormSizes& f) {
@@ -1763,7 +1769,15 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
         p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
         p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv, max_splits);
     }
-    if (big || p.pre_tiles)  // (behind prefixes 384: 33 us where 256 take 37)
+    // Windows are much of one length: where the (sequence, KV head) pairs fill 256 workgroups of eight waves, or whole
+    // rounds of 512 of four, to four fifths, each has a workgroup of its own, and nothing is left to join.  (32 windows
+    // of 1024 fp16 slots 36 us, q8 25, 64 of them 63; in even shares, joined: 42, 34 and 68.  40 windows, 52 us so or so,
+    // and 96 short ones, 41 us and 44 in three rounds of 256, are in even shares.)
+    const int64_t pairs = (int64_t)n_seqs * n_kv, rounds = (pairs + 511) / 512;
+    const int waves = pairs <= 256 && 5 * pairs >= 4 * 256 ? 8 : 5 * pairs >= 4 * 512 * rounds ? 4 : 0;
+    if (f.form == PAGED_WINDOW && !big && waves)
+        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, waves};
+    else if (big || p.pre_tiles)  // (behind prefixes 384: 33 us where 256 take 37)
         p.few = few_of(big ? 256 : 384, 8 * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     else
         p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
@@ -1783,6 +1797,13 @@ static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
         const unsigned tiles = (unsigned)a.tiles * a.map.n_kv * a.big.n + (unsigned)a.pre_tiles * a.map.n_kv * a.pre.n;
         hipLaunchKernelGGL((paged_chunk_kernel<FORM, TYPE, FMT>), dim3(few + tiles), dim3(512), CH_LDS, s, a);
     } else if constexpr (FORM != PAGED_PREFIX) {  // (prefixes have tiles)
+        if constexpr (FORM == PAGED_WINDOW)
+            if (a.few.waves == 8) {
+                e = hipFuncSetAttribute((const void*)paged_rows8_kernel<FORM, TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, rows_lds<8>(FORM));
+                if (e != hipSuccess) return e;
+                hipLaunchKernelGGL((paged_rows8_kernel<FORM, TYPE, FMT>), dim3(few), dim3(512), rows_lds<8>(FORM), s, a);
+                return hipGetLastError();
+            }
         hipLaunchKernelGGL((paged_rows_kernel<FORM, TYPE, FMT>), dim3(few), dim3(256), 0, s, a);
     }
     e = hipGetLastError();
