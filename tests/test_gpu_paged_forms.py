@@ -118,6 +118,26 @@ def test_window_of_long_sequences(fmt, type_, q_lens, kv_lens, window, sinks):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("heads,n_kv,q_lens,kv_lens", [
+    (64, 64, (1, 1, 1, 1), (700, 65, 1, 400)),                                # 256 pairs: a workgroup of eight waves each
+    (128, 64, (3, 0, 8, 1), (300, 200, 500, 0)),
+    (128, 64, (1, 2, 1, 1, 8, 1, 0, 1), (300, 90, 64, 1000, 450, 33, 20, 2)),  # 512: of four
+    (72, 72, (1,) * 12, tuple(range(100, 700, 50))),                          # 864: two rounds
+])
+def test_windows_that_fill_the_gpu(fmt, type_, heads, n_kv, q_lens, kv_lens):
+    """Sequences whole in one workgroup each."""
+    for window, sinks in ((200, 5), (33, 0), (64, 64)):
+        rng = np.random.default_rng(window)
+        pool, table = windowed(fmt, n_kv, 16, q_lens, kv_lens, window, sinks, rng)
+        form = Form(pool, window=window, sinks=sinks)
+        assert form.attention_work(heads, len(q_lens), sum(q_lens), max_q=max(q_lens), max_kv=max(kv_lens)) == 0
+        q = (rng.standard_normal((sum(q_lens), heads, D)) * 1.5).astype(NP[type_])
+        got = run_attention(pool, q, q_lens, kv_lens, table, type_, cache=form)
+        check(pool, q, q_lens, kv_lens, table, got, type_, window, sinks)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
 def test_a_window_of_everything_is_the_plain_attention(fmt, type_):
     """To the bit: the same slots in the same steps."""
     rng = np.random.default_rng(5)
