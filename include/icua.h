@@ -369,7 +369,7 @@ int icua_paged_attention_work(const icua_pages_t* pages, const icua_paged_attent
 /* The same for a window: a token at slot p of its sequence (kv_len - m + i for token i of m) sees slot j <= p if p - j <
  * window or j < sinks: its own and the window - 1 slots before it, and the sequence's first ones.  The slots between are
  * not read, whatever they hold, and their pages may be given back (table entries of any value; a page that is gone takes
- * part in nothing).  A window of max_kv or more is icua_paged_attention. */
+ * part in nothing).  A window and first slots that are max_kv or more together are icua_paged_attention. */
 typedef struct {
     int32_t window;          /* at least 1 */
     int32_t sinks;           /* at least 0 */

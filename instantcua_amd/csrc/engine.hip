@@ -1812,6 +1812,7 @@ static int attention_sizes(const icua_pages_t* pages, const icua_paged_attention
         if (f.window < 1 || f.sinks < 0) return fail("paged_attention: a window is at least 1 slot, its first slots at least 0");
         f.window = std::min(f.window, std::max(1, a.max_kv));  // as much as there is
         f.sinks = std::min(f.sinks, a.max_kv);
+        if ((int64_t)f.window + f.sinks >= a.max_kv) f.form = PAGED_ALL;  // every row sees all there is
     }
     if (f.form == PAGED_PREFIX) {
         if (f.n_groups < 0 || f.n_groups > PREFIX_GROUPS) return fail("paged_attention: n_groups must be in 0..64");

@@ -845,7 +845,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // Sequences with more query rows: 128 rows of a (sequence, KV head) a workgroup, eight waves.  Wave w has
 // rows 32 (w & 3) .. + 31 and of each 128 slots the half w >> 2; the two halves keep softmax states of their
-// own, joined through LDS at the end.  v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns,
+// own, joined through LDS at the end.  (Windows over fp16 slots: four waves and 64 slots, two workgroups a CU, so
+// that one's first loads and last stores are under the other's products: a prompt of 4096 tokens through a window of
+// 512 and 16 first slots 44 us, where eight waves take 51, with fp32 queries 57 and 67.  q8 has registers for eight
+// only, 156 us of a batch that takes 100; one group's prefix beside 64 tokens 35 us for 32.)  v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns,
 // lane (column, h) has slots 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major
 // V by transposing LDS reads.
 //
@@ -869,11 +872,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // of the CUs' (a third of that conflicts: the staged codes of four rows share a quarter of the places), products 18 %.
 constexpr int CH_ROWS = 128, CH_HALF = 64;
 constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
-constexpr int CH_STAGE = 4 * CH_MAT;            // two halves, K and V: 64 KiB
 constexpr int CH_SCALES = 8 * CH_HALF * 2;      // q8: a half's scales [K, V][group][slot]
 // And for the eight tiles of two stages whether V has values that are no numbers, whether the page exists, and
 // (q8, fp16 queries) the power of two that V's scales are below.
-constexpr int CH_FLAGS = 2 * CH_STAGE + 4 * CH_SCALES, CH_LDS = CH_FLAGS + 192;
+constexpr int ch_flags(int halves) { return 2 * halves * (2 * CH_MAT + CH_SCALES); }
+constexpr int ch_lds(int halves) { return ch_flags(halves) + 192; }
+// Halves of an iteration's slots, of four waves each.
+constexpr int ch_halves(int form, int fmt) { return form == PAGED_WINDOW && fmt == FMT_F16 ? 1 : 2; }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -943,13 +948,14 @@ __device__ __forceinline__ bool find_prefix_tile(const PagedAttnArgs& a, const P
 }
 
 template <int FORM, int TYPE, int FMT>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_chunk_kernel(PagedAttnArgs a) {
+    constexpr int HALVES = ch_halves(FORM, FMT), STEP = HALVES * CH_HALF;
     constexpr bool HL = TYPE == TYPE_F32, CODES = FMT == FMT_Q8;
     extern __shared__ __align__(1024) uint8_t lds[];
-    int* const tile_odd = (int*)(lds + CH_FLAGS);
+    int* const tile_odd = (int*)(lds + ch_flags(HALVES));
     int *const tile_there = tile_odd + 16, *const tile_top = tile_odd + 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
-    const int par = wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
+    const int par = HALVES == 1 ? 0 : wave >> 2, wi = wave & 3, group = a.n_heads / a.map.n_kv;
     // The first workgroups have the shared prefixes, the last ones the sequences of few rows: they are short, and
     // bound by memory.
     int index = blockIdx.x;
@@ -964,7 +970,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     const int few = index - a.tiles * a.map.n_kv * a.big.n;
     if (!pre && few >= 0) {
-        rows_work<FORM, TYPE, FMT, 8>(a, few, lds);
+        rows_work<FORM, TYPE, FMT, 4 * HALVES>(a, few, lds);
         return;
     }
     const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % parts.n;
@@ -981,7 +987,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int all_seen = before + tile * CH_ROWS / group;  // slots up to this one all rows of the workgroup see
     int lim = max(0, before + min(sp.n_q - 1, (tile * CH_ROWS + CH_ROWS - 1) / group) + 1);
     RowOf row = row_of(sp, r0 + c32, group, g);
-    // Iterations are of 128 slots, numbered without those that are skipped, 64 or a multiple of it: a half of an
+    // Iterations are of 64 slots a half, numbered without those that are skipped, 64 or a multiple of it: a half of an
     // iteration is a run of slots.  (Skipped 128 at a time, 16 first slots cost a window of 512 one iteration of 6.)
     SlotGap gap = {0, 0};
     bool joined = false;
@@ -998,7 +1004,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto slot_of = [&](int v) __attribute__((always_inline)) { return FORM == PAGED_ALL ? v : FORM == PAGED_PREFIX ? v + gap.skip : gap_slot(gap, v); };
     const int left = FORM == PAGED_ALL ? lim : max(0, lim - gap.skip);
     const int c0 = min(left, split * parts.chunk), c1 = min(left, c0 + parts.chunk);
-    const int it0 = c0 / 128, it1 = c1 > c0 ? (c1 + 127) / 128 : it0;
+    const int it0 = c0 / STEP, it1 = c1 > c0 ? (c1 + STEP - 1) / STEP : it0;
     // A window's rows see slots from first_own on, those of this wave from w_low .. w_high, and the first ones.
     const int first_own = row.last - a.f.window + 1, w_low = w_first - a.f.window + 1, w_high = w_last - a.f.window + 1;
 
@@ -1019,7 +1025,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         asm volatile("" : "+s"(p));
         return p;
     };
-    // Staging: wave w copies 16-slot tile w of an iteration's eight.  Lane i of `rows`: the pool row of this
+    // Staging: wave w copies 16-slot tile w of an iteration's.  Lane i of `rows`: the pool row of this
     // wave's tile in iteration sub + i (-1: no such page).
     int rows = -1, sub = it0 - WAVE;
     const int head_row = g * a.map.page_slots;
@@ -1028,7 +1034,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             auto b = arguments();
             const PageMap map = {b->map.n_pages, b->map.n_kv, b->map.page_slots};
             sub = it;
-            const int slot = slot_of((sub + lane) * 128 + 16 * wave);
+            const int slot = slot_of((sub + lane) * STEP + 16 * wave);
             rows = slot < (FORM == PAGED_ALL ? c1 : lim) ? seq_slot_row(map, b->tables + (int64_t)s * b->table_width, b->table_width, slot) : -1;
         }
         return __builtin_amdgcn_readlane(rows, it - sub);
@@ -1036,15 +1042,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const uint8_t *k_base = (const uint8_t*)a.k, *v_base = (const uint8_t*)a.v;
     // LDS: half hb of K (kv = 0) or V (1) in stage st, and the scales of a half.
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    auto half_at = [&](int kv, int st, int hb) { return (uint32_t)((kv * 2 + st) * 2 + hb) * CH_MAT; };
-    auto scales_at = [&](int st, int hb) { return (f16*)(lds + 2 * CH_STAGE + (st * 2 + hb) * CH_SCALES); };
+    auto half_at = [&](int kv, int st, int hb) { return (uint32_t)((kv * 2 + st) * HALVES + hb) * CH_MAT; };
+    auto scales_at = [&](int st, int hb) { return (f16*)(lds + 4 * HALVES * CH_MAT + (st * HALVES + hb) * CH_SCALES); };
     // fp16: this wave's tile of iteration it, pool row r, from memory to LDS; slots that are not there become
     // zeros.  Row l / 16 (+ 4 j) of the tile, place l % 16.
     int src_off[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) src_off[j] = (4 * j + lane / 16) * (HD * 2) + (((lane & 15) ^ swizzle(4 * j + lane / 16)) << 4);
     auto copy = [&](int kv, int it, int r) __attribute__((always_inline)) {
-        const int n = r < 0 ? 0 : lim - slot_of(it * 128 + 16 * wave);
+        const int n = r < 0 ? 0 : lim - slot_of(it * STEP + 16 * wave);
         const uint32_t dst = lds0 + half_at(kv, it & 1, par) + wi * 16 * HD * 2;
         const uint8_t* src = (kv ? v_base : k_base) + (int64_t)(max(r, 0) + head_row) * (HD * 2);
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
@@ -1065,7 +1071,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     u32x4 codes[2][2];
     uint16_t scale[2] = {0, 0};
     auto fetch = [&](int kv, int it, int r) __attribute__((always_inline)) {
-        const int n = r < 0 ? 0 : lim - slot_of(it * 128 + 16 * wave);
+        const int n = r < 0 ? 0 : lim - slot_of(it * STEP + 16 * wave);
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
         codes[kv][0] = codes[kv][1] = u32x4{0, 0, 0, 0};
         scale[kv] = 0;
@@ -1183,7 +1189,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) O[dt] = f32x16{};
     float m = NEG_INF, l = 0.f;
-    auto base_of = [&](int it) __attribute__((always_inline)) { return slot_of(it * 128 + CH_HALF * par); };
+    auto base_of = [&](int it) __attribute__((always_inline)) { return slot_of(it * STEP + CH_HALF * par); };
     // LDS addresses of operands in stage 0.  K of block 0: slot c32, dims 16 ks + 8 h .. + 7, at k_at ^ (ks <<
     // 5).  V^T: dims 32 dt + c32 of slots 4 h + {0 .. 3} (k = 1: + 8, the operand's other half), at v_at[k] ^
     // (dt << 6).  (A row's place in a stage is a multiple of its 256 bytes.)
@@ -1271,7 +1277,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // the products of the 16 before; the denominator sums the probabilities as the products take them.
     auto half_step = [&](int it) __attribute__((always_inline)) {
         f32x16 S[2] = {f32x16{}, f32x16{}};
-        const uint32_t st = (it & 1) * 2 * CH_MAT;
+        const uint32_t st = (it & 1) * HALVES * CH_MAT;
         v8h kf[8];
 #pragma unroll
         for (int k = 0; k < 6; ++k) kf[k] = k_operand(st + (k % 2) * 32 * HD * 2, k / 2);
@@ -1328,7 +1334,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
     };
     auto codes_scores = [&](int it, f32x16 S[2]) __attribute__((always_inline)) {
-        const uint32_t st = (it & 1) * 2 * CH_MAT;
+        const uint32_t st = (it & 1) * HALVES * CH_MAT;
         f32x16 y[2];
         S[0] = S[1] = f32x16{};
 #pragma unroll
@@ -1355,7 +1361,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // row's largest: d = 21 is where that shows (2e-3 of error instead of 1e-3 at most for a row).
     auto codes_values = [&](int it, const f32x16 S[2], const int4& tops) __attribute__((always_inline)) {
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
-        const uint32_t st = (it & 1) * 2 * CH_MAT;
+        const uint32_t st = (it & 1) * HALVES * CH_MAT;
         const f16* scales = scales_at(it & 1, par) + 4 * CH_HALF + 4 * h;
         const f16x2 ones = {(f16)1.f, (f16)1.f};
         float sum[2] = {0.f, 0.f};
@@ -1402,7 +1408,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // token left 4e-4 of error to rows of small values.)
     auto exact_values = [&](int it, int kt, const f32x16& S) __attribute__((always_inline)) {
         const float sub_m = m == NEG_INF ? 0.f : m - P_SHIFT;
-        const uint32_t Vs = (it & 1) * 2 * CH_MAT + kt * 32 * HD * 2;
+        const uint32_t Vs = (it & 1) * HALVES * CH_MAT + kt * 32 * HD * 2;
         const f16* scales = scales_at(it & 1, par) + 4 * CH_HALF + 32 * kt + 4 * h;
         float p[16];
 #pragma unroll
@@ -1448,10 +1454,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // Whether some row of the workgroup does not see all of an iteration: of an f16 pool, all of its values are
     // made finite then, also for waves whose rows see them.
     auto cleaned = [&](int it) __attribute__((always_inline)) {
-        if constexpr (FORM != PAGED_WINDOW) return slot_of(it * 128) + 127 > all_seen;
+        if constexpr (FORM != PAGED_WINDOW) return slot_of(it * STEP) + STEP - 1 > all_seen;
         bool some = false;
-        for (int half = 0; half < 2; ++half) {
-            const int at = slot_of(it * 128 + CH_HALF * half);
+        for (int half = 0; half < HALVES; ++half) {
+            const int at = slot_of(it * STEP + CH_HALF * half);
             some |= (at + CH_HALF - 1 > all_seen) | ((at + CH_HALF > a.f.sinks) & (at <= lim - 1 - a.f.window));
         }
         return some;
@@ -1497,7 +1503,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     // Iterations whose half some row of this wave sees.
     const int v_last = FORM == PAGED_ALL || w_last < gap.from ? w_last : max(gap.from - 1, w_last - gap.skip);  // w_last's number
-    const int my1 = active && base_of(it0) <= w_last ? min(it1, (v_last - CH_HALF * par) / 128 + 1) : it0;
+    const int my1 = active && base_of(it0) <= w_last ? min(it1, (v_last - CH_HALF * par) / STEP + 1) : it0;
     for (int it = it0; it < it1; ++it) {
         staged_barrier<0>();
         if (it + 1 < it1) stage(it + 1);
@@ -1532,22 +1538,27 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     // The halves' states join: waves 4 .. 7 hand theirs to waves 0 .. 3.
-    staged_barrier<0>();
     f32x4* const mo = (f32x4*)lds;                          // [4 waves][16][64 lanes]
     float2* const mml = (float2*)(lds + 4 * 16 * 64 * 16);  // [4 waves][64 lanes]
     l = swap32_add(l, l);
-    if (par == 1) {
+    float mt = m, lt = l, f0 = 1.f, f1 = 0.f;
+    if constexpr (HALVES == 2) {
+        staged_barrier<0>();
+        if (par == 1) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            mo[(wi * 16 + k) * 64 + lane] = f32x4{O[k / 4][4 * (k % 4)], O[k / 4][4 * (k % 4) + 1], O[k / 4][4 * (k % 4) + 2], O[k / 4][4 * (k % 4) + 3]};
-        mml[wi * 64 + lane] = make_float2(m, l);
+            for (int k = 0; k < 16; ++k)
+                mo[(wi * 16 + k) * 64 + lane] = f32x4{O[k / 4][4 * (k % 4)], O[k / 4][4 * (k % 4) + 1], O[k / 4][4 * (k % 4) + 2], O[k / 4][4 * (k % 4) + 3]};
+            mml[wi * 64 + lane] = make_float2(m, l);
+        }
+        staged_barrier<0>();
+        if (par == 1) return;
+        const float2 ml = mml[wi * 64 + lane];
+        mt = fmaxf(m, ml.x);
+        f0 = m == mt ? 1.f : __builtin_amdgcn_exp2f(m - mt);
+        f1 = ml.x == mt ? 1.f : __builtin_amdgcn_exp2f(ml.x - mt);
+        lt = l * f0 + ml.y * f1;
     }
-    staged_barrier<0>();
-    if (par == 1 || row.t < 0) return;
-    const float2 ml = mml[wi * 64 + lane];
-    const float mt = fmaxf(m, ml.x);
-    const float f0 = m == mt ? 1.f : __builtin_amdgcn_exp2f(m - mt), f1 = ml.x == mt ? 1.f : __builtin_amdgcn_exp2f(ml.x - mt);
-    const float lt = l * f0 + ml.y * f1;
+    if (row.t < 0) return;
     const bool partial = parts.n > 1 || joined;
     const float inv = partial ? 1.f : mt == NEG_INF && lt == 0.f ? 0.f : 1.f / lt;  // no slot seen: zeros
     const int64_t out_row = ((int64_t)row.t * a.n_heads + row.head) * parts.n + split;
@@ -1555,10 +1566,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     float2* const part_ml = FORM != PAGED_PREFIX ? a.part_ml : a.few_ml + (pre ? a.pre_at : a.part_at);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-        const f32x4 o1 = mo[(wi * 16 + k) * 64 + lane];
         f32x4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (O[k / 4][4 * (k % 4) + e] * f0 + o1[e] * f1) * inv;
+        for (int e = 0; e < 4; ++e) y[e] = O[k / 4][4 * (k % 4) + e];
+        if constexpr (HALVES == 2) {
+            const f32x4 o1 = mo[(wi * 16 + k) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = y[e] * f0 + o1[e] * f1;
+        }
+        y *= inv;
         const int d = 32 * (k / 4) + 8 * (k % 4) + 4 * h;
         if (partial)
             *(f32x4*)(part + out_row * HD + d) = y;
@@ -1746,6 +1762,7 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     PagedPlan p{};
     const bool prefix = f.form == PAGED_PREFIX;
     const int group = n_heads / n_kv, few = (int)std::min<int64_t>(ROWS_TILE, (int64_t)max_q * group);
+    const int halves = ch_halves(f.form, fmt);  // of a workgroup of the chunk kernel: one, and two workgroups a CU, or two
     const int max_splits = prefix ? PAGED_MAX_SPLITS / 2 : PAGED_MAX_SPLITS;  // a row has partials of two spans
     if (f.form == PAGED_WINDOW) max_kv = window_slots(max_kv, f.window, f.sinks);
     p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
@@ -1762,12 +1779,13 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
         // with 30; over q8 60 with 8, 45 with 12 and 53 with 30.)
         const double step = fmt == FMT_F16 ? 2. : 4., own = 6. + 1.5 * std::max(0, max_kv - f.max_prefix) / 256;
         const double us = std::max(16., n_kv * (tiles * steps * step + n_seqs * own) / 256);
-        const int64_t ranges = big ? 256 / std::max<int64_t>(1, tiles * n_kv) : (int64_t)(steps * step / (us - 8.) + 0.999);
+        const int64_t ranges = big ? 512 / halves / std::max<int64_t>(1, tiles * n_kv) : (int64_t)(steps * step / (us - 8.) + 0.999);
         p.pre = split_slots(1, ranges, f.max_prefix, max_splits);
     }
     if (big) {
         p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
-        p.big = split_slots((int64_t)p.tiles * n_kv, 256, max_kv, max_splits);
+        // (Windows of up to 512 slots are not split: 1024 tokens, windows of 128: 18 us, 27 in two parts, joined.)
+        p.big = split_slots((int64_t)p.tiles * n_kv, 512 / halves, max_kv, f.form == PAGED_WINDOW && max_kv <= 512 ? 1 : max_splits);
     }
     // Windows are much of one length: where the (sequence, KV head) pairs fill 256 workgroups of eight waves, or whole
     // rounds of 512 of four, to four fifths, each has a workgroup of its own, and nothing is left to join.  (32 windows
@@ -1778,7 +1796,7 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     if (f.form == PAGED_WINDOW && !big && waves)
         p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, waves};
     else if (big || p.pre_tiles)  // (behind prefixes 384: 33 us where 256 take 37)
-        p.few = few_of(big ? 256 : 384, 8 * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
+        p.few = few_of((big ? 512 : 768) / halves, 4 * halves * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     else
         p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     if (p.big.n > 1 || prefix) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
@@ -1792,10 +1810,11 @@ static hipError_t attention_of(const PagedAttnArgs& a, hipStream_t s) {
     const unsigned few = (unsigned)a.few.n * a.map.n_kv;
     hipError_t e;
     if (a.tiles || a.pre_tiles) {
-        e = hipFuncSetAttribute((const void*)paged_chunk_kernel<FORM, TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, CH_LDS);
+        constexpr int halves = ch_halves(FORM, FMT), lds = std::max(ch_lds(halves), (int)rows_lds<4 * halves>(FORM));
+        e = hipFuncSetAttribute((const void*)paged_chunk_kernel<FORM, TYPE, FMT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         const unsigned tiles = (unsigned)a.tiles * a.map.n_kv * a.big.n + (unsigned)a.pre_tiles * a.map.n_kv * a.pre.n;
-        hipLaunchKernelGGL((paged_chunk_kernel<FORM, TYPE, FMT>), dim3(few + tiles), dim3(512), CH_LDS, s, a);
+        hipLaunchKernelGGL((paged_chunk_kernel<FORM, TYPE, FMT>), dim3(few + tiles), dim3(256 * halves), lds, s, a);
     } else if constexpr (FORM != PAGED_PREFIX) {  // (prefixes have tiles)
         if constexpr (FORM == PAGED_WINDOW)
             if (a.few.waves == 8) {

@@ -134,3 +134,11 @@ int main() {
     subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
                     os.path.join(ROOT, "instantcua_amd", "csrc"), str(src), "-o", exe], check=True)
     assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout.strip() == "ok"
+
+
+def test_a_window_of_all_slots_takes_what_the_plain_call_takes():
+    c = cache()
+    for n_tokens, sizes in ((300, dict(max_q=300, max_kv=4000)), (8, dict(max_q=1, max_kv=4000))):
+        plain = c.attention_work(16, 8, n_tokens, **sizes)
+        for window, sinks in ((4000, 0), (3999, 1), (1, 3999), (2 ** 31 - 1, 2 ** 31 - 1), (1, 4000)):
+            assert c.attention_window_work(16, 8, n_tokens, window, sinks, **sizes) == plain
