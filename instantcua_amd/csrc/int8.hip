@@ -11,27 +11,43 @@ namespace {
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef f16 v8h __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------------------------------
 // Quantisation of rows.  y = x norm / sqrt(mean(x^2) + eps), or x:  scale = max |y| / 127, code = y / scale rounded
 // to the nearest, ties to even.  The root mean square is common to a row's values and leaves the codes as they are
-// without it: code = 127 t / max |t| of t = x norm.  All of it in 64 bits, where t is exact and the quotient rounds
-// as the exact one does but for ties, which the division decides: codes are those of the definition.
+// without it: code = 127 t / max |t| of t = x norm.  The maximum, its scale and the mean are of 64 bits, where t is
+// exact.  A quotient t (127 / max) in fp32 is less than 3 2^-24 of its at most 127 off, 2.3e-5: it rounds as the exact
+// one but within 4e-5 of half way between two codes (and in rows whose maximum is not near fp32's middle), where the
+// 64-bit one decides, and at 2^-40 from a tie the division itself: codes are those of the definition.
 
+// Eight values.
 template <int TYPE>
-__device__ __forceinline__ f32x4 load_x(const void* p, int64_t i) {
-    if constexpr (TYPE == TYPE_F32) return *(const f32x4*)((const float*)p + i);
-    const v4h h = *(const v4h*)((const f16*)p + i);
-    return f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+__device__ __forceinline__ void load_x(const void* p, int64_t i, float* x) {
+    if constexpr (TYPE == TYPE_F32) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const f32x4 v = *(const f32x4*)((const float*)p + i + 4 * k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * k + e] = v[e];
+        }
+    } else {
+        const v8h h = *(const v8h*)((const f16*)p + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)h[e];
+    }
 }
 
 // Over the lanes of a wave, every lane gets the result.
-template <typename OP>
-__device__ __forceinline__ double wave_reduce(double v, OP op) {
+template <typename T, typename OP>
+__device__ __forceinline__ T wave_reduce(T v, OP op) {
     auto other = [&](auto swap) __attribute__((always_inline)) {
-        const uint64_t b = __builtin_bit_cast(uint64_t, v);
-        return __builtin_bit_cast(double, (uint64_t)(uint32_t)swap((int)(uint32_t)b) | (uint64_t)(uint32_t)swap((int)(uint32_t)(b >> 32)) << 32);
+        if constexpr (sizeof(T) == 4) {
+            return __builtin_bit_cast(T, swap(__builtin_bit_cast(int, v)));
+        } else {
+            const uint64_t b = __builtin_bit_cast(uint64_t, v);
+            return __builtin_bit_cast(T, (uint64_t)(uint32_t)swap((int)(uint32_t)b) | (uint64_t)(uint32_t)swap((int)(uint32_t)(b >> 32)) << 32);
+        }
     };
     v = op(v, other([](int x) { return dpp_i<DPP_MIRROR>(x); }));
     v = op(v, other([](int x) { return dpp_i<DPP_HALF_MIRROR>(x); }));
@@ -41,96 +57,127 @@ __device__ __forceinline__ double wave_reduce(double v, OP op) {
     return op(v, other([](int x) { return __shfl_xor(x, 32); }));
 }
 
-// A workgroup a row; a thread has vectors of four values threadIdx.x + 256 i, in registers where KEEP of them hold the
-// row, else read a second time.  Bound by memory for many rows, a chain of two loads and two reductions for few.
-template <int TYPE, int KEEP>
+// A workgroup a row; a thread has vectors of eight values 8 threadIdx.x + 2048 i, in registers where KEEP of them hold
+// the row, else read a second time.  Bound by memory for many rows: 4096 of 6144 fp16 values, 76 MB, in 17 us, 4.5 TB/s
+// (in 64 bits throughout 23), of 2048 fp32 ones 8 us, with a norm 10; by a chain of two loads and a reduction for few,
+// 2.6 us.  4096 of 16384 fp16 values 45 us kept, 55 read twice; with a norm, which takes as many registers again, 8192
+// fp32 ones 70 us kept and 46 read twice.
+template <int TYPE, bool NORM, int KEEP>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(I8QuantArgs a) {
-    __shared__ double s_top[4], s_sum[4], s_odd[4];
+    __shared__ double s_top[4], s_sum[4];
+    __shared__ int s_none[4];
     const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t at = (int64_t)row * a.x_stride;
     constexpr int N = KEEP ? KEEP : 1;
-    f32x4 x[N], w[N];
+    float x[N][8], w[NORM ? N : 1][8];
     auto load = [&](int k, int i) __attribute__((always_inline)) {
-        x[k] = f32x4{};
-        w[k] = f32x4{1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+        if constexpr (NORM)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[k][e] = 1.f;
         if (i >= a.n_cols) return;
-        x[k] = load_x<TYPE>(a.x, at + i);
-        if (a.norm) w[k] = *(const f32x4*)(a.norm + i);
+        load_x<TYPE>(a.x, at + i, x[k]);
+        if constexpr (NORM) load_x<TYPE_F32>(a.norm, i, w[k]);
     };
+    uint32_t bits = 0;  // without a norm: the largest magnitude's bits, an infinity's or more if some y is none
     double top = 0., sum = 0., odd = 0.;  // odd: no number if some y is none
     auto look = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const double v = x[k][e], t = v * (double)w[k][e];
-            top = fmax(top, fabs(t));
-            sum = fma(v, v, sum);
-            odd = fma(t, t, odd);
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (NORM) {
+                const double v = x[k][e], t = v * (double)w[k][e];
+                top = fmax(top, fabs(t));
+                sum = fma(v, v, sum);
+                odd = fma(t, t, odd);
+            } else {
+                bits = max(bits, as_u32(x[k][e]) & 0x7FFFFFFFu);
+            }
         }
     };
     if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int k = 0; k < KEEP; ++k) load(k, 4 * threadIdx.x + 1024 * k);
+        for (int k = 0; k < KEEP; ++k) load(k, 8 * threadIdx.x + 2048 * k);
 #pragma unroll
         for (int k = 0; k < KEEP; ++k) look(k);
     } else {
-        for (int i = 4 * threadIdx.x; i < a.n_cols; i += 1024) {
+        for (int i = 8 * threadIdx.x; i < a.n_cols; i += 2048) {
             load(0, i);
             look(0);
         }
     }
-    auto add = [](double p, double q) { return p + q; };
-    top = wave_reduce(top, [](double p, double q) { return fmax(p, q); });
-    sum = wave_reduce(sum, add);
-    odd = wave_reduce(odd, add);
+    bool none;
+    if constexpr (NORM) {
+        top = wave_reduce(top, [](double p, double q) { return fmax(p, q); });
+        sum = wave_reduce(sum, [](double p, double q) { return p + q; });
+        none = __ballot(!(odd < __builtin_inf())) != 0;
+    } else {
+        bits = wave_reduce(bits, [](uint32_t p, uint32_t q) { return max(p, q); });
+        top = as_f32(bits);
+        none = bits >= 0x7F800000u;
+    }
     if (lane == 0) {
         s_top[wave] = top;
         s_sum[wave] = sum;
-        s_odd[wave] = odd;
+        s_none[wave] = none;
     }
     __syncthreads();
     top = fmax(fmax(s_top[0], s_top[1]), fmax(s_top[2], s_top[3]));
-    odd = s_odd[0] + s_odd[1] + s_odd[2] + s_odd[3];
-    const bool none = !(odd < __builtin_inf());
+    none = (s_none[0] | s_none[1] | s_none[2] | s_none[3]) != 0;
     if (threadIdx.x == 0) {
         sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        const double r = a.norm ? 1. / sqrt(sum / a.n_cols + (double)a.eps) : 1.;
+        const double r = NORM ? 1. / sqrt(sum / a.n_cols + (double)a.eps) : 1.;
         a.scales[row] = none ? __builtin_nanf("") : (float)(top * r / 127.);
     }
-    // The quotient by way of the reciprocal is 2^-51 off: next to half way between two codes the division decides.
     const double to = none || top == 0. ? 0. : 127. / top;
+    const bool middle = to == 0. || (top > 0x1p-60 && top < 0x1p60);  // no product of fp32 values leaves its range
+    const float to32 = middle ? (float)to : 0.f;
     auto store = [&](int k, int i) __attribute__((always_inline)) {
         if (i >= a.n_cols) return;
-        uint32_t word = 0;
+        int code[8];
+        float off = middle ? 0.f : 1.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const double t = (double)x[k][e] * (double)w[k][e];
-            const double q = t * to;
-            double r = __builtin_rint(q);
-            if (__builtin_expect(fabs(q - r) > 0.5 - 1e-9, 0)) r = __builtin_rint(t * 127. / top);
-            word |= (uint32_t)(none ? 0 : (int)r & 255) << (8 * e);
+        for (int e = 0; e < 8; ++e) {
+            const float q = (none ? 0.f : NORM ? x[k][e] * w[k][e] : x[k][e]) * to32, r = __builtin_rintf(q);
+            off = fmaxf(off, fabsf(q - r));
+            code[e] = (int)r;
         }
-        *(uint32_t*)(a.codes + (int64_t)row * a.codes_stride + i) = word;
+        if (__builtin_expect(off > 0.49996f, 0)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double t = NORM ? (double)x[k][e] * (double)w[k][e] : (double)x[k][e], q = t * to;
+                double r = __builtin_rint(q);
+                if (__builtin_expect(fabs(q - r) > 0.5 - 0x1p-40, 0)) r = __builtin_rint(t * 127. / top);
+                code[e] = (int)r;
+            }
+        }
+        uint2 word;
+        word.x = (code[0] & 255) | (code[1] & 255) << 8 | (code[2] & 255) << 16 | (uint32_t)code[3] << 24;
+        word.y = (code[4] & 255) | (code[5] & 255) << 8 | (code[6] & 255) << 16 | (uint32_t)code[7] << 24;
+        *(uint2*)(a.codes + (int64_t)row * a.codes_stride + i) = word;
     };
     if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int k = 0; k < KEEP; ++k) store(k, 4 * threadIdx.x + 1024 * k);
+        for (int k = 0; k < KEEP; ++k) store(k, 8 * threadIdx.x + 2048 * k);
     } else {
-        for (int i = 4 * threadIdx.x; i < a.n_cols; i += 1024) {
+        for (int i = 8 * threadIdx.x; i < a.n_cols; i += 2048) {
             load(0, i);
             store(0, i);
         }
     }
 }
 
-template <int TYPE>
+template <int TYPE, bool NORM>
 hipError_t quantize_of(const I8QuantArgs& a, hipStream_t s) {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.n_rows), dim3(256), 0, s, a); };
     if (a.n_cols <= 2048)
-        go(i8_quantize_kernel<TYPE, 2>);
+        go(i8_quantize_kernel<TYPE, NORM, 1>);
     else if (a.n_cols <= 6144)
-        go(i8_quantize_kernel<TYPE, 6>);
+        go(i8_quantize_kernel<TYPE, NORM, 3>);
+    else if (!NORM && a.n_cols <= 16384)
+        go(i8_quantize_kernel<TYPE, NORM, NORM ? 0 : 8>);
     else
-        go(i8_quantize_kernel<TYPE, 0>);
+        go(i8_quantize_kernel<TYPE, NORM, 0>);
     return hipGetLastError();
 }
 
@@ -158,10 +205,11 @@ __device__ __forceinline__ float gated_up(float g, float u) {
 // gates, the other half the same channels' ups.
 //
 // The order of issue is written out: under each product one operand of the 32 codes ahead is read, and two of them in
-// four carry the copies of a later stage (all in one of the four: 126 us where this took 111).  Large tiles are bound by
-// LDS, which gives a CU 64 bytes a cycle (ds_read_b128 of 64 different places: 16 cycles): 256 x 256 x 128 codes are
-// 192 KB of operands and 64 KB of copies, 4096 cycles, next to 2048 of products.  Waves of 128 x 128, with 3072, were
-// no faster (one wave a SIMD hides no latency); nor were two groups of waves in turn, or 64 codes a stage in four.
+// four carry the copies of a later stage (all in one of the four: 126 us where this took 111).  Large tiles, 8192^3 of
+// random codes in 480 to 515 us, 2.1 to 2.3 POPS, are bound by their copies: on the same data 438 us without those of
+// later stages, and no faster with half of either operand's reads.  256 x 256 x 128 codes are 64 KB of copies and 192 KB
+// of reads; waves of 128 x 128, with 128 KB of reads, were no faster, nor were two groups of waves in turn, or 64 codes
+// a stage in four.
 template <int TYPE, bool GATED, int BM, int BN, int WM, int WN, int KW, int NS>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * KW * 64) void i8_matmul_kernel(I8MatmulArgs a, int tiles_m, int tiles_n) {
     constexpr int BK = 128, THREADS = BM / WM * (BN / WN) * 64, STAGE = (BM + BN) * BK, KS = BK / 32;
@@ -541,7 +589,8 @@ hipError_t matmul_of(const I8MatmulArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_i8_quantize(int type, const I8QuantArgs& a, hipStream_t s) {
-    return type == TYPE_F32 ? quantize_of<TYPE_F32>(a, s) : quantize_of<TYPE_F16>(a, s);
+    if (a.norm) return type == TYPE_F32 ? quantize_of<TYPE_F32, true>(a, s) : quantize_of<TYPE_F16, true>(a, s);
+    return type == TYPE_F32 ? quantize_of<TYPE_F32, false>(a, s) : quantize_of<TYPE_F16, false>(a, s);
 }
 
 hipError_t launch_i8_matmul(int type, bool gated, const I8MatmulArgs& a, hipStream_t s) {

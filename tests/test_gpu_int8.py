@@ -78,6 +78,24 @@ def test_quantize_ties_and_sizes(type):
     assert (np.abs(scales - s) <= s * 2.0 ** -24 + tiny).all()
 
 
+@pytest.mark.parametrize("cols", [2048, 2064, 6160, 16384, 16400])
+@pytest.mark.parametrize("with_norm", [False, True])
+@pytest.mark.parametrize("size", [0, -61, 62, -100])
+def test_quantize_next_to_ties(cols, with_norm, size):
+    """Quotients some fp32 steps from half way between two codes, on both sides: closer than fp32 arithmetic tells."""
+    rng = np.random.default_rng(cols)
+    half = (np.arange(cols) % 127 - 63 + 0.5).astype(np.float32)
+    x = half * (1 + rng.integers(-3, 4, (4, cols)) * 2.0 ** -23).astype(np.float32)
+    norm = np.ones(cols, np.float32)
+    if with_norm:
+        norm = np.ldexp(np.float32(1), rng.integers(-3, 4, cols)).astype(np.float32)
+        norm[::3] *= np.float32(1 + 2.0 ** -23)
+    x = (x / norm * 2.0 ** size).astype(np.float32)
+    x[:, 7] = 127 * 2.0 ** size / norm[7]
+    codes, _ = run_quantize(x, norm if with_norm else None)
+    assert np.array_equal(codes, quantised(x, norm if with_norm else None)[0])
+
+
 def test_quantize_rows_that_are_no_numbers():
     rng = np.random.default_rng(3)
     x = rng.standard_normal((6, 256)).astype(np.float32)
