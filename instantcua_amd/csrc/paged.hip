@@ -1768,19 +1768,31 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     p.big = {1, std::max(128, (max_kv + 127) / 128 * 128)};
     p.pre = {1, std::max(128, (f.max_prefix + 127) / 128 * 128)};
     const bool big = (int64_t)max_q * group > ROWS_TILE;
+    int64_t shares = 256;  // workgroups that few-row sequences have beside prefixes
     if (prefix && n_tokens) {
-        // As many tiles as there may be; about half of a group's last one is in use.
+        // As many tiles as there may be; one of a group at least, and about half of its last one is in use.
         const int64_t rows = (int64_t)n_tokens * group, groups = std::min<int64_t>(f.n_groups, rows);
-        const int64_t tiles = std::max<int64_t>(1, (rows + 63 * groups) / CH_ROWS), steps = (f.max_prefix + 127) / 128;
+        const int64_t tiles = std::max<int64_t>(groups, (rows + 63 * groups) / CH_ROWS), steps = (f.max_prefix + 127) / 128;
         p.pre_tiles = (int)((rows + 127 * groups) / CH_ROWS);
-        // Beside few-row sequences a prefix's workgroups should end with them: of the CUs' time, at 2 us for 128 slots
-        // (q8 4) of a tile and 3 us for 256 slots of a sequence, half of the bound's, and 6 us to begin with, each
-        // takes its share less 8 us.  (64 tokens behind 7680 slots: 33 us with 8 or 10 ranges of slots, 36 with 6, 46
-        // with 30; over q8 60 with 8, 45 with 12 and 53 with 30.)
-        const double step = fmt == FMT_F16 ? 2. : 4., own = 6. + 1.5 * std::max(0, max_kv - f.max_prefix) / 256;
-        const double us = std::max(16., n_kv * (tiles * steps * step + n_seqs * own) / 256);
-        const int64_t ranges = big ? 512 / halves / std::max<int64_t>(1, tiles * n_kv) : (int64_t)(steps * step / (us - 8.) + 0.999);
-        p.pre = split_slots(1, ranges, f.max_prefix, max_splits);
+        if (big) {
+            p.pre = split_slots(1, 512 / halves / (tiles * n_kv), f.max_prefix, max_splits);
+        } else {
+            // Beside few-row sequences: all workgroups at a time, one a CU, as many ranges of slots as end with the
+            // sequences' shares (us of a tile's 128 slots, and of a sequence's 256, of which there are six tenths of the
+            // most that there may be).  64 tokens behind 7680 slots 29 us with 10 ranges and 176 shares, 32 with 384
+            // shares in a second round; 20 sequences of 8 tokens and fp32 queries, three prefixes, over q8 65 us with 6
+            // ranges and 112 shares, 74 with 11 and 384.
+            const double step = fmt == FMT_F16 ? 2.5 : 5., unit = fmt == FMT_F16 ? 3. : 3.5;
+            const int64_t units = (int64_t)(n_seqs * std::max(1., 0.6 * (max_kv - f.max_prefix) / 256 + 0.5)), wgs = tiles * n_kv;
+            double least = 1e30;
+            int64_t ranges = 1;
+            for (int64_t n = 1; n <= std::min<int64_t>(steps, max_splits) && (n == 1 || n * wgs + n_kv <= 256); ++n) {
+                const int64_t share = std::max<int64_t>(1, (256 - n * wgs % 256) / n_kv);
+                const double us = 0.1 * n + std::max(8. + (steps + n - 1) / n * step, 6. + (units + share - 1) / share * unit);
+                if (us < least) least = us, ranges = n, shares = share * n_kv;
+            }
+            p.pre = split_slots(1, ranges, f.max_prefix, max_splits);
+        }
     }
     if (big) {
         p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
@@ -1793,10 +1805,14 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     // and 96 short ones, 41 us and 44 in three rounds of 256, are in even shares.)
     const int64_t pairs = (int64_t)n_seqs * n_kv, rounds = (pairs + 511) / 512;
     const int waves = pairs <= 256 && 5 * pairs >= 4 * 256 ? 8 : 5 * pairs >= 4 * 512 * rounds ? 4 : 0;
-    if (f.form == PAGED_WINDOW && !big && waves)
-        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, waves};
-    else if (big || p.pre_tiles)  // (behind prefixes 384: 33 us where 256 take 37)
-        p.few = few_of((big ? 512 : 768) / halves, 4 * halves * ROWS_STEP, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
+    // Beside prompts windows of up to 1536 slots are whole, too: 32 sessions, chunks of 100 tokens and single ones, 1000
+    // slots, 58 us for 63.  (Of 2048 q8 slots they end last: 109 us for 101.)
+    const bool whole = f.form == PAGED_WINDOW && (big ? max_kv <= 1536 : waves > 0);
+    const int unit = 4 * halves * ROWS_STEP;  // slots of a step of a workgroup of the chunk kernel
+    if (whole)
+        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, big ? 4 : waves};
+    else if (big || p.pre_tiles)
+        p.few = few_of(big ? 512 / halves : shares, unit, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     else
         p.few = few_of(512, 4 * ROWS_STEP, fmt == FMT_F16 ? 4 : INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     if (p.big.n > 1 || prefix) p.part_rows = (size_t)n_tokens * n_heads * p.big.n;
