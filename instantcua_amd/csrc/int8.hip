@@ -418,10 +418,22 @@ hipError_t matmul_tiles(const I8MatmulArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Few tokens: a matrix value takes part in few products, and goes from memory to registers.  A workgroup has ROWS matrix rows (gated: as many gates and their ups) and 16 MB tokens; its eight waves
-// take 128 codes of all rows in turn, on v_mfma_i32_16x16x64_i8 (matrix rows as the result's rows, tokens as its
-// columns), and join their sums through LDS.  A row's 128 codes are one line of memory: lane (row, q) has 32 of them,
-// and the tokens' operands take theirs in the same order.
+// Tiles of 128 x 256: three stages where they fill the CUs and are deep, so that memory is waited for less (4096 tokens
+// of 2048 channels, 6144 deep, with their quantisation: 78 us, 87 with two; added to fp32 rows 90 and 97), else two
+// (2048 tokens, added: 52.5 us, 54 with three).
+template <int TYPE, bool GATED>
+hipError_t matmul_wide(const I8MatmulArgs& a, hipStream_t s) {
+    const int64_t tiles = (int64_t)((a.n_rows + 127) / 128) * ((a.n_out + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+    if (tiles >= 192 && a.n_in >= 6144) return matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 3>(a, s);
+    return matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 2>(a, s);
+}
+
+// Few tokens: a matrix value takes part in few products, and goes from memory to registers.  A workgroup has ROWS matrix
+// rows (gated: as many gates and their ups) and 16 MB tokens; its eight waves take 128 codes of all rows in turn, on
+// v_mfma_i32_16x16x64_i8 (matrix rows as the result's rows, tokens as its columns), and join their sums through LDS.  A
+// row's 128 codes are one line of memory: lane (row, q) has 32 of them, and the tokens' operands take theirs in the same
+// order.  Bound by memory and its latency: 8 tokens, 4096 channels, 2048 deep, 8 MB, in 4.0 us; 16 tokens of 6144 gated
+// channels, 25 MB, in 8.5 us, 3.0 TB/s.
 template <int TYPE, bool GATED, int RB, int MB, int DEPTH>
 __global__ __launch_bounds__(512) void i8_stream_kernel(I8MatmulArgs a) {
     constexpr int NW = 8, SETS = GATED ? 2 : 1, ROWS = 16 * RB, TOKENS = 16 * MB, VALUES = ROWS * TOKENS;
@@ -564,7 +576,7 @@ hipError_t matmul_of(const I8MatmulArgs& a, hipStream_t s) {
     static const Choice tiles[] = {
         {{64, 128 / G, 1, 2, 1.59f, 2.40f, 0.433f, 0.363f}, matmul_tiles<TYPE, GATED, 64, 128, 32, 64, 1, 3>},
         {{128, 128 / G, 1, 2, 0.12f, 3.51f, 0.686f, 0.572f}, matmul_tiles<TYPE, GATED, 128, 128, 64, 64, 1, 2>},
-        {{128, 256 / G, 1, 1, 0.00f, 4.79f, 0.111f, 0.910f}, matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 2>},
+        {{128, 256 / G, 1, 1, 0.00f, 4.79f, 0.111f, 0.910f}, matmul_wide<TYPE, GATED>},
         {{256, 256 / G, 1, 1, 0.00f, 8.11f, 1.219f, 0.631f}, matmul_tiles<TYPE, GATED, 256, 256, 128, 64, 1, 2>},
     };
     const Choice* best = nullptr;

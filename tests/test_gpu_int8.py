@@ -206,6 +206,11 @@ def test_matmul(type, form, m, n, k, gap):
     check(got, want, tol, type)
 
 
+@pytest.mark.parametrize("form,m,n,k,gap", [("add", 4090, 2040, 6160, 1), ("gated", 2040, 2040, 6160, 0), ("plain", 3970, 1800, 8192, 0)])
+def test_deep_products_that_fill_the_gpu(form, m, n, k, gap):
+    test_matmul(int8.F32, form, m, n, k, gap)
+
+
 @pytest.mark.parametrize("m,n,k,gap", [(1, 100, 256, 0), (40, 130, 512, 3), (300, 520, 1024, 0)])
 def test_matmul_adds_in_place(m, n, k, gap):
     rng = np.random.default_rng(m)
