@@ -200,7 +200,7 @@ __device__ __forceinline__ float gated_up(float g, float u) {
 // of the 16x16x64 one: 4.6 and 2.6 POPS of products of zeros, 3.5 and 2.2 of random codes, where the chip's power is
 // the limit): tokens are the result's rows, channels its columns, so that a wave's stores are runs of 32 channels.
 // Rows are staged in LDS 128 codes at a time, NS stages, by copies that run under the products; row r's 16-byte chunk
-// c lies at place c ^ (r & 7), so that eight rows' reads of one chunk meet no bank twice.  KW groups of waves have the
+// c lies at place c ^ (r / 2 & 7), so that sixteen rows' reads of one chunk meet no bank twice.  KW groups of waves have the
 // tile's 128 codes in turn, for few tiles, and join their sums through LDS.  Gated: half of a wave's matrix rows are
 // gates, the other half the same channels' ups.
 //
@@ -228,13 +228,13 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * KW * 64) void i8_matmul_kerne
     const int band = tile / (4 * tiles_n), bm = min(4, tiles_m - 4 * band), in_band = tile - band * 4 * tiles_n;
     const int m0 = (4 * band + in_band % bm) * BM, n0 = in_band / bm * OUT;
     // Copy i of a thread: 16 bytes of row (i * THREADS + tid) / 8 of the tile's x, or of its matrix rows.
-    const int chunk = 16 * (tid % 8 ^ tid / 8 % 8);
+    auto chunk = [&](int i) __attribute__((always_inline)) { return 16 * (tid % 8 ^ ((i < CX ? i : i - CX) * THREADS + tid) / 16 % 8); };
     const uint8_t *x0 = (const uint8_t*)a.x + m0 * a.x_stride, *w0 = (const uint8_t*)a.w + n0 * a.w_stride;
     uint32_t offset[CX + CW];
 #pragma unroll
     for (int i = 0; i < CX + CW; ++i) {
         const int r = ((i < CX ? i : i - CX) * THREADS + tid) / 8, o = r / WN * WOUT + r % WN % WOUT;
-        offset[i] = (uint32_t)(i < CX ? min(r, a.n_rows - 1 - m0) * (int)a.x_stride : min(o, a.n_out - 1 - n0) * (int)a.w_stride) + chunk;
+        offset[i] = (uint32_t)(i < CX ? min(r, a.n_rows - 1 - m0) * (int)a.x_stride : min(o, a.n_out - 1 - n0) * (int)a.w_stride) + chunk(i);
     }
     const int64_t ups = GATED ? a.n_out * a.w_stride : 0;
     // Iteration it of this part of the waves is of codes first_k(it) .. + 127; `steps` are the workgroup's, this part's
@@ -253,15 +253,15 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * KW * 64) void i8_matmul_kerne
     };
     // A stage that the last code lies in: zeros of x behind it, any of the matrix.
     auto copy_end = [&](int it) __attribute__((always_inline)) {
-        const bool there = first_k(it) + chunk < a.n_in;
 #pragma unroll
         for (int i = 0; i < CX + CW; ++i) {
+            const bool there = first_k(it) + chunk(i) < a.n_in;
             const uint32_t dst = lds0 + it % NS * STAGE + wave * 1024 + (i < CX ? i : i - CX) * THREADS * 16;
             const bool up = GATED && i >= CX && ((i - CX) * THREADS + wave * 64) / 8 % WN >= WOUT;
             if (i < CX)
                 copy_to_lds(there ? x0 + offset[i] + first_k(it) : (const uint8_t*)&g_zero_codes, dst);
             else
-                copy_to_lds(w0 + (up ? ups : 0) + (there ? offset[i] + first_k(it) : offset[i] - chunk), dst + BM * BK);
+                copy_to_lds(w0 + (up ? ups : 0) + (there ? offset[i] + first_k(it) : offset[i] - chunk(i)), dst + BM * BK);
         }
     };
     auto stage = [&](int it) __attribute__((always_inline)) {
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * KW * 64) void i8_matmul_kerne
     const uint32_t x_at = lds0 + (wm * WM + c32) * BK, w_at = lds0 + (BM + wn * WN + c32) * BK;
     // Operand k of the codes 32 ks .. + 31 of the stage at `at`.
     auto read = [&](int at, int ks, int k) __attribute__((always_inline)) {
-        const uint32_t c = ((2 * ks + h) ^ (c32 & 7)) << 4;
+        const uint32_t c = ((2 * ks + h) ^ (c32 >> 1 & 7)) << 4;
         if (k < NI)
             x[ks & 1][k] = *(__attribute__((address_space(3))) const i32x4*)(x_at + at + c + 32 * BK * k);
         else

@@ -1066,8 +1066,11 @@ __global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_w
             }
         }
     };
-    // q8: lane l has row l / 4 of the tile and its group l % 4, fetched before the products and put to
-    // LDS after them.
+    // q8: a lane has a group of a row of the tile, fetched before the products and put to LDS after them.  Lane l of row
+    // l % 16: the rows of 16 lanes meet no bank twice when they are put (12 sessions of chunks and single tokens 125 us,
+    // 132 with lane l of row l / 4, whose loads are of fewer lines: prefixes, whose short ranges wait for them, 64 us of
+    // drafts for 65).
+    const int q_row = FORM == PAGED_PREFIX ? lane >> 2 : lane & 15, q_group = FORM == PAGED_PREFIX ? lane & 3 : lane >> 4;
     u32x4 codes[2][2];
     uint16_t scale[2] = {0, 0};
     auto fetch = [&](int kv, int it, int r) __attribute__((always_inline)) {
@@ -1075,17 +1078,17 @@ __global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_w
         if (!kv && lane == 0) tile_there[(it & 1) * 8 + wave] = r >= 0;
         codes[kv][0] = codes[kv][1] = u32x4{0, 0, 0, 0};
         scale[kv] = 0;
-        if (lane / 4 < n) {
-            const int64_t at = (int64_t)r + head_row + lane / 4;
-            const uint8_t* c = (kv ? v_base : k_base) + at * HD + 32 * (lane & 3);
+        if (q_row < n) {
+            const int64_t at = (int64_t)r + head_row + q_row;
+            const uint8_t* c = (kv ? v_base : k_base) + at * HD + 32 * q_group;
             codes[kv][0] = *(const u32x4*)c;
             codes[kv][1] = *(const u32x4*)(c + 16);
-            scale[kv] = ((const uint16_t*)(kv ? a.v_sb : a.k_sb))[at * NG + (lane & 3)];
+            scale[kv] = ((const uint16_t*)(kv ? a.v_sb : a.k_sb))[at * NG + q_group];
         }
     };
     auto put = [&](int kv, int it) __attribute__((always_inline)) {
         uint8_t* dst = lds + half_at(kv, it & 1, par);
-        const int r = 16 * wi + lane / 4;
+        const int r = 16 * wi + q_row;
         // V with a scale that is no number is kept out of the products, for the rows that may not see it.
         const bool odd = kv && __ballot(!(fabsf(h2f(scale[1])) <= 65504.f));
         if (kv && lane == 0) tile_odd[(it & 1) * 8 + wave] = odd;
@@ -1102,7 +1105,7 @@ __global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_w
 #pragma unroll
                 for (int e = 0; e < 2; ++e) y[2 * x + e] = h2_bits(c[e]);
             }
-            *(u32x4*)(dst + r * (HD * 2) + (((4 * (lane & 3) + k) ^ swizzle(r)) << 4)) = y;
+            *(u32x4*)(dst + r * (HD * 2) + (((4 * q_group + k) ^ swizzle(r)) << 4)) = y;
         }
         if (kv && !HL) {  // the power of two that the largest scale is below; where less than 1, scales are raised by it
             int top = scale[1] & 0x7FFF;  // fp16 bits rise with the value
@@ -1118,7 +1121,7 @@ __global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_w
             if (lane == 0) tile_top[(it & 1) * 8 + wave] = top;
             sc *= __builtin_bit_cast(f16, (uint16_t)((15 - min(top, 0)) << 10));
         }
-        scales_at(it & 1, par)[kv * 4 * CH_HALF + (lane & 3) * CH_HALF + r] = sc;
+        scales_at(it & 1, par)[kv * 4 * CH_HALF + q_group * CH_HALF + r] = sc;
     };
 
     auto stage = [&](int it) __attribute__((always_inline)) {
