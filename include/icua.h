@@ -273,7 +273,8 @@ typedef struct {
     size_t work_bytes;
 } icua_i8_matmul_t;
 int icua_i8_matmul(const icua_i8_matmul_t* args, void* stream);
-/* Bytes of `work` for a call with exactly these sizes (the pointers in args are not looked at). */
+/* Bytes of `work` for a call with exactly these sizes (the pointers in args are not looked at): 0 for all of them at
+ * present, and `work` may be NULL then. */
 int icua_i8_matmul_work(const icua_i8_matmul_t* args, size_t* bytes);
 
 /* ---- paged K/V caches: several sequences in one pool of pages, on device buffers ----

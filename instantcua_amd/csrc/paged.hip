@@ -848,9 +848,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // own, joined through LDS at the end.  (Windows over fp16 slots: four waves and 64 slots, two workgroups a CU, so
 // that one's first loads and last stores are under the other's products: a prompt of 4096 tokens through a window of
 // 512 and 16 first slots 44 us, where eight waves take 51, with fp32 queries 57 and 67.  q8 has registers for eight
-// only, 156 us of a batch that takes 100; one group's prefix beside 64 tokens 35 us for 32.)  v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns,
-// lane (column, h) has slots 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major
-// V by transposing LDS reads.
+// only, 156 us of a batch that takes 100; one group's prefix beside 64 tokens 35 us for 32.)
+//
+// v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns, lane (column, h) has slots
+// 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major V by transposing LDS reads.
 //
 // K and V are staged in LDS, two stages of 128 slots, by copies that run under the products: fp16 from memory
 // to LDS directly; q8 through registers, as the exact codes in fp16, whose scales go to the groups' sums in fp32
@@ -868,8 +869,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // tokens, 16 heads, fp16 queries: 87 us, 0.79 PFLOP/s of the causal half; q8 142 us.  With fp32 queries, twice the
 // products (f16 pool) and also a split of each group's products (q8): 138 and 303 us; they spill 17 and 15 registers.
 //
-// q8, 12 sessions of chunks and single tokens, 126 us: vector instructions fill 51 % of the SIMDs' cycles, LDS 49 %
-// of the CUs' (a third of that conflicts: the staged codes of four rows share a quarter of the places), products 18 %.
+// q8, 12 sessions of chunks and single tokens, 121 us: vector instructions fill 53 % of the SIMDs' cycles, LDS 41 %
+// of the CUs' (an eighth of that conflicts), products 19 %.
 constexpr int CH_ROWS = 128, CH_HALF = 64;
 constexpr int CH_MAT = CH_HALF * HD * 2;        // bytes of a half's K or V
 constexpr int CH_SCALES = 8 * CH_HALF * 2;      // q8: a half's scales [K, V][group][slot]
