@@ -57,6 +57,8 @@ __device__ __forceinline__ T wave_reduce(T v, OP op) {
     return op(v, other([](int x) { return __shfl_xor(x, 32); }));
 }
 
+constexpr int QUANT_ROWS = 1 << 20;  // of a launch's first dimension, which has fewer than 2^32 threads
+
 // A workgroup a row; a thread has vectors of eight values 8 threadIdx.x + 2048 i, in registers where KEEP of them hold
 // the row, else read a second time.  Bound by memory for many rows: 4096 of 6144 fp16 values, 76 MB, in 17 us, 4.5 TB/s
 // (in 64 bits throughout 23), of 2048 fp32 ones 8 us, with a norm 10; by a chain of two loads and a reduction for few,
@@ -66,7 +68,8 @@ template <int TYPE, bool NORM, int KEEP>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(I8QuantArgs a) {
     __shared__ double s_top[4], s_sum[4];
     __shared__ int s_none[4];
-    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.y * QUANT_ROWS + blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (row >= a.n_rows) return;
     const int64_t at = (int64_t)row * a.x_stride;
     constexpr int N = KEEP ? KEEP : 1;
     float x[N][8], w[NORM ? N : 1][8];
@@ -169,7 +172,8 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(I8QuantArgs a) {
 
 template <int TYPE, bool NORM>
 hipError_t quantize_of(const I8QuantArgs& a, hipStream_t s) {
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.n_rows), dim3(256), 0, s, a); };
+    const dim3 grid(std::min(a.n_rows, QUANT_ROWS), (a.n_rows + QUANT_ROWS - 1) / QUANT_ROWS);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
     if (a.n_cols <= 2048)
         go(i8_quantize_kernel<TYPE, NORM, 1>);
     else if (a.n_cols <= 6144)

@@ -294,3 +294,22 @@ def test_matrices_are_quantised_by_their_channels():
     # the products' rms; together 0.011.
     rms = np.sqrt(((got - X.astype(np.float64) @ W.astype(np.float64).T) ** 2).mean() / 512)
     assert rms < 0.02
+
+
+def test_as_many_rows_as_a_call_takes():
+    """2^24 rows of 16 values, and as many of a product with two channels, looked at in places."""
+    rows = 1 << 24
+    look = np.r_[0:70, (1 << 20) - 3:(1 << 20) + 3, (1 << 23) - 1:(1 << 23) + 1, rows - 70:rows]
+    rng = np.random.default_rng(1)
+    x = np.tile(rng.standard_normal((1 << 12, 16)).astype(np.float16), (1 << 12, 1))
+    x[look] = rng.standard_normal((len(look), 16)).astype(np.float16)
+    codes, scales = dev(np.full((rows, 16), 77, np.int8)), dev(np.full(rows, 5, np.float32))
+    int8.quantize(dev(x), codes, scales, rows, 16, type=int8.F16)
+    want, s = quantised(x[look])
+    c, sx = codes.to_array(np.int8, (rows, 16)), scales.to_array(np.float32, rows)
+    assert np.array_equal(c[look], want) and (np.abs(sx[look] - s) <= s * 2.0 ** -24).all()
+    w, sw = rng.integers(-127, 128, (2, 16)).astype(np.int8), np.ones(2, np.float32)
+    y = dev(np.full((rows, 2), 7, np.float32))
+    int8.matmul(codes, scales, dev(w), dev(sw), y, rows, 2, 16)
+    want, tol = product(c[look], sx[look], w, sw)
+    check(y.to_array(np.float32, (rows, 2))[look], want, tol, int8.F32)
