@@ -554,12 +554,21 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
             more[lane] = i32x4{u.end, u.x.gap.from, u.x.gap.skip, 0};
         }
     };
-    u = few_units<FORM>(a, gr, group, 0);
-    int total = u.sum;
-    for (int s0 = WAVE; s0 < a.n_seqs; s0 += WAVE) total += few_units<FORM>(a, gr, group, s0).sum;
-    const int per = few_per(a, total), end = min(total, (w + 1) * per);
+    // Whole windows: sequence w, if it is one of these, without a look at those before.
+    const bool one = FORM == PAGED_WINDOW && a.few.whole;
+    int s0 = one ? w / WAVE * WAVE : 0, before = 0, pos, end;
+    u = few_units<FORM>(a, gr, group, s0);
+    if (one) {
+        end = __builtin_amdgcn_readlane(u.end, w % WAVE);
+        pos = end - __builtin_amdgcn_readlane(u.n, w % WAVE);
+    } else {
+        int total = u.sum;
+        for (int s1 = WAVE; s1 < a.n_seqs; s1 += WAVE) total += few_units<FORM>(a, gr, group, s1).sum;
+        const int per = few_per(a, total);
+        pos = w * per;
+        end = min(total, pos + per);
+    }
     keep();
-    int pos = w * per, s0 = 0, before = 0;
     while (pos < end) {
         // The sequence that has unit pos, and where its units begin.
         const uint64_t past = __ballot(before + (FORM == PAGED_ALL ? u.end : more[lane][0]) > pos);
@@ -1759,7 +1768,7 @@ static PagedSplit split_slots(int64_t groups, int64_t want, int max_kv, int max_
 static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, int rows, int max_kv, int max_splits) {
     const int most = std::max(1, (max_kv + unit - 1) / unit);
     const int n = (int)std::min(std::max<int64_t>(1, want / n_kv), (int64_t)n_seqs * most);
-    return {n, unit, most < 2 ? 1 : (most - 2) / (max_splits - 1) + 1, twice, rows, 4};
+    return {n, unit, most < 2 ? 1 : (most - 2) / (max_splits - 1) + 1, twice, rows, 4, 0};
 }
 
 PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv, const PagedFormSizes& f) {
@@ -1814,7 +1823,7 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     const bool whole = f.form == PAGED_WINDOW && (big ? max_kv <= 1536 : waves > 0);
     const int unit = 4 * halves * ROWS_STEP;  // slots of a step of a workgroup of the chunk kernel
     if (whole)
-        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, big ? 4 : waves};
+        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, big ? 4 : waves, !big || n_seqs > DENSE};
     else if (big || p.pre_tiles)
         p.few = few_of(big ? 512 / halves : shares, unit, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     else

@@ -138,6 +138,20 @@ def test_windows_that_fill_the_gpu(fmt, type_, heads, n_kv, q_lens, kv_lens):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("window,sinks", [(40, 3), (200, 0), (700, 70)])
+def test_windows_of_many_sequences_beside_chunks(fmt, type_, window, sinks):
+    """Single tokens, drafts, chunks and sequences without tokens, more than a wave looks at, in any order."""
+    rng = np.random.default_rng(window)
+    q_lens = tuple(int(m) for m in rng.choice([1, 1, 1, 0, 5, 8, 9, 40], 150))
+    kv_lens = tuple(int(m + rng.integers(0, 900)) for m in q_lens)
+    pool, table = windowed(fmt, 2, 32, q_lens, kv_lens, window, sinks, rng)
+    q = rng.standard_normal((sum(q_lens), 4, D)).astype(NP[type_])
+    got = run_attention(pool, q, q_lens, kv_lens, table, type_, extra=2, cache=Form(pool, window=window, sinks=sinks))
+    check(pool, q, q_lens, kv_lens, table, got, type_, window, sinks)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
 def test_a_window_of_everything_is_the_plain_attention(fmt, type_):
     """To the bit: the same slots in the same steps."""
     rng = np.random.default_rng(5)
