@@ -280,7 +280,7 @@ struct PagedFew {
                                     // shares above `twice` doubled
     int rows;                       // upper bound of a sequence's query rows a KV head
     int waves;                      // of a workgroup, where these sequences have a kernel of their own: 4 or 8
-    int whole;                      // a unit has all that a sequence's rows see, and workgroup w has sequence w (windows)
+    int whole;                      // windows: workgroup w has sequence w, all of whose visible slots are a unit
 };
 struct PagedPlan {
     PagedFew few;                   // sequences of at most 16 query rows a KV head

@@ -1819,11 +1819,14 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     const int64_t pairs = (int64_t)n_seqs * n_kv, rounds = (pairs + 511) / 512;
     const int waves = pairs <= 256 && 5 * pairs >= 4 * 256 ? 8 : 5 * pairs >= 4 * 512 * rounds ? 4 : 0;
     // Beside prompts windows of up to 1536 slots are whole, too: 32 sessions, chunks of 100 tokens and single ones, 1000
-    // slots, 58 us for 63.  (Of 2048 q8 slots they end last: 109 us for 101.)
+    // slots, 58 us for 63.  (Of 2048 q8 slots they end last: 109 us for 101.)  Workgroup w has sequence w then, without a
+    // search (1024 single tokens 100 us, searched for 379; 600 sessions, chunks and single tokens, 299 and 430), but in
+    // smaller batches of both, where workgroups of chunks' numbers, which end at once, leave half the CUs idle (40
+    // sessions over q8 46 us, 40 searched for; 150 as long).
     const bool whole = f.form == PAGED_WINDOW && (big ? max_kv <= 1536 : waves > 0);
     const int unit = 4 * halves * ROWS_STEP;  // slots of a step of a workgroup of the chunk kernel
     if (whole)
-        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, big ? 4 : waves, !big || n_seqs > DENSE};
+        p.few = {n_seqs, (max_kv + 8 * ROWS_STEP - 1) / (8 * ROWS_STEP) * (8 * ROWS_STEP), 1, INT32_MAX, few, big ? 4 : waves, !big || n_seqs > 128};
     else if (big || p.pre_tiles)
         p.few = few_of(big ? 512 / halves : shares, unit, INT32_MAX, n_kv, n_seqs, few, max_kv, max_splits);
     else
