@@ -461,11 +461,20 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, const PrefixGrou
     y.sp = seq_span(a.q_start, a.kv_len, min(s, a.n_seqs - 1), a.n_tokens, a.max_kv);
     if (s >= a.n_seqs) y.sp = {0, 0, 0};
     if constexpr (FORM == PAGED_WINDOW) y.gap = window_gap(y.sp.n_kv - y.sp.n_q, y.sp.n_kv, a.f.window, a.f.sinks, 32);
-    if constexpr (FORM == PAGED_PREFIX)
-        for (int g = 0; g < a.f.n_groups; ++g) {
-            const int n = __builtin_amdgcn_readlane(gr.n, g), first = __builtin_amdgcn_readlane(gr.s0, g), last = __builtin_amdgcn_readlane(gr.s1, g);
-            if (n && s >= first && s < last) y.gap.skip = n;
+    if constexpr (FORM == PAGED_PREFIX) {
+        int first, last, n;
+        if (a.f.n_groups == 1) {
+            first = __builtin_amdgcn_readfirstlane(gr.s0), last = __builtin_amdgcn_readfirstlane(gr.s1), n = __builtin_amdgcn_readfirstlane(gr.n);
+        } else {  // the last group that begins at s or before
+            int g = 0;
+            for (int step = 1 << (31 - __builtin_clz(a.f.n_groups - 1)); step; step >>= 1) {
+                const int next = g + step, begin = __shfl(gr.s0, next % WAVE);
+                if (next < a.f.n_groups && begin <= s) g = next;
+            }
+            first = __shfl(gr.s0, g), last = __shfl(gr.s1, g), n = __shfl(gr.n, g);
         }
+        if (s >= first && s < last) y.gap.skip = n;
+    }
     return y;
 }
 // The last slot of a prefix of n slots that this lane's token t sees; true if all tokens of the group's sequences
