@@ -1780,6 +1780,11 @@ static PagedFew few_of(int64_t want, int unit, int twice, int n_kv, int n_seqs, 
     return {n, unit, most < 2 ? 1 : (most - 2) / (max_splits - 1) + 1, twice, rows, 4, 0};
 }
 
+// The most tiles that sequences of more rows may have.
+static int64_t big_tiles(int n_tokens, int group, int n_seqs) {
+    return (int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1));
+}
+
 PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, int max_q, int max_kv, const PagedFormSizes& f) {
     PagedPlan p{};
     const bool prefix = f.form == PAGED_PREFIX;
@@ -1796,28 +1801,39 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
         const int64_t rows = (int64_t)n_tokens * group, groups = std::min<int64_t>(f.n_groups, rows);
         const int64_t tiles = std::max<int64_t>(groups, (rows + 63 * groups) / CH_ROWS), steps = (f.max_prefix + 127) / 128;
         p.pre_tiles = (int)((rows + 127 * groups) / CH_ROWS);
+        // us of a tile's 128 slots, and of a sequence's 256; what sequences have of their own is six tenths of the most.
+        const double step = fmt == FMT_F16 ? 2.5 : 5., unit = fmt == FMT_F16 ? 3. : 3.5;
+        const int own = max_kv - f.max_prefix;
+        const int64_t wgs = tiles * n_kv;
+        double least = 1e30;
+        int64_t ranges = 1;
         if (big) {
-            p.pre = split_slots(1, 512 / halves / (tiles * n_kv), f.max_prefix, max_splits);
+            // Beside chunks: the least of the CUs' time for all tiles, or of the longest workgroup, and of what a range more
+            // costs to join.  (6 sessions, chunks of up to 300 tokens behind 1008 slots: 45 us with the two ranges that this
+            // takes, 40 with one, 51 with the three that fill the CUs; 4 sessions, chunks of 60 behind 3200: 26 us with 8
+            // ranges, 36 with 25.)
+            const double rest = (double)big_tiles(n_tokens, group, n_seqs) * n_kv * (8. + 0.6 * own / 128 * step);
+            const double join = 0.5 + (double)n_tokens * n_heads * (HD + 2) * 8 / 5e6;
+            for (int64_t n = 1; n <= std::min<int64_t>(steps, max_splits); ++n) {
+                const double longest = 8. + (steps + n - 1) / n * step, us = std::max(longest, (n * wgs * longest + rest) / 256) + n * join;
+                if (us < least) least = us, ranges = n;
+            }
         } else {
             // Beside few-row sequences: all workgroups at a time, one a CU, as many ranges of slots as end with the
-            // sequences' shares (us of a tile's 128 slots, and of a sequence's 256, of which there are six tenths of the
-            // most that there may be).  64 tokens behind 7680 slots 29 us with 10 ranges and 176 shares, 32 with 384
-            // shares in a second round; 20 sequences of 8 tokens and fp32 queries, three prefixes, over q8 65 us with 6
-            // ranges and 112 shares, 74 with 11 and 384.
-            const double step = fmt == FMT_F16 ? 2.5 : 5., unit = fmt == FMT_F16 ? 3. : 3.5;
-            const int64_t units = (int64_t)(n_seqs * std::max(1., 0.6 * (max_kv - f.max_prefix) / 256 + 0.5)), wgs = tiles * n_kv;
-            double least = 1e30;
-            int64_t ranges = 1;
+            // sequences' shares.  64 tokens behind 7680 slots 29 us with 10 ranges and 176 shares, 32 with 384 shares in a
+            // second round; 20 sequences of 8 tokens and fp32 queries, three prefixes, over q8 65 us with 6 ranges and 112
+            // shares, 74 with 11 and 384.
+            const int64_t units = (int64_t)(n_seqs * std::max(1., 0.6 * own / 256 + 0.5));
             for (int64_t n = 1; n <= std::min<int64_t>(steps, max_splits) && (n == 1 || n * wgs + n_kv <= 256); ++n) {
                 const int64_t share = std::max<int64_t>(1, (256 - n * wgs % 256) / n_kv);
                 const double us = 0.1 * n + std::max(8. + (steps + n - 1) / n * step, 6. + (units + share - 1) / share * unit);
                 if (us < least) least = us, ranges = n, shares = share * n_kv;
             }
-            p.pre = split_slots(1, ranges, f.max_prefix, max_splits);
         }
+        p.pre = split_slots(1, ranges, f.max_prefix, max_splits);
     }
     if (big) {
-        p.tiles = (int)((int64_t)n_tokens * group / CH_ROWS + std::min<int64_t>(n_seqs, (int64_t)n_tokens * group / (ROWS_TILE + 1)));
+        p.tiles = (int)big_tiles(n_tokens, group, n_seqs);
         // (Windows of up to 512 slots are not split: 1024 tokens, windows of 128: 18 us, 27 in two parts, joined.)
         p.big = split_slots((int64_t)p.tiles * n_kv, 512 / halves, max_kv, f.form == PAGED_WINDOW && max_kv <= 512 ? 1 : max_splits);
     }
