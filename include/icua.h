@@ -380,8 +380,8 @@ int icua_paged_attention_window_work(const icua_pages_t* pages, const icua_paged
 
 /* The same as icua_paged_attention for sequences that share their first slots: sequences group_start[g] ..
  * group_start[g + 1] - 1 have the same K/V in slots 0 .. prefix_len[g] - 1 (the same pages, as a rule), which are read
- * once for all of the group's tokens, through the table of its first sequence; kv_len and tables still count and hold
- * the shared slots of every sequence.  Sequences before the first group and behind the last one share nothing.  What a
+ * once for all of the group's tokens, through the table of its first sequence (if that has fewer slots, of the first one
+ * that has all of them, or the most); kv_len and tables still count and hold the shared slots of every sequence.  Sequences before the first group and behind the last one share nothing.  What a
  * token sees does not change: one that does not see all of the prefix (a sequence shorter than it, say) sees its part.
  * Slots are shared 128 at a time: up to 127 at the prefix's end are read by each sequence. */
 typedef struct {

@@ -944,12 +944,31 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& a, const PrefixGr
     return false;
 }
 
-// The same for the groups' tokens over their prefixes: the group's first sequence and the one behind its last.
-__device__ __forceinline__ bool find_prefix_tile(const PagedAttnArgs& a, const PrefixGroup& gr, int group, int index, int& s0, int& s1, int& tile, int& tiles, Span& span) {
-    int t0 = 0, t1 = 0;
+// The sequence of s0 .. s1 - 1 through whose table the group's first n slots are read, where s0 has fewer (an idle place,
+// a session that is still to get some of them): the first one with n slots, or of those with the most.
+__device__ __forceinline__ int longest_sequence(const PagedAttnArgs& a, int s0, int s1, int n) {
+    const int lane = threadIdx.x & 63;
+    int at = s0, most = 0;
+    for (int b = s0; b < s1 && most < n; b += WAVE) {
+        const int len = b + lane < s1 ? min(a.kv_len[b + lane], n) : 0;
+        int top = len;
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) top = max(top, __shfl_xor(top, o));
+        if (top > most) {
+            most = __builtin_amdgcn_readfirstlane(top);
+            at = b + __ffsll((unsigned long long)__ballot(len == top)) - 1;
+        }
+    }
+    return at;
+}
+
+// The same for the groups' tokens over their prefixes: sequences s0 .. s1 - 1, of which s has the table.
+__device__ __forceinline__ bool find_prefix_tile(const PagedAttnArgs& a, const PrefixGroup& gr, int group, int index, int& s, int& s0, int& s1, int& tile, int& tiles, Span& span) {
+    int t0 = 0, t1 = 0, slots = 0;
     if (gr.n) {
         t0 = min(max(a.q_start[gr.s0], 0), a.n_tokens);
         t1 = min(max(a.q_start[gr.s1], t0), a.n_tokens);
+        slots = a.kv_len[gr.s0];
     }
     const int n = ((t1 - t0) * group + CH_ROWS - 1) / CH_ROWS;
     for (int g = 0; g < a.f.n_groups; ++g) {
@@ -959,6 +978,7 @@ __device__ __forceinline__ bool find_prefix_tile(const PagedAttnArgs& a, const P
             s1 = __builtin_amdgcn_readlane(gr.s1, g);
             tile = index;
             span = {{__builtin_amdgcn_readlane(t0, g), __builtin_amdgcn_readlane(t1, g) - __builtin_amdgcn_readlane(t0, g), __builtin_amdgcn_readlane(gr.n, g)}, {0, 0}};
+            s = __builtin_amdgcn_readlane(slots, g) >= span.sp.n_kv ? s0 : longest_sequence(a, s0, s1, span.sp.n_kv);
             return true;
         }
         index -= tiles;
@@ -994,9 +1014,9 @@ __global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_w
     }
     const int g = index % a.map.n_kv, at = index / a.map.n_kv, split = at % parts.n;
     const PrefixGroup gr = load_groups<FORM>(a);
-    int s, tile, tiles, group_s1 = 0;
+    int s, tile, tiles, group_s0 = 0, group_s1 = 0;
     Span span;
-    if (!(pre ? find_prefix_tile(a, gr, group, at / parts.n, s, group_s1, tile, tiles, span) : find_tile<FORM>(a, gr, group, CH_ROWS, at / parts.n, s, tile, tiles, span))) return;
+    if (!(pre ? find_prefix_tile(a, gr, group, at / parts.n, s, group_s0, group_s1, tile, tiles, span) : find_tile<FORM>(a, gr, group, CH_ROWS, at / parts.n, s, tile, tiles, span))) return;
     tile = tiles - 1 - tile;  // those that see the most slots first
     const SeqSpan sp = span.sp;
     const int before = sp.n_kv - sp.n_q;  // token i sees slots up to before + i
@@ -1204,7 +1224,7 @@ __global__ __launch_bounds__(256 * ch_halves(FORM, FMT)) __attribute__((amdgpu_w
         look_at_pages(max(c0, gap.from) + gap.skip, c1 + gap.skip);
     }
     if constexpr (FORM == PAGED_PREFIX)
-        if (pre && !prefix_last(a, s, group_s1, lim, row.t, row.last)) w_first = all_seen = __builtin_amdgcn_readfirstlane(-1);
+        if (pre && !prefix_last(a, group_s0, group_s1, lim, row.t, row.last)) w_first = all_seen = __builtin_amdgcn_readfirstlane(-1);
     if (it0 < it1) staged(it0);
 
     f32x16 O[4];
