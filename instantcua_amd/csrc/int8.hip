@@ -191,13 +191,24 @@ hipError_t quantize_of(const I8QuantArgs& a, hipStream_t s) {
 
 __device__ __constant__ const u32x4 g_zero_codes = {0, 0, 0, 0};  // what lies behind a row's last code
 
-// g / (1 + exp(-g)) u, by e = exp(-|g|) <= 1: g / (1 + e) u for g >= 0, e g / (1 + e) u else.  The exponential carries
-// 2^32, and u its inverse, so that neither it nor the reciprocal leaves fp32's normal numbers (the instructions make
-// others zero) where the result is one.
+// g / (1 + exp(-g)) u, by e = exp(-|g|) <= 1: g / (1 + e) u for g >= 0, e g / (1 + e) u else.  Up to |g| = GATE_NEAR
+// e is a normal number of fp32 (the instructions make others zero), and so is what it is multiplied with: u comes last,
+// whose product is below fp32's range where the result is.
+constexpr float GATE_NEAR = 80.f;
 __device__ __forceinline__ float gated_up(float g, float u) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(fabsf(g), -1.4426950408889634f, 32.f));
-    const float s = __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0x1p-32f, 1.f));
-    return g * s * (u * 0x1p-32f) * (g >= 0.f ? 0x1p32f : e);
+    const float e = __builtin_amdgcn_exp2f(fabsf(g) * -1.4426950408889634f);
+    const float s = __builtin_amdgcn_rcpf(1.f + e);
+    return g * s * (g >= 0.f ? 1.f : e) * u;
+}
+// The same for gates of any size: e = x 2^n, and for g < 0 the power goes to the product in two parts, before u, where
+// the product is below 1, and behind it.
+__device__ __forceinline__ float gated_up_far(float g, float u) {
+    const float n = fmaxf(__builtin_rintf(fabsf(g) * -1.4426950408889634f), -1000.f);
+    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(fabsf(g), -1.4426950408889634f, -n));
+    const int i = (int)n, half = i >> 1;
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_ldexpf(x, i));
+    if (!(g < 0.f)) return g * s * u;
+    return __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(g * s * x, half) * u, i - half);
 }
 
 // A tile of BM tokens and BN matrix rows a workgroup, WM x WN of it a wave, on v_mfma_i32_32x32x32_i8 (twice the rate
@@ -393,12 +404,27 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * KW * 64) void i8_matmul_kerne
 #pragma unroll
                 for (int e = 0; e < 16; ++e) add[e] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(add0, at + (8 * (e / 4) + e % 4) * add_row, 0, 0));
             }
+            float value[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) value[e] = (float)acc[i][j][e] * sx[e / 4][e % 4] * sw[j];
+            if constexpr (GATED) {
+                float up[16], top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    up[e] = (float)acc[i][j + NO][e] * sx[e / 4][e % 4] * su[j];
+                    top = fmaxf(top, fabsf(value[e]));
+                }
+                if (__builtin_expect(__ballot(top > GATE_NEAR) != 0, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) value[e] = gated_up_far(value[e], up[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) value[e] = gated_up(value[e], up[e]);
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                float y = (float)acc[i][j][e] * sx[e / 4][e % 4] * sw[j];
-                if constexpr (GATED) {
-                    y = gated_up(y, (float)acc[i][j + NO][e] * sx[e / 4][e % 4] * su[j]);
-                }
+                float y = value[e];
                 if (a.add) y += add[e];
                 const uint32_t at = y_at + (8 * (e / 4) + e % 4) * y_row;
                 if constexpr (TYPE == TYPE_F32)
@@ -531,7 +557,10 @@ __global__ __launch_bounds__(512) void i8_stream_kernel(I8MatmulArgs a) {
 #pragma unroll
             for (int w = 0; w < NW; ++w) sum[s] += s_sum[w][s * RB * MB + block][at];
         float y = (float)sum[0] * sx[i] * sw[i];
-        if constexpr (GATED) y = gated_up(y, (float)sum[SETS - 1] * sx[i] * su[i]);
+        if constexpr (GATED) {
+            const float up = (float)sum[SETS - 1] * sx[i] * su[i];
+            y = fabsf(y) > GATE_NEAR ? gated_up_far(y, up) : gated_up(y, up);
+        }
         if (a.add) y += add[i];
         const int64_t o = (int64_t)(m0 + m) * a.y_stride + n0 + n;
         if constexpr (TYPE == TYPE_F32)

@@ -1,0 +1,55 @@
+"""GPU tests of the products on 8-bit integers at the ends of fp32's range: gates and ups of any size together, rows
+of zeros, quotients that only exact arithmetic tells from a tie."""
+import numpy as np
+import pytest
+
+from instantcua_amd import int8
+from test_gpu_int8 import run_matmul
+
+pytestmark = pytest.mark.gpu
+
+NEAR = [5, -5, 0.01, -0.7, -30, 30, -79, 79, 1e-30, -1e-20]
+FAR = [-81, -88, -100, -104, -115, -150, -200, 81, 200, 1e20, -1e20]
+UPS = [1, -64, 1e-30, 1e-33, 2e-36, -2e-37, 1e-38, 1e-40, 2.0 ** -149, 1e20, 1e30, -3e38]
+
+
+@pytest.mark.parametrize("m", [1, 20, 150, 1100])
+@pytest.mark.parametrize("gates", [NEAR, FAR, NEAR + FAR])
+def test_gates_and_ups_of_any_size(m, gates):
+    """Sums of one, so that gates and ups are the scales.  The exponent of e = exp(-|g|) is 1.5 |g| 2^-24 off (its
+    constant and a rounding), e 2^-23 more (the instruction), 1 + e 2^-24, its inverse 2^-23, three products 2^-24 each:
+    1.5 |g| + 8 in all, and two roundings to fp32's smallest step."""
+    g, u = (np.asarray(a, np.float32) for a in zip(*[(a, b) for a in gates for b in UPS]))
+    n = len(g)
+    x, w = np.zeros((m, 32), np.int8), np.zeros((2 * n, 32), np.int8)
+    x[:, 3], w[:, 3] = 1, 1
+    got = run_matmul(x, np.ones(m, np.float32), w, np.concatenate([g, u]), gated=True)
+    a, b = g.astype(np.float64), u.astype(np.float64)
+    # exp(-|g|) of these leaves no double but for the largest gates, where the result is zero.
+    want = a * np.where(a < 0, np.exp(-np.abs(a)), 1) / (1 + np.exp(-np.abs(a))) * b
+    tol = (1.5 * np.abs(np.where(np.abs(a) < 1e3, a, 0)) + 8) * 2.0 ** -24 * np.abs(want) + 2.0 ** -149
+    most = float(np.finfo(np.float32).max)
+    over = np.abs(want) > most
+    assert (np.abs(want[~over]) < most * (1 - 2.0 ** -10)).all()
+    assert (got[:, over] == np.sign(want[over]) * np.inf).all()
+    err = np.abs(got[:, ~over].astype(np.float64) - want[~over])
+    bad = err - tol[~over]
+    assert np.isfinite(got[:, ~over]).all() and (bad <= 0).all(), (g[~over][bad.max(0).argmax()], u[~over][bad.max(0).argmax()], float(err.max()))
+
+
+@pytest.mark.parametrize("m", [1, 150])
+def test_gates_and_ups_that_are_no_numbers(m):
+    """As the definition has them: g / (1 + exp(-g)) u."""
+    inf, nan = np.inf, np.nan
+    pairs = [(nan, 1), (1, nan), (inf, 2), (inf, 0), (-inf, 1), (-3, inf), (3, -inf), (0, inf), (-200, inf), (2, 3)]
+    g, u = (np.asarray(a, np.float32) for a in zip(*pairs))
+    n = len(g)
+    x, w = np.zeros((m, 16), np.int8), np.ones((2 * n, 16), np.int8)
+    x[:, 0] = 1
+    with np.errstate(all="ignore"):
+        a = g.astype(np.float64)
+        want = a / (1 + np.exp(-a)) * u
+    got = run_matmul(x, np.ones(m, np.float32), w, np.concatenate([g, u]), gated=True)
+    assert np.array_equal(np.isnan(got), np.broadcast_to(np.isnan(want), got.shape))
+    some = np.isinf(want)
+    assert (got[:, some] == want[some]).all() and abs(got[0, -1] - want[-1]) < 1e-5
