@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(I8QuantArgs a) {
     if (threadIdx.x == 0) {
         sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
         const double r = NORM ? 1. / sqrt(sum / a.n_cols + (double)a.eps) : 1.;
-        a.scales[row] = none ? __builtin_nanf("") : (float)(top * r / 127.);
+        a.scales[row] = none ? __builtin_nanf("") : top == 0. ? 0.f : (float)(top * r / 127.);  // (r of zeros may be infinite)
     }
     const double to = none || top == 0. ? 0. : 127. / top;
     const bool middle = to == 0. || (top > 0x1p-60 && top < 0x1p60);  // no product of fp32 values leaves its range

@@ -1,10 +1,10 @@
 """GPU tests of the products on 8-bit integers at the ends of fp32's range: gates and ups of any size together, rows
-of zeros, quotients that only exact arithmetic tells from a tie."""
+of zeros."""
 import numpy as np
 import pytest
 
 from instantcua_amd import int8
-from test_gpu_int8 import run_matmul
+from test_gpu_int8 import quantised, run_matmul, run_quantize
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,22 @@ def test_gates_and_ups_that_are_no_numbers(m):
     assert np.array_equal(np.isnan(got), np.broadcast_to(np.isnan(want), got.shape))
     some = np.isinf(want)
     assert (got[:, some] == want[some]).all() and abs(got[0, -1] - want[-1]) < 1e-5
+
+
+@pytest.mark.parametrize("type", [int8.F32, int8.F16])
+@pytest.mark.parametrize("cols", [16, 2064, 6160, 16400])
+def test_rows_of_zeros_without_eps(type, cols):
+    """Their codes and scales are zero, with and without a norm; other rows need no eps."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((5, cols)).astype(np.float16).astype(np.float32)
+    x[1], x[4] = 0, -0.0
+    norm = rng.uniform(0.5, 2, cols).astype(np.float32)
+    for w in (None, norm):
+        codes, scales = run_quantize(x, w, type=type, eps=0.0)
+        assert (codes[[1, 4]] == 0).all() and (scales[[1, 4]] == 0).all()
+        rest = [0, 2, 3]
+        want, s = quantised(x[rest], w, eps=0.0)
+        assert np.array_equal(codes[rest], want) and (np.abs(scales[rest] - s) <= s * 2.0 ** -23).all()
+    # And through a product: zeros, not values that are no numbers.
+    y = run_matmul(codes, scales, np.ones((3, cols), np.int8), np.ones(3, np.float32))
+    assert (y[[1, 4]] == 0).all() and np.isfinite(y).all()
