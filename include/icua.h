@@ -231,7 +231,7 @@ enum { ICUA_TYPE_F32 = 0, ICUA_TYPE_F16 = 1 };
 
 /* Codes and scales of rows: y = x / sqrt(mean(x^2) + eps) * norm (norm NULL: y = x, eps is not used),
  *   scale = max |y| / 127,  code = 127 y / max |y|, rounded to the nearest, ties to even:
- * -127 .. 127, and exactly those of the definition (the arithmetic is 64-bit).  A row of zeros has codes and scale
+ * -127 .. 127, and exactly those of the definition (the arithmetic is 64-bit, and exact next to ties).  A row of zeros has codes and scale
  * zero; a row with an infinity or NaN (in y) has codes zero and a scale that is no number.
  * Scales beyond fp32's range become 0 or infinite. */
 typedef struct {

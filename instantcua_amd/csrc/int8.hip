@@ -19,7 +19,19 @@ typedef f16 v8h __attribute__((ext_vector_type(8)));
 // without it: code = 127 t / max |t| of t = x norm.  The maximum, its scale and the mean are of 64 bits, where t is
 // exact.  A quotient t (127 / max) in fp32 is less than 3 2^-24 of its at most 127 off, 2.3e-5: it rounds as the exact
 // one but within 4e-5 of half way between two codes (and in rows whose maximum is not near fp32's middle), where the
-// 64-bit one decides, and at 2^-40 from a tie the division itself: codes are those of the definition.
+// 64-bit one decides, and within 2^-40 of it, where that may be off too, the exact sign of 254 t - (2 k + 1) max |t|:
+// codes are those of the definition.  (Without a norm t has 24 bits, quotients that are no ties are 2^-25 from one, and a
+// division tells them.)
+
+// t 127 / top to the nearest, ties to even, for a quotient next to half way between two codes.  Values are products of
+// two fp32 numbers, so that the difference of the two products below is a few steps of the last place of either.
+__device__ __forceinline__ double code_next_to_tie(double t, double top, double q) {
+#pragma clang fp contract(off)  // a and b are the rounded products
+    const double below = floor(q), odd = 2. * below + 1.;
+    const double a = 254. * t, b = odd * top;
+    const double off = (a - b) + (fma(254., t, -a) - fma(odd, top, -b));
+    return off > 0. ? below + 1. : off < 0. ? below : 2. * __builtin_rint(0.5 * below + 0.25);
+}
 
 // Eight values.
 template <int TYPE>
@@ -150,7 +162,7 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(I8QuantArgs a) {
             for (int e = 0; e < 8; ++e) {
                 const double t = NORM ? (double)x[k][e] * (double)w[k][e] : (double)x[k][e], q = t * to;
                 double r = __builtin_rint(q);
-                if (__builtin_expect(fabs(q - r) > 0.5 - 0x1p-40, 0)) r = __builtin_rint(t * 127. / top);
+                if (__builtin_expect(fabs(q - r) > 0.5 - 0x1p-40, 0)) r = NORM ? code_next_to_tie(t, top, q) : __builtin_rint(t * 127. / top);
                 code[e] = (int)r;
             }
         }

@@ -1,5 +1,8 @@
 """GPU tests of the products on 8-bit integers at the ends of fp32's range: gates and ups of any size together, rows
-of zeros."""
+of zeros, quotients that only exact arithmetic tells from a tie."""
+import math
+import random
+
 import numpy as np
 import pytest
 
@@ -72,3 +75,41 @@ def test_rows_of_zeros_without_eps(type, cols):
     # And through a product: zeros, not values that are no numbers.
     y = run_matmul(codes, scales, np.ones((3, cols), np.int8), np.ones(3, np.float32))
     assert (y[[1, 4]] == 0).all() and np.isfinite(y).all()
+
+
+def next_to_ties(n, seed):
+    """n of (x, norm, largest x, k, off) and the largest's norm: 254 x norm = (2 k + 1) largest + off, of 24-bit numbers
+    and |off| of at most 16, so that the quotient 127 x norm / largest is k + 1/2 but for off / (2 largest), 2^-43 or less."""
+    rng = random.Random(seed)
+    top_norm, found = rng.randrange(1 << 23, 1 << 24) | 1, []
+    while len(found) < n:
+        norm = rng.randrange(1 << 23, 1 << 24) | 1
+        for k in range(20, 127):
+            p, m = 254 * norm, (2 * k + 1) * top_norm
+            g = math.gcd(p, m)
+            for off in (i * g for i in (-2, -1, 1, 2) if abs(i) * g <= 16):
+                for x in range(off // g * pow(p // g, -1, m // g) % (m // g), 1 << 24, m // g):
+                    top = (p * x - off) // m
+                    if 1 << 22 <= top < 1 << 24 and x >= 1 << 20:
+                        found.append((x, norm, top, k, off))
+    return top_norm, found[:n]
+
+
+@pytest.mark.parametrize("size", [0, -70, 20])
+def test_quotients_closer_to_ties_than_64_bits_tell(size):
+    """In whole numbers: the nearest code, where 127 x norm / largest in 64 bits is a tie; and exact ties, to even."""
+    top_norm, found = next_to_ties(300, 4)
+    rows, cols = len(found), -(-(len(found) + 2) // 16) * 16
+    x, norm, want = np.zeros((rows, cols), np.float32), np.ones(cols, np.float32), np.zeros((rows, cols), np.int8)
+    norm[0], want[:, 0], odd = top_norm, 127, 0
+    for i, (a, b, top, k, off) in enumerate(found):
+        sign = -1 if i % 2 else 1
+        x[i, 0], x[i, 1 + i], norm[1 + i], want[i, 1 + i] = top, sign * a, b, sign * (k + (off > 0))
+        odd += int(np.rint(a * b * 127.0 / (top * top_norm))) != k + (off > 0)
+    assert odd > 3  # some of them are what they are for
+    x[5, :], want[5, :] = 0, 0
+    x[5, 0], x[5, -1], want[5, 0], want[5, -1] = 254, 3, 127, 0
+    norm[-1] = top_norm  # 254 and 3: 1.5, to 2
+    want[5, -1] = 2
+    codes, _ = run_quantize((x * 2.0 ** (size - 24)).astype(np.float32), (norm * 2.0 ** -24).astype(np.float32))
+    assert np.array_equal(codes, want), np.argwhere(codes != want)[:5]
