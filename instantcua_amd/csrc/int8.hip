@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "icua_device.h"
+#include "icua_int8.h"
 #include "icua_kernels.h"
 
 namespace icua {
@@ -460,16 +461,6 @@ hipError_t matmul_tiles(const I8MatmulArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Tiles of 128 x 256: three stages where they fill the CUs and are deep, so that memory is waited for less (4096 tokens
-// of 2048 channels, 6144 deep, with their quantisation: 78 us, 87 with two; added to fp32 rows 90 and 97), else two
-// (2048 tokens, added: 52.5 us, 54 with three).
-template <int TYPE, bool GATED>
-hipError_t matmul_wide(const I8MatmulArgs& a, hipStream_t s) {
-    const int64_t tiles = (int64_t)((a.n_rows + 127) / 128) * ((a.n_out + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
-    if (tiles >= 192 && a.n_in >= 6144) return matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 3>(a, s);
-    return matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 2>(a, s);
-}
-
 // Few tokens: a matrix value takes part in few products, and goes from memory to registers.  A workgroup has ROWS matrix
 // rows (gated: as many gates and their ups) and 16 MB tokens; its eight waves take 128 codes of all rows in turn, on
 // v_mfma_i32_16x16x64_i8 (matrix rows as the result's rows, tokens as its columns), and join their sums through LDS.  A
@@ -588,59 +579,29 @@ hipError_t matmul_stream(const I8MatmulArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Which form a call takes: that of the least time by a model of each,
-//   start + n each + steps max(late ceil(n / beside), busy n)  us,
-// n tiles a CU (256 CUs), steps of 128 codes a wave group, `beside` tiles that a CU holds at a time, `late` the time of
-// a step that waits for memory, `busy` of one that has the CU to itself.  The four times are fitted to each form's
-// measured ones over 8 to 4096 tokens, 1024 to 12288 channels and depths of 1024 to 6144 (root mean square of their
-// ratios 5 to 16 %); the form taken is 3 % slower than the best one on average.  128 x 128 tiles alone: 12.6 us for 64
-// tokens, 4096 channels, 2048 deep, where 32 x 32 tiles take 5.6, and 133 us for 4096 tokens of gated 6144, where 256 x
-// 256 tiles take 107; 256 x 256 tiles alone 23 us for the former.
-struct Form {
-    int tokens, channels, parts, beside;
-    float start, each, late, busy;
-    float time(const I8MatmulArgs& a) const {
-        const int64_t tiles = (int64_t)((a.n_rows + tokens - 1) / tokens) * ((a.n_out + channels - 1) / channels);
-        const float n = (float)((tiles + 255) / 256), rounds = (float)((tiles + 256 * beside - 1) / (256 * beside));
-        const int steps = ((a.n_in + 127) / 128 + parts - 1) / parts;
-        return start + n * each + steps * std::max(late * rounds, busy * n);
-    }
-};
-
 template <int TYPE, bool GATED>
 hipError_t matmul_of(const I8MatmulArgs& a, hipStream_t s) {
-    struct Choice {
-        Form f;
-        hipError_t (*go)(const I8MatmulArgs&, hipStream_t);
-    };
-    constexpr int G = GATED ? 2 : 1;  // matrix rows of an output channel
-    static const Choice stream[] = {
-        {{16, 16, 8, 2, 2.05f, 0.13f, 0.835f, 0.864f}, matmul_stream<TYPE, GATED, 1, 1, 2>},
-        {{32, 16, 8, 2, 2.18f, 0.13f, 1.164f, 1.183f}, matmul_stream<TYPE, GATED, 1, 2, 2>},
-    };
-    static const Choice tiles[] = {
-        {{64, 128 / G, 1, 2, 1.59f, 2.40f, 0.433f, 0.363f}, matmul_tiles<TYPE, GATED, 64, 128, 32, 64, 1, 3>},
-        {{128, 128 / G, 1, 2, 0.12f, 3.51f, 0.686f, 0.572f}, matmul_tiles<TYPE, GATED, 128, 128, 64, 64, 1, 2>},
-        {{128, 256 / G, 1, 1, 0.00f, 4.79f, 0.111f, 0.910f}, matmul_wide<TYPE, GATED>},
-        {{256, 256 / G, 1, 1, 0.00f, 8.11f, 1.219f, 0.631f}, matmul_tiles<TYPE, GATED, 256, 256, 128, 64, 1, 2>},
-    };
-    const Choice* best = nullptr;
-    auto look = [&](const Choice& c) {
-        if (!best || c.f.time(a) < best->f.time(a)) best = &c;
-    };
-    if (a.n_rows <= 128)  // (and many more would be many small workgroups)
-        for (const Choice& c : stream) look(c);
-    for (const Choice& c : tiles) look(c);
-    if constexpr (!GATED) {  // waves of 32 x 32, which do not hold gates and ups
-        static const Choice small[] = {
-            {{32, 32, 8, 1, 0.77f, 2.56f, 0.990f, 0.878f}, matmul_tiles<TYPE, GATED, 32, 32, 32, 32, 8, 2>},
-            {{32, 64, 4, 1, 0.04f, 3.74f, 0.617f, 0.639f}, matmul_tiles<TYPE, GATED, 32, 64, 32, 32, 4, 3>},
-            {{64, 64, 1, 2, 1.79f, 1.47f, 0.296f, 0.221f}, matmul_tiles<TYPE, GATED, 64, 64, 32, 32, 1, 4>},
-            {{64, 64, 1, 4, 0.57f, 1.25f, 0.487f, 0.212f}, matmul_tiles<TYPE, GATED, 64, 64, 32, 32, 1, 2>},
-        };
-        for (const Choice& c : small) look(c);
+    const I8FormId form = i8_form(GATED, a.n_rows, a.n_out, a.n_in);
+    switch (form) {
+        case I8_STREAM_16: return matmul_stream<TYPE, GATED, 1, 1, 2>(a, s);
+        case I8_STREAM_32: return matmul_stream<TYPE, GATED, 1, 2, 2>(a, s);
+        case I8_64x128: return matmul_tiles<TYPE, GATED, 64, 128, 32, 64, 1, 3>(a, s);
+        case I8_128x128: return matmul_tiles<TYPE, GATED, 128, 128, 64, 64, 1, 2>(a, s);
+        case I8_128x256: return matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 2>(a, s);
+        case I8_128x256_DEEP: return matmul_tiles<TYPE, GATED, 128, 256, 64, 64, 1, 3>(a, s);
+        case I8_256x256: return matmul_tiles<TYPE, GATED, 256, 256, 128, 64, 1, 2>(a, s);
+        default: break;
     }
-    return best->go(a, s);
+    if constexpr (!GATED) {  // waves of 32 x 32, which do not hold gates and ups
+        switch (form) {
+            case I8_32x32: return matmul_tiles<TYPE, GATED, 32, 32, 32, 32, 8, 2>(a, s);
+            case I8_32x64: return matmul_tiles<TYPE, GATED, 32, 64, 32, 32, 4, 3>(a, s);
+            case I8_64x64_DEEP: return matmul_tiles<TYPE, GATED, 64, 64, 32, 32, 1, 4>(a, s);
+            case I8_64x64: return matmul_tiles<TYPE, GATED, 64, 64, 32, 32, 1, 2>(a, s);
+            default: break;
+        }
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
