@@ -1,4 +1,4 @@
-"""GPU tests of attention with shared prefixes where the group's first sequence does not hold them, against the
+"""GPU tests of attention with shared prefixes in as many groups as a call takes, and where a group's first sequence does not hold its, against the
 float64 definition: idle places, sessions that are still to get the prefix, tables with other sequences' pages behind
 the slots in use."""
 import os
@@ -60,3 +60,20 @@ def test_the_first_sequence_lacks_the_prefix(fmt, type_, lens, starts, prefixes)
         q = rng.standard_normal((sum(q_lens), heads, D)).astype(NP[type_])
         got = run_attention(pool, q, q_lens, kv_lens, table, type_, extra=1, cache=Form(pool, starts=starts, lens=prefixes, max_prefix=max(prefixes)))
         check(pool, q, q_lens, kv_lens, table, got, type_, chunk=True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("n_groups,seqs,q_choice", [(64, 200, [1]), (64, 150, [1, 1, 0, 3, 9, 30]), (33, 140, [1, 8]), (17, 70, [1, 1, 40]), (2, 130, [1, 0, 5]), (63, 64, [1, 2])])
+def test_many_groups(fmt, type_, n_groups, seqs, q_choice):
+    """Groups of none, one and several sequences, sequences in front of the first and behind the last, of any lengths."""
+    rng = np.random.default_rng(n_groups + seqs)
+    starts = [int(s) for s in np.sort(rng.integers(2, seqs - 1, n_groups + 1))]
+    prefixes = [int(p) for p in rng.choice([100, 128, 200, 256, 300, 400], n_groups)]
+    q_lens = [int(m) for m in rng.choice(q_choice, seqs)]
+    kv_lens = [int(rng.integers(0, 700)) if rng.random() < 0.3 else int(400 + m + rng.integers(0, 200)) for m in q_lens]
+    heads, n_kv, page = (4, 2, 32) if n_groups % 2 else (3, 1, 16)
+    pool, table = grouped(fmt, n_kv, page, kv_lens, starts, prefixes, rng)
+    q = rng.standard_normal((sum(q_lens), heads, D)).astype(NP[type_])
+    got = run_attention(pool, q, q_lens, kv_lens, table, type_, extra=2, cache=Form(pool, starts=starts, lens=prefixes, max_prefix=400))
+    check(pool, q, q_lens, kv_lens, table, got, type_, chunk=True)
