@@ -308,7 +308,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * KW * 64) void i8_matmul_kerne
 #pragma unroll
     for (int it = 0; it < NS; ++it)
         if (it < mine) stage(it);
-    // What the outputs take is asked for behind the first codes, and waited for after the products.
+    // What the outputs take is asked for behind the first codes, and waited for with them.
     constexpr int NO = WOUT / 32, SIZE = TYPE == TYPE_F32 ? 4 : 2;
     const int first_m = m0 + wm * WM, first_n = n0 + wn * WOUT;
     static_assert(BM <= THREADS * KW);

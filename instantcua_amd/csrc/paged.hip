@@ -613,8 +613,9 @@ __device__ __forceinline__ void rows_work(const PagedAttnArgs& a, int index, uin
         const SlotGap gap = {FORM == PAGED_WINDOW ? x[1] : 0, x[2]};
         const bool joined = FORM == PAGED_PREFIX && gap.skip > 0;  // to its prefix's part
         const int c1 = min(FORM == PAGED_ALL ? lim : max(0, lim - gap.skip), start + count * a.few.unit);  // of numbers without the gap
-        // Whether this lane's row sees a slot, and whether no row does.  (Without short cuts: selects, no branches.
-        // With them the compiler, ROCm 7.2's, left out the select of -inf for slots before the window.)
+        // Whether this lane's row sees a slot, and whether no row does.  (Without short cuts: selects, no branches.  Where
+        // p[i] = -inf comes after branches inside branches, the compiler, ROCm 7.2's, joins the copies of p's tuple of
+        // registers so that the write is lost: its block is an s_and_saveexec with its s_or right behind it, empty.)
         auto sees = [&](int slot) __attribute__((always_inline)) -> bool {
             if constexpr (FORM != PAGED_WINDOW) return slot <= row.last;
             return (slot <= row.last) & ((slot < a.f.sinks) | (slot > row.last - a.f.window));
@@ -865,8 +866,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // rows 32 (w & 3) .. + 31 and of each 128 slots the half w >> 2; the two halves keep softmax states of their
 // own, joined through LDS at the end.  (Windows over fp16 slots: four waves and 64 slots, two workgroups a CU, so
 // that one's first loads and last stores are under the other's products: a prompt of 4096 tokens through a window of
-// 512 and 16 first slots 44 us, where eight waves take 51, with fp32 queries 57 and 67.  q8 has registers for eight
-// only, 156 us of a batch that takes 100; one group's prefix beside 64 tokens 35 us for 32.)
+// 512 and 16 first slots 38 us, where eight waves take 45, with fp32 queries 54 and 65.  q8 has registers for eight
+// only, 156 us of a batch that took 100; one group's prefix beside 64 tokens 35 us for 32.)
 //
 // v_mfma_f32_32x32x16_f16, transposed as above: 32 query rows as columns, lane (column, h) has slots
 // 8 b + 4 h + 0 .. 3 of a 32-slot block, b = 0 .. 3; V^T operands come from row-major V by transposing LDS reads.
@@ -1854,7 +1855,8 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     }
     if (big) {
         p.tiles = (int)big_tiles(n_tokens, group, n_seqs);
-        // (Windows of up to 512 slots are not split: 1024 tokens, windows of 128: 18 us, 27 in two parts, joined.)
+        // (Windows that go through up to 512 slots, 258 and no first ones, are not split: 1024 tokens, windows of 128: 18
+        // us, 27 in two parts, joined.)
         p.big = split_slots((int64_t)p.tiles * n_kv, 512 / halves, max_kv, f.form == PAGED_WINDOW && max_kv <= 512 ? 1 : max_splits);
     }
     // Windows are much of one length: where the (sequence, KV head) pairs fill 256 workgroups of eight waves, or whole
@@ -1863,8 +1865,8 @@ PagedPlan paged_plan(int fmt, int n_heads, int n_kv, int n_seqs, int n_tokens, i
     // and 96 short ones, 41 us and 44 in three rounds of 256, are in even shares.)
     const int64_t pairs = (int64_t)n_seqs * n_kv, rounds = (pairs + 511) / 512;
     const int waves = pairs <= 256 && 5 * pairs >= 4 * 256 ? 8 : 5 * pairs >= 4 * 512 * rounds ? 4 : 0;
-    // Beside prompts windows of up to 1536 slots are whole, too: 32 sessions, chunks of 100 tokens and single ones, 1000
-    // slots, 58 us for 63.  (Of 2048 q8 slots they end last: 109 us for 101.)  Workgroup w has sequence w then, without a
+    // Beside prompts windows that go through up to 1536 slots, 1282 and no first ones, are whole, too: 32 sessions, chunks
+    // of 100 tokens and single ones, windows of 1000, 58 us for 63.  (Of 2048 over q8 they end last: 109 us for 101.)  Workgroup w has sequence w then, without a
     // search (1024 single tokens 100 us, searched for 379; 600 sessions, chunks and single tokens, 299 and 430), but in
     // smaller batches of both, where workgroups of chunks' numbers, which end at once, leave half the CUs idle (40
     // sessions over q8 46 us, 40 searched for; 150 as long).

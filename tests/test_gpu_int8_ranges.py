@@ -79,7 +79,8 @@ def test_rows_of_zeros_without_eps(type, cols):
 
 def next_to_ties(n, seed):
     """n of (x, norm, largest x, k, off) and the largest's norm: 254 x norm = (2 k + 1) largest + off, of 24-bit numbers
-    and |off| of at most 16, so that the quotient 127 x norm / largest is k + 1/2 but for off / (2 largest), 2^-43 or less."""
+    and |off| of at most 16, so that the quotient 127 x norm / largest is k + 1/2 but for off / (2 largest), 2^-42 or
+    less."""
     rng = random.Random(seed)
     top_norm, found = rng.randrange(1 << 23, 1 << 24) | 1, []
     while len(found) < n:

@@ -1,6 +1,6 @@
-"""GPU tests of attention with shared prefixes in as many groups as a call takes, and where a group's first sequence does not hold its, against the
-float64 definition: idle places, sessions that are still to get the prefix, tables with other sequences' pages behind
-the slots in use."""
+"""GPU tests of attention with shared prefixes in as many groups as a call takes, and where a group's first sequence
+does not hold its prefix, against the float64 definition: idle places, sessions that are still to get the prefix,
+tables with other sequences' pages behind the slots in use."""
 import os
 import sys
 
