@@ -77,3 +77,25 @@ def test_many_groups(fmt, type_, n_groups, seqs, q_choice):
     q = rng.standard_normal((sum(q_lens), heads, D)).astype(NP[type_])
     got = run_attention(pool, q, q_lens, kv_lens, table, type_, extra=2, cache=Form(pool, starts=starts, lens=prefixes, max_prefix=400))
     check(pool, q, q_lens, kv_lens, table, got, type_, chunk=True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("what", [60000.0, np.nan, np.inf])
+def test_slots_that_no_sequence_of_the_group_has(fmt, type_, what):
+    """The prefix is said to be longer than any of them: what the tables' pages hold behind their slots takes no part,
+    nor accuracy from what is seen."""
+    rng = np.random.default_rng(3)
+    q_lens, kv_lens, starts, prefixes = (1, 1, 9, 30, 1), (250, 300, 310, 333, 900), [0, 4], [512]
+    pool, table = grouped(fmt, 2, 16, kv_lens, starts, prefixes, rng)
+    spare = np.setdiff1d(np.arange(pool.n_pages), np.concatenate([table[s, :-(-n // 16)] for s, n in enumerate(kv_lens)]))
+    for s, n in enumerate(kv_lens):
+        table[s, -(-n // 16):] = rng.choice(spare)
+    for i in range(2):
+        if pool.q8:
+            pool.data[i][spare], pool.scales[i][spare] = 127, what
+        else:
+            pool.data[i][spare] = what
+    q = rng.standard_normal((sum(q_lens), 4, D)).astype(NP[type_])
+    got = run_attention(pool, q, q_lens, kv_lens, table, type_, cache=Form(pool, starts=starts, lens=prefixes, max_prefix=512))
+    check(pool, q, q_lens, kv_lens, table, got, type_, chunk=True)
